@@ -11,3 +11,6 @@ from .w4a4 import (  # noqa: F401
     mul_mat, mul_mat_fused, fused_workspace_bytes, hadamard, quantize_act, RqError, SharedActivation,
     pack, pack_groups, set_clip, set_rot_len, dequantize_rows, quantize_weights, dequantize,
 )
+from .mx import (  # noqa: F401
+    MXWeight, mx_quantize, mx_dequantize, mx_mul_mat, route, expert_ffn, expert_workspace_bytes,
+)

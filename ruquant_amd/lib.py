@@ -84,6 +84,21 @@ PROTOTYPES = {
                                             ctypes.c_void_p]),
 }
 
+# include/rq_mx4.h
+_int, _i64, _ptr, _size = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+PROTOTYPES.update({
+    "rq_mx4_quantize": (_int, [_int, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr]),
+    "rq_mx4_dequantize": (_int, [_int, _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr]),
+    "rq_mx4_prepared_bytes": (_size, [_i64, _i64, _i64]),
+    "rq_mx4_prepare": (_int, [_ptr, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr]),
+    "rq_mx4_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "rq_mx4_mul_mat": (_int, [_ptr, _i64, _i64, _int, _ptr, _i64, _i64, _int, _ptr, _i64, _ptr, _size, _ptr]),
+    "rq_route": (_int, [_int, _ptr, _i64, _i64, _i64, _int, _ptr, _int, _int, _int, _int, ctypes.c_float, _ptr, _ptr, _ptr]),
+    "rq_mx4_experts_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _int]),
+    "rq_mx4_experts": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _int, _ptr, _i64, _i64, _ptr, _ptr, _int, _int, _ptr, _i64,
+                              _ptr, _size, _ptr]),
+})
+
 for _name in ("rq_w4a4_mul_mat", "rq_w4a4_mul_mat_fused"):
     PROTOTYPES[_name + "_once"] = PROTOTYPES[_name]   # the same arguments
 
