@@ -16,19 +16,24 @@ typedef int   v4i __attribute__((ext_vector_type(4)));
 typedef int   v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
 inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // ---------------------------------------------------------------------------------------------------
-// One MFMA (16x16x128, both operands fp4) takes from lane l of its first operand row l % 16 and inputs 32 (l / 16) .. + 31 of
-// a run of 128 inputs: one block, 16 bytes of codes and one scale. A "step" below is such a run of 128, a "chunk" four steps.
+// One MFMA (32x32x64, both operands fp4) takes from lane l of its first operand row l % 32 and inputs 32 (l / 32) .. + 31 of a run
+// of 64 inputs: one block, 16 bytes of codes and one scale; the second operand's columns likewise. Lane l holds of the 32 x 32
+// result column l % 32 and rows 8 (i / 4) + 4 (l / 32) + i % 4, i = 0 .. 15. (Over the chip this form reaches 7.6 PFLOP/s from one
+// wavefront per SIMD, the 16x16x128 form with scales 4.7.) A "step" below is 128 inputs, two such runs, a "chunk" four steps.
 //
 // Prepared weight: per expert
-//   codes : N / 16 row blocks x K / 128 steps x 64 lanes x 16 bytes (N padded to 64, K to 128, zeros): a wavefront reads a
-//           fragment as 1 KiB of consecutive bytes, and a row block's steps follow one another.
-//   scales: N / 16 row blocks x K / 512 chunks x 64 lanes x 4 bytes, the lane's scales of the chunk's four steps.
-// Activations (workspace): rows of K / 2 bytes (K padded to 256: whole 128-byte lines), and per row and chunk 4 x 4 bytes of
-//   scales, [block of a step][step]: the four bytes that a lane needs of a chunk are one word here too.
+//   codes : N / 32 row blocks x K / 64 runs x 64 lanes x 16 bytes (N padded to 64, K to 128, zeros): a wavefront reads a fragment
+//           as 1 KiB of consecutive bytes, and a row block's runs follow one another.
+//   scales: N / 32 row blocks x K / 256 x 64 lanes x 4 bytes (K padded to 512), the lane's scales of four runs.
+// Activations (workspace), in one of two forms:
+//   panels: as a weight of so many rows (the tiled product: its loads are whole runs of 1 KiB);
+//   rows  : rows of K / 2 bytes (K padded to 256: whole 128-byte lines), and per row and 256 inputs 2 x 4 bytes of scales, [block of
+//           a run][run]: the four bytes that a lane needs are one word here too (the skinny product: few rows are read, in any order).
 // ---------------------------------------------------------------------------------------------------
 struct WeightLayout {
     int64_t N, K;
@@ -39,13 +44,19 @@ inline WeightLayout weight_layout(int64_t N, int64_t K) {
     WeightLayout L;
     L.N = N;
     L.K = K;
-    L.row_blocks = (int) (up_to(N, 64) / 16);
+    L.row_blocks = (int) (up_to(N, 64) / 32);
     L.steps = (int) (up_to(K, 128) / 128);
     L.chunks = (int) (up_to(K, 512) / 512);
-    L.code_bytes = (int64_t) L.row_blocks * L.steps * 1024;
-    L.expert_bytes = L.code_bytes + (int64_t) L.row_blocks * L.chunks * 256;
+    L.code_bytes = (int64_t) L.row_blocks * L.steps * 2048;
+    L.expert_bytes = L.code_bytes + (int64_t) L.row_blocks * L.chunks * 512;
     return L;
 }
+// place of block b's scale of a row in the row block's scales of the panel form
+__host__ __device__ __forceinline__ int64_t panel_scale_at(int row, int64_t b) {
+    return (b >> 3) * 256 + ((b & 1) * 32 + row) * 4 + ((b >> 1) & 3);
+}
+// place of block b's scale in a row of activations (row form)
+__host__ __device__ __forceinline__ int64_t act_scale_at(int64_t b) { return (b >> 3) * 8 + (b & 1) * 4 + ((b >> 1) & 3); }
 
 struct ActLayout {
     int64_t code_stride, scale_stride;   // bytes per row
@@ -95,16 +106,22 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8], float down) {
     return u;
 }
 
-__device__ __forceinline__ v4f mfma(const v4i &a, const v4i &b, const v4f &c, int sa, int sb) {
+// the product of a run of 64 inputs; J: which byte of the scales' words is this run's
+template <int J>
+__device__ __forceinline__ v16f mfma(const v4i &a, const v4i &b, const v16f &c, int sa, int sb) {
     const v8i A = { a[0], a[1], a[2], a[3], 0, 0, 0, 0 };
     const v8i B = { b[0], b[1], b[2], b[3], 0, 0, 0, 0 };
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, J, sa, J, sb);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
-// x -> activations in the workspace's form (rows m of `codes` / `scales`)
+// x -> activations in row form
 hipError_t launch_act_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, uint8_t *scales,
                                hipStream_t stream);
+// x -> activations in panel form: row r of the panels is row row_of[r] of x (none if negative), or row r if row_of is null. *rows
+// (on the device; null: L.N) of them are looked at. What the panels hold behind the last row is left as it is.
+hipError_t launch_panel_quantize(int dtype, const void *x, int64_t ldx, const WeightLayout &L, const int *row_of, const int *rows,
+                                 uint8_t *panels, hipStream_t stream);
 
 // How a product's tokens are cut into tiles. A plain product has one segment of M tokens; the experts' products have one
 // per expert, and the device knows how long they are.
@@ -117,43 +134,110 @@ enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 struct ProductArgs {
     WeightLayout   L;
     const uint8_t *w, *w2;          // prepared weights; kGateUp: w the gate, w2 the up projection
-    const uint8_t *a_codes, *a_scales;
+    const uint8_t *a_codes, *a_scales;   // rows; panels: both behind a_codes
     ActLayout      A;
+    WeightLayout   P;                    // of the panels
     int64_t        M;               // tokens (kDense)
     const Tile    *tiles;           // kGateUp, kDown: the tiles, on the device
     const int     *n_tiles;         //   and how many there are
     int            most_tiles;      //   at most
-    const int     *row_of;          // kGateUp: position -> row of the activations; kDown: position -> row of the output
+    const int     *row_of;          // position -> row: kGateUp of the activations (row form), kDown of the output
     int            out_dtype;
     void          *y;               // kDense: the result; kDown: fp32 rows of the slots
     int64_t        ldy;
-    uint8_t       *h_codes, *h_scales;   // kGateUp: activations of the down projection, rows by position
+    uint8_t       *h_codes, *h_scales;   // kGateUp: activations of the down projection by position, in the form that it reads
     ActLayout      H;
+    WeightLayout   HP;
 };
-// The scale of block b of row p of the feed-forward's h. Behind the last block that the rows of h have (their padding to 64), the
-// step's remaining scales are set too: the down projection multiplies them by zero codes, and a NaN would show.
-__device__ __forceinline__ void store_h_scale(const ProductArgs &a, int64_t p, int b, int X) {
-    uint8_t *to = a.h_scales + p * a.H.scale_stride + (b >> 4) * 16;
-    to[(b & 3) * 4 + ((b >> 2) & 3)] = (uint8_t) X;
-    if (b == a.L.row_blocks / 2 - 1) {
-        for (int c = b + 1; c & 3; ++c) to[(c & 3) * 4 + ((c >> 2) & 3)] = 0;
+// Four consecutive outputs n .. n + 3 of a row (`base` elements in), those in front of N.
+__device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int64_t n, int64_t N, const v4f &v) {
+    const int64_t at = base + n;
+    if (n + 3 < N && (at & 3) == 0 && ((uintptr_t) y & 15) == 0) {
+        if (dtype == RQ_F32) {
+            *reinterpret_cast<v4f *>(reinterpret_cast<float *>(y) + at) = v;
+        } else {
+            uint32_t w[2];
+            for (int i = 0; i < 2; ++i) {
+                const uint16_t lo = dtype == RQ_F16 ? __builtin_bit_cast(uint16_t, from_float<RQ_F16>(v[2 * i])) : bf16_bits(v[2 * i]);
+                const uint16_t hi = dtype == RQ_F16 ? __builtin_bit_cast(uint16_t, from_float<RQ_F16>(v[2 * i + 1])) : bf16_bits(v[2 * i + 1]);
+                w[i] = lo | (uint32_t) hi << 16;
+            }
+            *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(y) + at) = make_uint2(w[0], w[1]);
+        }
+        return;
+    }
+    for (int i = 0; i < 4; ++i) {
+        if (n + i >= N) break;
+        if (dtype == RQ_F32) reinterpret_cast<float *>(y)[at + i] = v[i];
+        else if (dtype == RQ_F16) reinterpret_cast<__half *>(y)[at + i] = from_float<RQ_F16>(v[i]);
+        else reinterpret_cast<__hip_bfloat16 *>(y)[at + i] = from_float<RQ_BF16>(v[i]);
     }
 }
-// few tokens per tile (up to 64; tile_tokens 16, 32 or 64): weights go from memory into registers
+// Block b (32 rows) of h = silu(gate) * up for the token in column lane % 32, from both lanes that hold it, as activations of the down
+// projection in row p. Behind the last block that the rows of h have (their padding to 64), the step's remaining scales are set
+// too: the down projection multiplies them by zero codes, and a NaN would show.
+template <bool PANELS>
+__device__ __forceinline__ void store_h(const ProductArgs &a, const v16f &gate, const v16f &up, int lane, bool there, int64_t p, int b) {
+    float    h[16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        h[i] = gate[i] / (1.0f + expf(-gate[i])) * up[i];
+        top = max(top, __float_as_uint(h[i]) & 0x7FFFFFFFu);
+    }
+    top = max(top, (uint32_t) __shfl_xor((int) top, 32));
+    const int X = block_scale(top);
+    uint32_t  c[2];   // rows 8 q + 4 (lane / 32) .. + 3 in half-word q
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = h[8 * q + i];
+        c[q] = X == 255 ? 0u : pack8(v, scale_down(X));
+    }
+    const uint32_t o[2] = { (uint32_t) __shfl_xor((int) c[0], 32), (uint32_t) __shfl_xor((int) c[1], 32) };
+    if (lane < 32 && there) {
+        const uint4 codes = make_uint4((c[0] & 0xFFFF) | o[0] << 16, c[0] >> 16 | (o[0] & 0xFFFF0000u), (c[1] & 0xFFFF) | o[1] << 16,
+                                       c[1] >> 16 | (o[1] & 0xFFFF0000u));
+        uint8_t *to;
+        if constexpr (PANELS) {
+            const int64_t block = p >> 5;
+            const int     row = (int) p & 31;
+            *reinterpret_cast<uint4 *>(a.h_codes + (block * a.HP.steps * 2 + (b >> 1)) * 1024 + ((b & 1) * 32 + row) * 16) = codes;
+            to = a.h_codes + a.HP.code_bytes + block * a.HP.chunks * 512;
+            to[panel_scale_at(row, b)] = (uint8_t) X;
+            if (b == a.L.row_blocks - 1) {
+                for (int k = b + 1; k & 3; ++k) to[panel_scale_at(row, k)] = 0;
+            }
+        } else {
+            *reinterpret_cast<uint4 *>(a.h_codes + p * a.H.code_stride + (int64_t) b * 16) = codes;
+            to = a.h_scales + p * a.H.scale_stride;
+            to[act_scale_at(b)] = (uint8_t) X;
+            if (b == a.L.row_blocks - 1) {
+                for (int k = b + 1; k & 3; ++k) to[act_scale_at(k)] = 0;
+            }
+        }
+    }
+}
+// few tokens per tile (tile_tokens 32 or 64): weights go from memory into registers
 hipError_t launch_skinny(int mode, const ProductArgs &a, int tile_tokens, hipStream_t stream);
 // many: both operands through LDS (tile_tokens 128)
 hipError_t launch_tiled(int mode, const ProductArgs &a, hipStream_t stream);
 constexpr int kTiledTokens = 128;
 
-// sorts the slots by expert and cuts them into tiles of tile_tokens positions
+// Sorts the slots by expert, every expert's from a multiple of 32 positions on, and cuts them into tiles of tile_tokens positions.
 struct SortArgs {
     const int32_t *ids;
     int            slots, top, E, tile_tokens;
-    int           *token_of, *slot_of;   // by position: token, slot
+    int           *token_of, *slot_of;   // by position: token, slot; token -1 where there is none
     Tile          *tiles;
-    int           *n_tiles;
+    int           *n_tiles;              // [0]: tiles, [1]: positions
 };
 hipError_t launch_sort(const SortArgs &a, hipStream_t stream);
+inline int64_t most_positions(int64_t slots, int64_t E) {
+    const int64_t some = slots < E ? slots : E;
+    return up_to(slots + 31 * some, 32);
+}
 inline int64_t most_tiles(int64_t slots, int64_t E, int tile_tokens) {
     const int64_t some = slots < E ? slots : E;
     return some + slots / tile_tokens;

@@ -16,16 +16,22 @@ constexpr int64_t kMaxTokens = 1 << 22;   // rows of a call; slots of an experts
 constexpr int kSkinnyTokens = 64;
 
 struct ExpertsPlan {
-    int     tile_tokens;   // 16, 32, 64: skinny; 128: tiled
-    int64_t slots, tiles;
-    size_t  x_codes, x_scales, h_codes, h_scales, rows, token_of, slot_of, tile_table, n_tiles, total;   // offsets
+    int     tile_tokens;   // 32, 64: skinny; 128: tiled
+    bool    panels;        // activations in panel form: by position, as the tiled product reads them
+    int64_t slots, positions, tiles;
+    WeightLayout XP, HP;
+    size_t  x, x_scales, h, h_scales, rows, token_of, slot_of, tile_table, n_tiles, total;   // offsets
 };
 ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top) {
     ExpertsPlan p;
     p.slots = M * top;
     const double per = (double) p.slots / (double) E;   // of an expert, on average
-    p.tile_tokens = per <= 8 ? 16 : per <= 16 ? 32 : per <= 40 ? 64 : 128;
+    p.tile_tokens = per <= 16 ? 32 : per <= 40 ? 64 : 128;
+    p.panels = p.tile_tokens > kSkinnyTokens;
     p.tiles = most_tiles(p.slots, E, p.tile_tokens);
+    p.positions = most_positions(p.slots, E);
+    p.XP = weight_layout(p.positions, K);
+    p.HP = weight_layout(p.positions, F);
     const ActLayout X = act_layout(K), H = act_layout(F);
     size_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -33,15 +39,15 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
         at += (size_t) pad256(bytes);
         return here;
     };
-    p.x_codes = take(M * X.code_stride);
-    p.x_scales = take(M * X.scale_stride);
-    p.h_codes = take(p.slots * H.code_stride);
-    p.h_scales = take(p.slots * H.scale_stride);
+    p.x = take(p.panels ? p.XP.expert_bytes : M * X.code_stride);
+    p.x_scales = take(p.panels ? 0 : M * X.scale_stride);
+    p.h = take(p.panels ? p.HP.expert_bytes : p.positions * H.code_stride);
+    p.h_scales = take(p.panels ? 0 : p.positions * H.scale_stride);
     p.rows = take(p.slots * N * 4);
-    p.token_of = take(p.slots * 4);
-    p.slot_of = take(p.slots * 4);
+    p.token_of = take(p.positions * 4);
+    p.slot_of = take(p.positions * 4);
     p.tile_table = take(p.tiles * (int64_t) sizeof(Tile));
-    p.n_tiles = take(4);
+    p.n_tiles = take(8);
     p.total = at;
     return p;
 }
@@ -55,7 +61,7 @@ bool good_experts(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top
 extern "C" size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M) {
     if (rq_mx4_prepared_bytes(1, N, K) == 0 || M < 0 || M > kMaxTokens) return 0;
     const ActLayout A = act_layout(K);
-    return (size_t) (pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
+    return (size_t) (M > kSkinnyTokens ? weight_layout(M, K).expert_bytes : pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
 }
 
 extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in_dtype, const void *x, int64_t ldx, int64_t M,
@@ -80,10 +86,13 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
     a.out_dtype = out_dtype;
     a.y = y;
     a.ldy = ldy;
-    const hipError_t e = launch_act_quantize(in_dtype, x, ldx, M, K, codes, scales, st);
-    if (e != hipSuccess) return e;
-    if (M <= kSkinnyTokens) return launch_skinny(kDense, a, M <= 16 ? 16 : M <= 32 ? 32 : 64, st);
-    return launch_tiled(kDense, a, st);
+    if (M <= kSkinnyTokens) {
+        const hipError_t e = launch_act_quantize(in_dtype, x, ldx, M, K, codes, scales, st);
+        return e != hipSuccess ? e : launch_skinny(kDense, a, M <= 32 ? 32 : 64, st);
+    }
+    a.P = weight_layout(M, K);
+    const hipError_t e = launch_panel_quantize(in_dtype, x, ldx, a.P, nullptr, nullptr, codes, st);
+    return e != hipSuccess ? e : launch_tiled(kDense, a, st);
 }
 
 extern "C" int rq_route(int dtype, const void *logits, int64_t ldl, int64_t M, int64_t E, int scoring, const float *bias, int groups,
@@ -132,33 +141,38 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     s.tiles = (Tile *) (ws + p.tile_table);
     s.n_tiles = (int *) (ws + p.n_tiles);
     hipError_t e = launch_sort(s, st);
-    if (e == hipSuccess) e = launch_act_quantize(in_dtype, x, ldx, M, K, ws + p.x_codes, ws + p.x_scales, st);
+    if (e == hipSuccess) {
+        e = p.panels ? launch_panel_quantize(in_dtype, x, ldx, p.XP, s.token_of, s.n_tiles + 1, ws + p.x, st)
+                     : launch_act_quantize(in_dtype, x, ldx, M, K, ws + p.x, ws + p.x_scales, st);
+    }
     ProductArgs a = {};
     a.L = weight_layout(F, K);
     a.A = act_layout(K);
     a.w = (const uint8_t *) gate;
     a.w2 = (const uint8_t *) up;
-    a.a_codes = ws + p.x_codes;
+    a.a_codes = ws + p.x;
     a.a_scales = ws + p.x_scales;
     a.tiles = s.tiles;
     a.n_tiles = s.n_tiles;
     a.most_tiles = (int) p.tiles;
     a.row_of = s.token_of;
-    a.h_codes = ws + p.h_codes;
+    a.h_codes = ws + p.h;
     a.h_scales = ws + p.h_scales;
     a.H = act_layout(F);
-    const bool skinny = p.tile_tokens <= kSkinnyTokens;
-    if (e == hipSuccess) e = skinny ? launch_skinny(kGateUp, a, p.tile_tokens, st) : launch_tiled(kGateUp, a, st);
+    a.P = p.XP;
+    a.HP = p.HP;
+    if (e == hipSuccess) e = p.panels ? launch_tiled(kGateUp, a, st) : launch_skinny(kGateUp, a, p.tile_tokens, st);
     ProductArgs d = a;
     d.L = weight_layout(N, F);
     d.A = a.H;
+    d.P = p.HP;
     d.w = (const uint8_t *) down;
     d.a_codes = a.h_codes;
     d.a_scales = a.h_scales;
     d.row_of = s.slot_of;
     d.y = ws + p.rows;
     d.ldy = N;
-    if (e == hipSuccess) e = skinny ? launch_skinny(kDown, d, p.tile_tokens, st) : launch_tiled(kDown, d, st);
+    if (e == hipSuccess) e = p.panels ? launch_tiled(kDown, d, st) : launch_skinny(kDown, d, p.tile_tokens, st);
     if (e == hipSuccess) e = launch_combine((const float *) (ws + p.rows), N, ids, weights, M, top, (int) E, out_dtype, y, ldy, st);
     return e;
 }

@@ -60,9 +60,45 @@ __global__ __launch_bounds__(kThreads) void rq_mx_quantize_kernel(const typename
     if (!ACT || (int64_t) u * 4 < code_stride) *reinterpret_cast<uint32_t *>(codes + (int64_t) m * code_stride + (int64_t) u * 4) = c;
     if ((u & 3) == 0) {
         const uint32_t b = u >> 2;
-        const uint32_t at = ACT ? (b >> 4) * 16 + (b & 3) * 4 + ((b >> 2) & 3) : b;
-        scales[(int64_t) m * scale_stride + at] = (uint8_t) X;
+        scales[(int64_t) m * scale_stride + (ACT ? act_scale_at(b) : b)] = (uint8_t) X;
     }
+}
+
+// The panel form: a workgroup has 32 rows x 256 elements, eight threads a row and run of 64, so that a wavefront reads eight rows'
+// lines and writes two lines of codes; a thread's four scales are one word.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(kThreads) void rq_mx_panel_quantize_kernel(const typename Element<DT>::type *x, int64_t ldx, WeightLayout L,
+                                                                        const int *row_of, const int *rows, uint8_t *panels) {
+    const int     parts = 2 * L.chunks;
+    const int     block = blockIdx.x / parts, part = blockIdx.x - block * parts;
+    const int     row = threadIdx.x >> 3, u = threadIdx.x & 7;
+    const int64_t r = (int64_t) block * 32 + row;
+    if ((int64_t) block * 32 >= (rows ? *rows : L.N)) return;
+    const int64_t m = r < L.N ? row_of ? row_of[r] : r : -1;
+    if (m < 0) return;   // (all eight threads of a row)
+    uint8_t *codes = panels + ((int64_t) block * L.steps * 2 + part * 4) * 1024 + ((u >> 2) * 32 + row) * 16 + (u & 3) * 4;
+    uint32_t word = 0;
+    float    v[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t k = (int64_t) part * 256 + j * 64 + u * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = 0;
+        if (k < L.K) load8<DT, VEC>(x + m * ldx + k, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
+        top = max(top, (uint32_t) __shfl_xor((int) top, 1));
+        top = max(top, (uint32_t) __shfl_xor((int) top, 2));
+        const int X = block_scale(top);
+        if (part * 4 + j < 2 * L.steps) *reinterpret_cast<uint32_t *>(codes + j * 1024) = X == 255 ? 0u : pack8(v[j], scale_down(X));
+        word |= (uint32_t) X << (8 * j);
+    }
+    if ((u & 3) == 0)
+        reinterpret_cast<uint32_t *>(panels + L.code_bytes + ((int64_t) block * parts + part) * 256)[(u >> 2) * 32 + row] = word;
 }
 
 template <int DT, bool VEC>
@@ -106,24 +142,24 @@ __global__ __launch_bounds__(kThreads) void rq_mx_prepare_kernel(const uint8_t *
                                                                  uint8_t *prepared) {
     const int64_t e = (int64_t) blockIdx.z * gridDim.y + blockIdx.y;
     if (e >= E) return;
-    const int64_t pieces = L.code_bytes / 16, words = (int64_t) L.row_blocks * L.chunks * 64;
+    const int64_t pieces = L.code_bytes / 16, words = (int64_t) L.row_blocks * L.chunks * 128;
     const uint8_t *c = codes + e * L.N * (L.K / 2), *s = scales + e * L.N * (L.K / 32);
     uint8_t       *to = prepared + e * L.expert_bytes;
     for (int64_t i = (int64_t) blockIdx.x * kThreads + threadIdx.x; i < pieces + words; i += (int64_t) gridDim.x * kThreads) {
         const int lane = (int) (i < pieces ? i : i - pieces) & 63;
         if (i < pieces) {
-            const int64_t block = (i >> 6) / L.steps, step = (i >> 6) - block * L.steps;
-            const int64_t row = block * 16 + (lane & 15), k = step * 128 + (lane >> 4) * 32;
+            const int64_t block = (i >> 6) / (2 * L.steps), run = (i >> 6) - block * 2 * L.steps;
+            const int64_t row = block * 32 + (lane & 31), k = run * 64 + (lane >> 5) * 32;
             uint4         v = make_uint4(0, 0, 0, 0);
             if (row < L.N && k < L.K) v = *reinterpret_cast<const uint4 *>(c + row * (L.K / 2) + k / 2);
             reinterpret_cast<uint4 *>(to)[i] = v;
         } else {
             const int64_t w = (i - pieces) >> 6;
-            const int64_t block = w / L.chunks, chunk = w - block * L.chunks;
-            const int64_t row = block * 16 + (lane & 15);
+            const int64_t block = w / (2 * L.chunks), part = w - block * 2 * L.chunks;   // (of 256 inputs)
+            const int64_t row = block * 32 + (lane & 31);
             uint32_t      v = 0;
             for (int j = 0; j < 4; ++j) {
-                const int64_t b = chunk * 16 + j * 4 + (lane >> 4);
+                const int64_t b = part * 8 + j * 2 + (lane >> 5);
                 v |= (row < L.N && b < L.K / 32 ? (uint32_t) s[row * (L.K / 32) + b] : 127u) << (8 * j);
             }
             reinterpret_cast<uint32_t *>(to + L.code_bytes)[i - pieces] = v;
@@ -158,6 +194,18 @@ hipError_t quantize(const void *x_, int64_t ldx, int64_t M, int64_t K, uint8_t *
 }
 
 template <int DT>
+hipError_t panel_quantize(const void *x_, int64_t ldx, const WeightLayout &L, const int *row_of, const int *rows, uint8_t *panels,
+                          hipStream_t stream) {
+    using T = typename Element<DT>::type;
+    const T   *x = reinterpret_cast<const T *>(x_);
+    const bool vec = (uintptr_t) x % 16 == 0 && ldx * (int64_t) sizeof(T) % 16 == 0;
+    const dim3 grid((unsigned) ((L.N + 31) / 32 * 2 * L.chunks));
+    if (vec) hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, true>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels);
+    else hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, false>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels);
+    return hipGetLastError();
+}
+
+template <int DT>
 hipError_t dequantize(const uint8_t *codes, const uint8_t *scales, int64_t M, int64_t K, void *out_, int64_t ldo, hipStream_t stream) {
     using T = typename Element<DT>::type;
     T            *out = reinterpret_cast<T *>(out_);
@@ -188,6 +236,13 @@ hipError_t launch_act_quantize(int dtype, const void *x, int64_t ldx, int64_t M,
     if (dtype == RQ_F32) return quantize<RQ_F32, true>(x, ldx, M, K, codes, scales, A.code_stride, A.scale_stride, per_row, stream);
     if (dtype == RQ_F16) return quantize<RQ_F16, true>(x, ldx, M, K, codes, scales, A.code_stride, A.scale_stride, per_row, stream);
     return quantize<RQ_BF16, true>(x, ldx, M, K, codes, scales, A.code_stride, A.scale_stride, per_row, stream);
+}
+
+hipError_t launch_panel_quantize(int dtype, const void *x, int64_t ldx, const WeightLayout &L, const int *row_of, const int *rows,
+                                 uint8_t *panels, hipStream_t stream) {
+    if (dtype == RQ_F32) return panel_quantize<RQ_F32>(x, ldx, L, row_of, rows, panels, stream);
+    if (dtype == RQ_F16) return panel_quantize<RQ_F16>(x, ldx, L, row_of, rows, panels, stream);
+    return panel_quantize<RQ_BF16>(x, ldx, L, row_of, rows, panels, stream);
 }
 
 }  // namespace mx

@@ -1,7 +1,7 @@
 // MXFP4 product for few tokens per weight: the weights stream from memory into registers, once.
 //
-// A workgroup owns some row blocks of 16 rows, its wavefronts split the inputs, and their partial sums are joined through LDS in
-// the wavefronts' order. The weight fragment is the MFMA's first operand, the tokens are its 16 columns.
+// A workgroup owns RB blocks of 32 rows (kGateUp: of each projection), its wavefronts split the inputs, and their partial sums are
+// joined through LDS in the wavefronts' order. The weight fragment is the MFMA's first operand, the tokens are its 32 columns.
 #include "rq_mx.h"
 
 namespace rq {
@@ -12,11 +12,10 @@ constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kDepth = 4;   // steps in flight per wavefront
 
-// RB row blocks (kGateUp: RB of each projection), TB blocks of 16 tokens
 template <int MODE, int RB, int TB>
 __global__ __launch_bounds__(kThreads) void rq_mx_skinny_kernel(const ProductArgs a) {
     constexpr int kMat = MODE == kGateUp ? 2 : 1;
-    constexpr int T = 16 * TB;
+    constexpr int T = 32 * TB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Tile tile = { 0, 0, 0, 0 };
     if constexpr (MODE == kDense) {
@@ -27,31 +26,37 @@ __global__ __launch_bounds__(kThreads) void rq_mx_skinny_kernel(const ProductArg
         tile = a.tiles[blockIdx.y];
     }
     const int      block0 = blockIdx.x * RB;
-    const uint8_t *w[kMat];
-    w[0] = a.w + (int64_t) tile.expert * a.L.expert_bytes;
-    if constexpr (kMat == 2) w[1] = a.w2 + (int64_t) tile.expert * a.L.expert_bytes;
-
-    // this lane's token in each block of 16, as a row of the activations (a token past the count repeats the last one)
+    const uint8_t *w[kMat][RB], *ws[kMat][RB];
+#pragma unroll
+    for (int m = 0; m < kMat; ++m) {
+        const uint8_t *base = (m ? a.w2 : a.w) + (int64_t) tile.expert * a.L.expert_bytes;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            w[m][r] = base + (int64_t) (block0 + r) * a.L.steps * 2048 + lane * 16;
+            ws[m][r] = base + a.L.code_bytes + (int64_t) (block0 + r) * a.L.chunks * 512 + lane * 4;
+        }
+    }
+    // this lane's token in each block of 32, as a row of the activations (a token past the count repeats the last one)
     const uint8_t *act[TB], *act_s[TB];
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
-        const int p = tile.first + min(t * 16 + (lane & 15), tile.count - 1);
+        const int     p = tile.first + min(t * 32 + (lane & 31), tile.count - 1);
         const int64_t row = MODE == kGateUp ? a.row_of[p] : p;
-        act[t] = a.a_codes + row * a.A.code_stride + (lane >> 4) * 16;
-        act_s[t] = a.a_scales + row * a.A.scale_stride + (lane >> 4) * 4;
+        act[t] = a.a_codes + row * a.A.code_stride + (lane >> 5) * 16;
+        act_s[t] = a.a_scales + row * a.A.scale_stride + (lane >> 5) * 4;
     }
     const int s0 = (int) ((int64_t) a.L.steps * wave / kWaves), s1 = (int) ((int64_t) a.L.steps * (wave + 1) / kWaves);
 
-    v4f acc[kMat][RB][TB];
+    v16f acc[kMat][RB][TB];
 #pragma unroll
     for (int m = 0; m < kMat; ++m)
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) acc[m][r][t] = v4f{ 0, 0, 0, 0 };
+            for (int t = 0; t < TB; ++t) acc[m][r][t] = v16f{ 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 };
 
     struct Frag {
-        v4i A[kMat][RB], B[TB];
+        v4i A[kMat][RB][2], B[TB][2];
         int sa[kMat][RB], sb[TB];
     };
     auto load = [&](Frag &f, int s) __attribute__((always_inline)) {
@@ -59,24 +64,31 @@ __global__ __launch_bounds__(kThreads) void rq_mx_skinny_kernel(const ProductArg
         for (int m = 0; m < kMat; ++m) {
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
-                const int64_t b = block0 + r;
-                f.A[m][r] = reinterpret_cast<const v4i *>(w[m] + (b * a.L.steps + s) * 1024)[lane];
-                f.sa[m][r] = reinterpret_cast<const int *>(w[m] + a.L.code_bytes + (b * a.L.chunks + (s >> 2)) * 256)[lane] >> (8 * (s & 3));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) f.A[m][r][h] = *reinterpret_cast<const v4i *>(w[m][r] + (int64_t) s * 2048 + h * 1024);
+                f.sa[m][r] = *reinterpret_cast<const int *>(ws[m][r] + (s >> 1) * 256);
             }
         }
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            f.B[t] = *reinterpret_cast<const v4i *>(act[t] + (int64_t) s * 64);
-            f.sb[t] = *reinterpret_cast<const int *>(act_s[t] + (s >> 2) * 16) >> (8 * (s & 3));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) f.B[t][h] = *reinterpret_cast<const v4i *>(act[t] + (int64_t) s * 64 + h * 32);
+            f.sb[t] = *reinterpret_cast<const int *>(act_s[t] + (s >> 1) * 8);
         }
     };
-    auto multiply = [&](const Frag &f) __attribute__((always_inline)) {
+    auto multiply = [&](const Frag &f, int s) __attribute__((always_inline)) {
+        const int by = (s & 1) * 16;
 #pragma unroll
         for (int m = 0; m < kMat; ++m)
 #pragma unroll
-            for (int r = 0; r < RB; ++r)
+            for (int r = 0; r < RB; ++r) {
+                const int sa = f.sa[m][r] >> by;
 #pragma unroll
-                for (int t = 0; t < TB; ++t) acc[m][r][t] = mfma(f.A[m][r], f.B[t], acc[m][r][t], f.sa[m][r], f.sb[t]);
+                for (int t = 0; t < TB; ++t) {
+                    acc[m][r][t] = mfma<0>(f.A[m][r][0], f.B[t][0], acc[m][r][t], sa, f.sb[t] >> by);
+                    acc[m][r][t] = mfma<1>(f.A[m][r][1], f.B[t][1], acc[m][r][t], sa, f.sb[t] >> by);
+                }
+            }
     };
     Frag ring[kDepth];
 #pragma unroll
@@ -86,95 +98,77 @@ __global__ __launch_bounds__(kThreads) void rq_mx_skinny_kernel(const ProductArg
 #pragma unroll
         for (int i = 0; i < kDepth; ++i) {
             if (s + i < s1) {
-                multiply(ring[i]);
+                multiply(ring[i], s + i);
                 if (s + i + kDepth < s1) load(ring[i], s + i + kDepth);
             }
         }
     }
 
-    // join: [wave][matrix][row block][token block][lane] of four floats, rows (lane / 16) * 4 + i, token lane % 16
-    constexpr int kCells = kMat * RB * TB * 64;
-    __shared__ v4f part[kWaves][kCells];
+    // join: [wave][matrix, row block, token block][quad][lane] of four floats: rows 8 quad + 4 (lane / 32) + i, token lane % 32
+    constexpr int kCells = kMat * RB * TB * 256;
+    extern __shared__ __attribute__((aligned(16))) v4f part[];
 #pragma unroll
     for (int m = 0; m < kMat; ++m)
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) part[wave][((m * RB + r) * TB + t) * 64 + lane] = acc[m][r][t];
+            for (int t = 0; t < TB; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const v16f &c = acc[m][r][t];
+                    part[wave * kCells + (((m * RB + r) * TB + t) * 4 + q) * 64 + lane] = v4f{ c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3] };
+                }
     __syncthreads();
     for (int c = threadIdx.x; c < kCells; c += kThreads) {
-        v4f sum = part[0][c];
+        v4f sum = part[c];
 #pragma unroll
-        for (int v = 1; v < kWaves; ++v) sum += part[v][c];
+        for (int v = 1; v < kWaves; ++v) sum += part[v * kCells + c];
         if constexpr (MODE == kGateUp) {
-            part[0][c] = sum;
+            part[c] = sum;
         } else {
-            const int l = c & 63, t = (c >> 6) % TB, r = (c >> 6) / TB;
-            const int token = t * 16 + (l & 15);
-            const int64_t n = (int64_t) (block0 + r) * 16 + (l >> 4) * 4;
+            const int l = c & 63, q = (c >> 6) & 3, t = (c >> 8) % TB, r = (c >> 8) / TB;
+            const int token = t * 32 + (l & 31);
             if (token < tile.count) {
                 const int64_t row = MODE == kDown ? a.row_of[tile.first + token] : tile.first + token;
-                for (int i = 0; i < 4; ++i) {
-                    if (n + i >= a.L.N) break;
-                    if (MODE == kDown || a.out_dtype == RQ_F32) reinterpret_cast<float *>(a.y)[row * a.ldy + n + i] = sum[i];
-                    else if (a.out_dtype == RQ_F16) reinterpret_cast<__half *>(a.y)[row * a.ldy + n + i] = from_float<RQ_F16>(sum[i]);
-                    else reinterpret_cast<__hip_bfloat16 *>(a.y)[row * a.ldy + n + i] = from_float<RQ_BF16>(sum[i]);
-                }
+                store_out(MODE == kDown ? RQ_F32 : a.out_dtype, a.y, row * a.ldy, (int64_t) (block0 + r) * 32 + q * 8 + (l >> 5) * 4, a.L.N, sum);
             }
         }
     }
     if constexpr (MODE == kGateUp) {
-        // h = silu(gate) * up, and its blocks of 32 rows (two row blocks) as activations of the down projection
         __syncthreads();
-        for (int c = threadIdx.x; c < RB / 2 * T; c += kThreads) {
-            const int token = c % T, pair = c / T;
-            if (token >= tile.count) continue;
-            float    h[32];
-            uint32_t top = 0;
-            for (int i = 0; i < 32; ++i) {
-                const int cell = ((pair * 2 + (i >> 4)) * TB + (token >> 4)) * 64 + ((i >> 2) & 3) * 16 + (token & 15);
-                const float g = part[0][cell][i & 3], u = part[0][RB * TB * 64 + cell][i & 3];
-                h[i] = g / (1.0f + expf(-g)) * u;
-                top = max(top, __float_as_uint(h[i]) & 0x7FFFFFFFu);
-            }
-            const int X = block_scale(top);
-            uint32_t  code[4];
+        if (wave < RB * TB) {
+            const int r = wave / TB, t = wave % TB;
+            v16f      gate, up;
+#pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float v[8];
-                for (int i = 0; i < 8; ++i) v[i] = h[8 * q + i];
-                code[q] = X == 255 ? 0u : pack8(v, scale_down(X));
+                const v4f x = part[((r * TB + t) * 4 + q) * 64 + lane], y = part[(((RB + r) * TB + t) * 4 + q) * 64 + lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gate[4 * q + i] = x[i], up[4 * q + i] = y[i];
             }
-            const int64_t p = tile.first + token;
-            const int     b = (block0 >> 1) + pair;   // block of the row of h
-            *reinterpret_cast<uint4 *>(a.h_codes + p * a.H.code_stride + b * 16) = make_uint4(code[0], code[1], code[2], code[3]);
-            store_h_scale(a, p, b, X);
+            const int token = t * 32 + (lane & 31);
+            store_h<false>(a, gate, up, lane, token < tile.count, tile.first + token, block0 + r);
         }
     }
 }
 
 template <int MODE, int RB, int TB>
 hipError_t launch(const ProductArgs &a, hipStream_t stream) {
-    const int64_t tiles = MODE == kDense ? (a.M + 16 * TB - 1) / (16 * TB) : a.most_tiles;
-    hipLaunchKernelGGL((rq_mx_skinny_kernel<MODE, RB, TB>), dim3(a.L.row_blocks / RB, (unsigned) tiles), dim3(kThreads), 0, stream, a);
+    constexpr int kBytes = kWaves * (MODE == kGateUp ? 2 : 1) * RB * TB * 4096;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(rq_mx_skinny_kernel<MODE, RB, TB>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (set != hipSuccess) return set;
+    const int64_t tiles = MODE == kDense ? (a.M + 32 * TB - 1) / (32 * TB) : a.most_tiles;
+    hipLaunchKernelGGL((rq_mx_skinny_kernel<MODE, RB, TB>), dim3(a.L.row_blocks / RB, (unsigned) tiles), dim3(kThreads), kBytes, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_skinny(int mode, const ProductArgs &a, int tile_tokens, hipStream_t stream) {
-    if (mode == kDense) {
-        if (tile_tokens == 16) return launch<kDense, 2, 1>(a, stream);
-        if (tile_tokens == 32) return launch<kDense, 2, 2>(a, stream);
-        return launch<kDense, 2, 4>(a, stream);
-    }
-    if (mode == kDown) {
-        if (tile_tokens == 16) return launch<kDown, 2, 1>(a, stream);
-        if (tile_tokens == 32) return launch<kDown, 2, 2>(a, stream);
-        return launch<kDown, 2, 4>(a, stream);
-    }
-    if (tile_tokens == 16) return launch<kGateUp, 2, 1>(a, stream);
-    if (tile_tokens == 32) return launch<kGateUp, 2, 2>(a, stream);
-    return launch<kGateUp, 2, 4>(a, stream);
+    const bool one = tile_tokens == 32;
+    if (mode == kDense) return one ? launch<kDense, 1, 1>(a, stream) : launch<kDense, 1, 2>(a, stream);
+    if (mode == kDown) return one ? launch<kDown, 1, 1>(a, stream) : launch<kDown, 1, 2>(a, stream);
+    return one ? launch<kGateUp, 1, 1>(a, stream) : launch<kGateUp, 1, 2>(a, stream);
 }
 
 }  // namespace mx

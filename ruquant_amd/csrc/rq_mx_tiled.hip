@@ -1,175 +1,299 @@
-// MXFP4 product for many tokens: tiles of 128 rows x 128 tokens, both operands through LDS.
+// MXFP4 product for many tokens: tiles of rows x tokens, both operands through LDS.
 #include "rq_mx.h"
 
 namespace rq {
 namespace mx {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTileRows = 128;
-constexpr int kTok = kTiledTokens;
-constexpr int kWeightBytes = kTileRows * 128;   // of a stage (256 inputs)
-constexpr int kStage = kWeightBytes + kTok * 128;
-
-__device__ __forceinline__ void to_lds(const uint8_t *from, uint8_t *to) {   // 16 bytes a lane, `to` + 16 * lane
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) from,
-                                     (__attribute__((address_space(3))) void *) to, 16, 0, 0);
+// 64 lanes x 16 bytes to 1 KiB of LDS at `lds` (wave-uniform; the hardware adds lane * 16). Assembly, so that the count of
+// outstanding loads is this file's (the waits of the steps); nothing is written to registers.
+__device__ __forceinline__ void load_run(const uint8_t *from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(__builtin_amdgcn_readfirstlane((int) lds)) : "memory", "m0");
+}
+__device__ __forceinline__ void load_run(const uint8_t *base, uint32_t lane_off, uint32_t lds) {   // base: wave-uniform
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(base), "s"(__builtin_amdgcn_readfirstlane((int) lds)) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier() {
+    asm volatile("s_barrier" : : : "memory");
+}
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+    const uint64_t b = (uint64_t) (uintptr_t) p;
+    return reinterpret_cast<const uint8_t *>(
+        (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) b) |
+                     (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (b >> 32)) << 32));
 }
 
-// Wavefront (wr, wc) of four has 64 rows x 64 tokens. kGateUp: 32 rows of each projection, so that a lane holds both of a row.
-template <int MODE>
-__global__ __launch_bounds__(kThreads) void rq_mx_tiled_kernel(const ProductArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStage];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1;
+// Wavefront (wr, wc) of 2 x WC has RB blocks of 32 rows x TB of 32 tokens. kGateUp: RB / 2 of each projection, so that a lane holds
+// both values of a row of h. R: slots of the ring of steps in LDS.
+template <int MODE, int RB, int TB, int WC, int R>
+struct Tiled {
+    static constexpr int kWaves = 2 * WC, kThreads = 64 * kWaves;
+    static constexpr int kABlocks = 2 * RB, kBBlocks = WC * TB;
+    static constexpr int kSlot = (kABlocks + kBBlocks) * 2048;   // one step of both operands
+    static constexpr int kScales = R * kSlot;                    // behind the ring: one chunk of their scales
+    static constexpr int kBytes = kScales + (kABlocks + kBBlocks) * 512;
+    // 1 KiB each, of a wavefront per step; runs of the scales per chunk (some are fetched twice so that all fetch as many)
+    static constexpr int kARuns = 2 * kABlocks / kWaves, kBRuns = 2 * kBBlocks / kWaves, kRuns = kARuns + kBRuns;
+    static constexpr int kScaleRuns = (kABlocks + kBBlocks) / 2, kScales1 = (kScaleRuns + kWaves - 1) / kWaves;
+    static_assert(2 * kABlocks % kWaves == 0 && 2 * kBBlocks % kWaves == 0 && kBBlocks % 2 == 0, "split of the loads");
+    static constexpr int kTileRows = MODE == kGateUp ? 32 * RB : 64 * RB;            // (of each matrix)
+    static constexpr int kTileTokens = 32 * WC * TB;
+
+    // what this wavefront moves
+    const uint8_t *a_src[kARuns], *b_src[kBRuns];   // wave-uniform
+    const uint8_t *s_src[kScales1];                 // the lane's
+    uint32_t       lds0, lane16;
+    int            wave, wr, wc, lane, steps;
+    const uint8_t *a_lds, *b_lds, *as_lds, *bs_lds;   // this lane's places in slot 0
+    v16f           acc[RB][TB];
+    v4i            A[RB][2];
+    int            sA[RB];
+
+    __device__ __forceinline__ void fetch_run(int t, int slot, int i) {
+        const uint32_t to = lds0 + slot * kSlot;
+        if (i < kARuns) load_run(a_src[i] + (int64_t) t * 2048, lane16, to + (wave * kARuns + i) * 1024);
+        else load_run(b_src[i - kARuns] + (int64_t) t * 2048, lane16, to + (2 * kABlocks + wave * kBRuns + i - kARuns) * 1024);
+    }
+    __device__ __forceinline__ void fetch_scales(int c) {
+#pragma unroll
+        for (int i = 0; i < kScales1; ++i) load_run(s_src[i] + (int64_t) c * 512, lds0 + kScales + (i * kWaves + wave) % kScaleRuns * 1024);
+    }
+    __device__ __forceinline__ void read_a(int slot, int i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) A[i][h] = *reinterpret_cast<const v4i *>(a_lds + slot * kSlot + (2 * i + h) * 1024);
+    }
+    __device__ __forceinline__ void read_b(v4i (&B)[TB][2], int slot, int i) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) B[i][h] = *reinterpret_cast<const v4i *>(b_lds + slot * kSlot + (2 * i + h) * 1024);
+    }
+    // the scales of inputs 256 half .. + 255 of the chunk in LDS
+    __device__ __forceinline__ void read_sa(int half, int i) { sA[i] = *reinterpret_cast<const int *>(as_lds + i * 512 + half * 256); }
+    __device__ __forceinline__ void read_sb(int (&sB)[TB], int half, int i) const {
+        sB[i] = *reinterpret_cast<const int *>(bs_lds + i * 512 + half * 256);
+    }
+
+    // Step t = 4 c + J: its products from A and B, behind each row block's the read of its fragments of step t + 1, between them the
+    // reads of step t + 1's activations into N and the fetch of step t + R - 1 into the slot of step t - 1 (whose reads the products
+    // of step t - 1 have waited for, in every wavefront that has passed this step's barrier). The scales are read every second
+    // step; those of the next chunk are fetched by the second step of a chunk, last of its loads, and read by the fourth. MORE: all
+    // of those steps exist.
+    template <int J, bool MORE>
+    __device__ __forceinline__ void step(int t, int slot, const v4i (&B)[TB][2], v4i (&N)[TB][2], int (&sB)[TB], int (&sN)[TB]) {
+        const int  next = slot + 1 == R ? 0 : slot + 1, last = slot == 0 ? R - 1 : slot - 1;
+        const bool get = MORE || t + R - 1 < steps;
+        // step t + 1 has arrived; those behind it need not have
+        if (MORE || t + R - 2 < steps) wait_loads<(R - 3) * kRuns + (MORE && J == 2 ? kScales1 : 0)>();
+        else wait_loads<0>();
+        barrier();
+        if (!MORE && get) {
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) fetch_run(t + R - 1, last, i);
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+#pragma unroll
+            for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1)>(A[r][0], B[b][0], acc[r][b], sA[r], sB[b]);
+            // (past the last step: what the ring holds, for nobody)
+#pragma unroll
+            for (int i = r * TB / RB; i < (r + 1) * TB / RB; ++i) {
+                read_b(N, next, i);
+                if (J & 1) read_sb(sN, J == 1, i);
+            }
+            if (MORE) {
+#pragma unroll
+                for (int i = r * kRuns / RB; i < (r + 1) * kRuns / RB; ++i) fetch_run(t + R - 1, last, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1) + 1>(A[r][1], B[b][1], acc[r][b], sA[r], sB[b]);
+            read_a(next, r);
+            if (J & 1) read_sa(J == 1, r);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (J & 1) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) sB[i] = sN[i];
+        }
+        if (J == 1 && (MORE || t + 3 < steps)) fetch_scales((t >> 2) + 1);
+    }
+
+    __device__ __forceinline__ void loop() {
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int t = 0; t < TB; ++t) acc[r][t] = v16f{ 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 };
+        fetch_scales(0);
+#pragma unroll
+        for (int t = 0; t < R - 1; ++t) {
+            if (t < steps) {
+#pragma unroll
+                for (int i = 0; i < kRuns; ++i) fetch_run(t, t, i);
+            }
+        }
+        if (steps >= R - 1) wait_loads<(R - 2) * kRuns>();
+        else wait_loads<0>();
+        barrier();
+        v4i B[TB][2], N[TB][2];
+        int sB[TB], sN[TB];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) read_a(0, i), read_sa(0, i);
+#pragma unroll
+        for (int i = 0; i < TB; ++i) read_b(B, 0, i), read_sb(sB, 0, i);
+        int  t = 0, slot = 0;
+        auto next = [&]() __attribute__((always_inline)) { ++t, slot = slot + 1 == R ? 0 : slot + 1; };
+        while (t + R + 2 < steps) {
+            step<0, true>(t, slot, B, N, sB, sN), next();
+            step<1, true>(t, slot, N, B, sB, sN), next();
+            step<2, true>(t, slot, B, N, sB, sN), next();
+            step<3, true>(t, slot, N, B, sB, sN), next();
+        }
+        while (true) {
+            step<0, false>(t, slot, B, N, sB, sN), next();
+            if (t >= steps) break;
+            step<1, false>(t, slot, N, B, sB, sN), next();
+            if (t >= steps) break;
+            step<2, false>(t, slot, B, N, sB, sN), next();
+            if (t >= steps) break;
+            step<3, false>(t, slot, N, B, sB, sN), next();
+            if (t >= steps) break;
+        }
+        wait_loads<0>();   // (none of this wavefront's loads lands in LDS behind this)
+    }
+};
+
+template <int MODE, int RB, int TB, int WC, int R>
+__global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void rq_mx_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles) {
+    using G = Tiled<MODE, RB, TB, WC, R>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    // Workgroups go to the XCDs in turn. Each XCD takes a run of the tiles in an order in which the token tiles run fastest, so that
+    // those that share rows of the weight share an L2.
+    const int total = row_tiles * token_tiles;
+    const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
+    const int v = xcd * each + min(xcd, more) + (int) (blockIdx.x >> 3);
+    const int row_tile = v / token_tiles, token_tile = v - row_tile * token_tiles;
     Tile tile = { 0, 0, 0, 0 };
     if constexpr (MODE == kDense) {
-        tile.first = blockIdx.y * kTok;
-        tile.count = (int) (a.M - tile.first < kTok ? a.M - tile.first : kTok);
+        tile.first = token_tile * G::kTileTokens;
+        tile.count = (int) (a.M - tile.first < G::kTileTokens ? a.M - tile.first : G::kTileTokens);
     } else {
-        if ((int) blockIdx.y >= *a.n_tiles) return;
-        tile = a.tiles[blockIdx.y];
+        if (token_tile >= *a.n_tiles) return;
+        tile = a.tiles[token_tile];
     }
-    constexpr int  kBlocks = MODE == kGateUp ? 4 : 8;   // row blocks of the tile, per matrix
-    const int      block0 = blockIdx.x * kBlocks;
+    G g;
+    g.lane = threadIdx.x & 63;
+    g.wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    g.wr = g.wave / WC;
+    g.wc = g.wave % WC;
+    g.lane16 = g.lane * 16;
+    g.steps = a.L.steps;
+    g.lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void *) lds;
+    g.a_lds = lds + g.wr * RB * 2048 + g.lane * 16;
+    g.b_lds = lds + (2 * G::kABlocks + g.wc * TB * 2) * 1024 + g.lane * 16;
+    g.as_lds = lds + G::kScales + g.wr * RB * 512 + g.lane * 4;
+    g.bs_lds = lds + G::kScales + (G::kABlocks + g.wc * TB) * 512 + g.lane * 4;
+    constexpr int  kBlocks = G::kTileRows / 32;   // row blocks of the tile, per matrix
+    const int      block0 = row_tile * kBlocks;
     const uint8_t *w = a.w + (int64_t) tile.expert * a.L.expert_bytes;
     const uint8_t *w2 = MODE == kGateUp ? a.w2 + (int64_t) tile.expert * a.L.expert_bytes : w;
-    // row block i (0 .. 7) of the tile: its matrix and place; blocks past the weight's repeat its last one
-    auto codes_of = [&](int i) __attribute__((always_inline)) {
-        const int b = MODE == kGateUp ? block0 + (i >> 2) * 2 + (i & 1) : block0 + i;
-        const uint8_t *base = MODE == kGateUp && (i & 2) ? w2 : w;
-        return base + (int64_t) min(b, a.L.row_blocks - 1) * a.L.steps * 1024;
+    // row block i of the tile, in the order of its wavefronts: its matrix and place; blocks past the weight's repeat its last one
+    auto place = [&](int i) __attribute__((always_inline)) {
+        const int b = MODE == kGateUp ? block0 + i / RB * (RB / 2) + i % RB % (RB / 2 > 0 ? RB / 2 : 1) : block0 + i;
+        return min(b, a.L.row_blocks - 1);
     };
-    auto scales_of = [&](int i) __attribute__((always_inline)) {
-        const int b = MODE == kGateUp ? block0 + (i >> 2) * 2 + (i & 1) : block0 + i;
-        const uint8_t *base = MODE == kGateUp && (i & 2) ? w2 : w;
-        return base + a.L.code_bytes + (int64_t) min(b, a.L.row_blocks - 1) * a.L.chunks * 256;
-    };
-    // what this lane moves: of weight blocks 2 wave and 2 wave + 1 both steps, of activation rows 32 wave .. + 31 a line each; a
-    // row's eight pieces lie in LDS in an order that its number turns, so that the reads below spread over the banks
-    const uint8_t *wsrc[2], *asrc[4];
+    auto matrix = [&](int i) __attribute__((always_inline)) { return MODE == kGateUp && i % RB >= RB / 2 ? w2 : w; };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) wsrc[i] = codes_of(2 * wave + i) + lane * 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int     r = wave * 32 + i * 8 + (lane >> 3);
-        const int     p = tile.first + min(r, tile.count - 1);
-        const int64_t row = MODE == kGateUp ? a.row_of[p] : p;
-        asrc[i] = a.a_codes + row * a.A.code_stride + (((lane & 7) ^ (r & 7)) * 16);
+    for (int i = 0; i < G::kARuns; ++i) {
+        const int run = g.wave * G::kARuns + i;
+        g.a_src[i] = uniform(matrix(run >> 1) + (int64_t) place(run >> 1) * a.L.steps * 2048 + (run & 1) * 1024);
     }
-    const uint8_t *ws[4], *as[4];
+    // the tile's token blocks; those past the last repeat it, and those past the activations the activations' last
+    const int token0 = tile.first >> 5, token_blocks = min((tile.count + 31) >> 5, a.P.row_blocks - token0);
+    auto token_place = [&](int i) __attribute__((always_inline)) { return token0 + min(i, token_blocks - 1); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        ws[i] = scales_of(wr * 4 + i) + lane * 4;
-        const int     p = tile.first + min(wc * 64 + i * 16 + (lane & 15), tile.count - 1);
-        const int64_t row = MODE == kGateUp ? a.row_of[p] : p;
-        as[i] = a.a_scales + row * a.A.scale_stride + (lane >> 4) * 4;
+    for (int i = 0; i < G::kBRuns; ++i) {
+        const int run = g.wave * G::kBRuns + i;
+        g.b_src[i] = uniform(a.a_codes + (int64_t) token_place(run >> 1) * a.P.steps * 2048 + (run & 1) * 1024);
     }
-    const int stages = (a.L.steps + 1) / 2;
-    auto fetch = [&](int st) __attribute__((always_inline)) {
-        uint8_t *to = lds + (st & 1) * kStage;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < G::kScales1; ++i) {   // of two row blocks, or of two token blocks
+        const int  run = (i * G::kWaves + g.wave) % G::kScaleRuns;
+        const bool rows = run < RB;
+        const int  r = 2 * run + (g.lane >> 5);
+        g.s_src[i] = (rows ? matrix(r) + a.L.code_bytes + (int64_t) place(r) * a.L.chunks * 512
+                           : a.a_codes + a.P.code_bytes + (int64_t) token_place(r - 2 * RB) * a.P.chunks * 512) + (g.lane & 31) * 16;
+    }
+    g.loop();
+    const int lane = g.lane, wr = g.wr, wc = g.wc;
+    if constexpr (MODE == kGateUp) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int s = min(2 * st + h, a.L.steps - 1);   // (an odd last step is fetched twice and used once)
-                to_lds(wsrc[i] + (int64_t) s * 1024, to + ((2 * wave + i) * 2 + h) * 1024);
+        for (int t = 0; t < TB; ++t) {
+            const int token = (wc * TB + t) * 32 + (lane & 31);
+#pragma unroll
+            for (int q = 0; q < RB / 2; ++q) {
+                const int b = block0 + wr * (RB / 2) + q;
+                if (b < a.L.row_blocks) store_h<true>(a, g.acc[q][t], g.acc[RB / 2 + q][t], lane, token < tile.count, tile.first + token, b);
             }
         }
+    } else {
+        // 32 tokens x 32 rows at a time through LDS (a region of the wavefront's own), so that a token's outputs leave as one run
+        constexpr int kStride = 36;
+        static_assert(G::kWaves * 32 * kStride * 4 <= G::kBytes, "a region per wavefront");
+        float *mine = reinterpret_cast<float *>(lds) + g.wave * 32 * kStride;
+        barrier();   // (the ring is not read any more)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to_lds(asrc[i] + (int64_t) st * 128, to + kWeightBytes + (wave * 4 + i) * 1024);
-    };
-    v4f acc[4][4];
+        for (int t = 0; t < TB; ++t) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < RB; ++r) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[r][t] = v4f{ 0, 0, 0, 0 };
-    fetch(0);
-    for (int st = 0; st < stages; ++st) {
-        __syncthreads();
-        if (st + 1 < stages) fetch(st + 1);
-        const uint8_t *from = lds + (st & 1) * kStage;
-        int sw[4], sa[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sw[i] = *reinterpret_cast<const int *>(ws[i] + (int64_t) (st >> 1) * 256) >> (16 * (st & 1));
-            sa[i] = *reinterpret_cast<const int *>(as[i] + (int64_t) (st >> 1) * 16) >> (16 * (st & 1));
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (2 * st + h >= a.L.steps) break;
-            v4i A[4], B[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                A[i] = reinterpret_cast<const v4i *>(from + ((wr * 4 + i) * 2 + h) * 1024)[lane];
-                const int r = wc * 64 + i * 16 + (lane & 15);
-                B[i] = *reinterpret_cast<const v4i *>(from + kWeightBytes + r * 128 + (((h * 4 + (lane >> 4)) ^ (r & 7)) * 16));
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[r][t] = mfma(A[r], B[t], acc[r][t], sw[r] >> (8 * h), sa[t] >> (8 * h));
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int  token = wc * 64 + t * 16 + (lane & 15);
-        const bool there = token < tile.count;
-        if constexpr (MODE == kGateUp) {
-            // rows 32 (2 blockIdx.x + wr) .. + 31: one block of h per token, of which this lane has two runs of four
-            float    h[2][4];
-            uint32_t top = 0;
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float g = acc[r][t][i], u = acc[r + 2][t][i];
-                    h[r][i] = g / (1.0f + expf(-g)) * u;
-                    top = max(top, __float_as_uint(h[r][i]) & 0x7FFFFFFFu);
+                for (int q = 0; q < 4; ++q) {
+                    const v4f v = { g.acc[r][t][4 * q], g.acc[r][t][4 * q + 1], g.acc[r][t][4 * q + 2], g.acc[r][t][4 * q + 3] };
+                    *reinterpret_cast<v4f *>(mine + (lane & 31) * kStride + q * 8 + (lane >> 5) * 4) = v;
                 }
-            top = max(top, (uint32_t) __shfl_xor((int) top, 16));
-            top = max(top, (uint32_t) __shfl_xor((int) top, 32));
-            const int X = block_scale(top);
-            float     v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = h[i >> 2][i & 3];
-            const uint32_t c = X == 255 ? 0u : pack8(v, scale_down(X));
-            const int      b = blockIdx.x * 2 + wr;
-            if (there && b < a.L.row_blocks / 2) {
-                const int64_t p = tile.first + token;
-                uint8_t      *to = a.h_codes + p * a.H.code_stride + b * 16 + (lane >> 4) * 2;
-                *reinterpret_cast<uint16_t *>(to) = (uint16_t) c;
-                *reinterpret_cast<uint16_t *>(to + 8) = (uint16_t) (c >> 16);
-                if (lane < 16) store_h_scale(a, p, b, X);
-            }
-        } else if (there) {
-            const int64_t row = MODE == kDown ? a.row_of[tile.first + token] : tile.first + token;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t n = (int64_t) (block0 + wr * 4 + r) * 16 + (lane >> 4) * 4;
+                __builtin_amdgcn_wave_barrier();
                 for (int i = 0; i < 4; ++i) {
-                    if (n + i >= a.L.N) break;
-                    if (MODE == kDown || a.out_dtype == RQ_F32) reinterpret_cast<float *>(a.y)[row * a.ldy + n + i] = acc[r][t][i];
-                    else if (a.out_dtype == RQ_F16) reinterpret_cast<__half *>(a.y)[row * a.ldy + n + i] = from_float<RQ_F16>(acc[r][t][i]);
-                    else reinterpret_cast<__hip_bfloat16 *>(a.y)[row * a.ldy + n + i] = from_float<RQ_BF16>(acc[r][t][i]);
+                    const int at = i * 8 + (lane >> 3), token = (wc * TB + t) * 32 + at;
+                    if (token < tile.count) {
+                        const int64_t row = MODE == kDown ? a.row_of[tile.first + token] : tile.first + token;
+                        const v4f     v = *reinterpret_cast<const v4f *>(mine + at * kStride + (lane & 7) * 4);
+                        store_out(MODE == kDown ? RQ_F32 : a.out_dtype, a.y, row * a.ldy, (int64_t) (block0 + wr * RB + r) * 32 + (lane & 7) * 4,
+                                  a.L.N, v);
+                    }
                 }
+                __builtin_amdgcn_wave_barrier();
             }
         }
     }
 }
 
-template <int MODE>
+template <int MODE, int RB, int TB, int WC, int R>
 hipError_t launch(const ProductArgs &a, hipStream_t stream) {
-    constexpr int kBlocks = MODE == kGateUp ? 4 : 8;
-    const int64_t tiles = MODE == kDense ? (a.M + kTok - 1) / kTok : a.most_tiles;
-    hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE>), dim3((a.L.row_blocks + kBlocks - 1) / kBlocks, (unsigned) tiles), dim3(kThreads), 0,
-                       stream, a);
+    using G = Tiled<MODE, RB, TB, WC, R>;
+    const int row_tiles = (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
+    const int token_tiles = MODE == kDense ? (int) ((a.M + G::kTileTokens - 1) / G::kTileTokens) : a.most_tiles;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
+    if (set != hipSuccess) return set;
+    hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE, RB, TB, WC, R>), dim3((unsigned) row_tiles * token_tiles), dim3(G::kThreads), G::kBytes, stream,
+                       a, row_tiles, token_tiles);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_tiled(int mode, const ProductArgs &a, hipStream_t stream) {
-    return mode == kDense ? launch<kDense>(a, stream) : mode == kGateUp ? launch<kGateUp>(a, stream) : launch<kDown>(a, stream);
+    static const int v = getenv("RQ_T") ? atoi(getenv("RQ_T")) : 0;
+    if (mode == kDense) {
+        if (v == 1) return launch<kDense, 4, 2, 4, 4>(a, stream);
+        if (v == 2) return launch<kDense, 4, 2, 4, 3>(a, stream);
+        if (v == 3) return launch<kDense, 2, 2, 4, 4>(a, stream);
+        if (v == 4) return launch<kDense, 2, 2, 4, 6>(a, stream);
+        return launch<kDense, 4, 2, 2, 3>(a, stream);
+    }
+    return mode == kGateUp ? launch<kGateUp, 4, 2, 2, 3>(a, stream) : launch<kDown, 4, 2, 2, 3>(a, stream);
 }
 
 }  // namespace mx

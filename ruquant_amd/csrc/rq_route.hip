@@ -130,7 +130,7 @@ hipError_t route(const RouteArgs &a, hipStream_t stream) {
 // slots is that in which they arrive, and no result depends on it: every slot's row is computed by itself.
 constexpr int kSortThreads = 1024;
 __global__ __launch_bounds__(kSortThreads) void rq_sort_kernel(const SortArgs a) {
-    __shared__ int count[RQ_ROUTE_MAX_E], first[RQ_ROUTE_MAX_E], tile0[RQ_ROUTE_MAX_E];
+    __shared__ int count[RQ_ROUTE_MAX_E], first[RQ_ROUTE_MAX_E];
     const int t = threadIdx.x;
     for (int e = t; e < a.E; e += kSortThreads) count[e] = 0;
     __syncthreads();
@@ -139,10 +139,10 @@ __global__ __launch_bounds__(kSortThreads) void rq_sort_kernel(const SortArgs a)
         if (e >= 0 && e < a.E) atomicAdd(&count[e], 1);
     }
     __syncthreads();
-    // prefix sums of the counts and of the tiles, an expert a thread (E <= 1024)
-    const int mine = t < a.E ? count[t] : 0, tiles = (mine + a.tile_tokens - 1) / a.tile_tokens;
+    // prefix sums of the positions (in 32s) and of the tiles, an expert a thread (E <= 1024)
+    const int mine = t < a.E ? count[t] : 0, room = (mine + 31) & ~31, tiles = (mine + a.tile_tokens - 1) / a.tile_tokens;
     __shared__ int sum1[kSortThreads], sum2[kSortThreads];
-    sum1[t] = mine;
+    sum1[t] = room;
     sum2[t] = tiles;
     __syncthreads();
     for (int o = 1; o < kSortThreads; o <<= 1) {
@@ -153,16 +153,20 @@ __global__ __launch_bounds__(kSortThreads) void rq_sort_kernel(const SortArgs a)
         __syncthreads();
     }
     if (t < a.E) {
-        first[t] = sum1[t] - mine;
-        tile0[t] = sum2[t] - tiles;
+        const int at = sum1[t] - room;
+        first[t] = at;
         for (int i = 0; i < tiles; ++i) {
-            Tile &to = a.tiles[tile0[t] + i];
+            Tile &to = a.tiles[sum2[t] - tiles + i];
             to.expert = t;
-            to.first = first[t] + i * a.tile_tokens;
+            to.first = at + i * a.tile_tokens;
             to.count = min(a.tile_tokens, mine - i * a.tile_tokens);
         }
+        for (int i = mine; i < room; ++i) a.token_of[at + i] = -1;
     }
-    if (t == kSortThreads - 1) *a.n_tiles = sum2[t];
+    if (t == kSortThreads - 1) {
+        a.n_tiles[0] = sum2[t];
+        a.n_tiles[1] = sum1[t];
+    }
     __syncthreads();
     for (int i = t; i < a.slots; i += kSortThreads) {
         const int e = a.ids[i];
