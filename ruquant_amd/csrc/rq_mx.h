@@ -149,21 +149,17 @@ struct ProductArgs {
     ActLayout      H;
     WeightLayout   HP;
 };
+template <int DT>
+__device__ __forceinline__ uint32_t pair_bits(float lo, float hi) {   // of a 16-bit type
+    return (uint32_t) __builtin_bit_cast(uint16_t, from_float<DT>(lo)) | (uint32_t) __builtin_bit_cast(uint16_t, from_float<DT>(hi)) << 16;
+}
 // Four consecutive outputs n .. n + 3 of a row (`base` elements in), those in front of N.
 __device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int64_t n, int64_t N, const v4f &v) {
     const int64_t at = base + n;
     if (n + 3 < N && (at & 3) == 0 && ((uintptr_t) y & 15) == 0) {
-        if (dtype == RQ_F32) {
-            *reinterpret_cast<v4f *>(reinterpret_cast<float *>(y) + at) = v;
-        } else {
-            uint32_t w[2];
-            for (int i = 0; i < 2; ++i) {
-                const uint16_t lo = dtype == RQ_F16 ? __builtin_bit_cast(uint16_t, from_float<RQ_F16>(v[2 * i])) : bf16_bits(v[2 * i]);
-                const uint16_t hi = dtype == RQ_F16 ? __builtin_bit_cast(uint16_t, from_float<RQ_F16>(v[2 * i + 1])) : bf16_bits(v[2 * i + 1]);
-                w[i] = lo | (uint32_t) hi << 16;
-            }
-            *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(y) + at) = make_uint2(w[0], w[1]);
-        }
+        if (dtype == RQ_F32) *reinterpret_cast<v4f *>(reinterpret_cast<float *>(y) + at) = v;
+        else if (dtype == RQ_F16) *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(y) + at) = make_uint2(pair_bits<RQ_F16>(v[0], v[1]), pair_bits<RQ_F16>(v[2], v[3]));
+        else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(y) + at) = make_uint2(pair_bits<RQ_BF16>(v[0], v[1]), pair_bits<RQ_BF16>(v[2], v[3]));
         return;
     }
     for (int i = 0; i < 4; ++i) {
@@ -172,6 +168,24 @@ __device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int6
         else if (dtype == RQ_F16) reinterpret_cast<__half *>(y)[at + i] = from_float<RQ_F16>(v[i]);
         else reinterpret_cast<__hip_bfloat16 *>(y)[at + i] = from_float<RQ_BF16>(v[i]);
     }
+}
+// 16 bytes of consecutive outputs from LDS: four in fp32, eight in the 16-bit types.
+__device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int64_t n, int64_t N, const float *v) {
+    const v4f x = *reinterpret_cast<const v4f *>(v);
+    if (dtype == RQ_F32) {
+        store_out(RQ_F32, y, base, n, N, x);
+        return;
+    }
+    const v4f     z = *reinterpret_cast<const v4f *>(v + 4);
+    const int64_t at = base + n;
+    if (n + 7 < N && (at & 7) == 0 && ((uintptr_t) y & 15) == 0) {
+        const uint4 w = dtype == RQ_F16 ? make_uint4(pair_bits<RQ_F16>(x[0], x[1]), pair_bits<RQ_F16>(x[2], x[3]), pair_bits<RQ_F16>(z[0], z[1]), pair_bits<RQ_F16>(z[2], z[3]))
+                                        : make_uint4(pair_bits<RQ_BF16>(x[0], x[1]), pair_bits<RQ_BF16>(x[2], x[3]), pair_bits<RQ_BF16>(z[0], z[1]), pair_bits<RQ_BF16>(z[2], z[3]));
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(y) + at) = w;
+        return;
+    }
+    store_out(dtype, y, base, n, N, x);
+    store_out(dtype, y, base, n + 4, N, z);
 }
 // Block b (32 rows) of h = silu(gate) * up for the token in column lane % 32, from both lanes that hold it, as activations of the down
 // projection in row p. Behind the last block that the rows of h have (their padding to 64), the step's remaining scales are set
@@ -228,7 +242,7 @@ constexpr int kTiledTokens = 128;
 // Sorts the slots by expert, every expert's from a multiple of 32 positions on, and cuts them into tiles of tile_tokens positions.
 struct SortArgs {
     const int32_t *ids;
-    int            slots, top, E, tile_tokens;
+    int            slots, top, E, tile_tokens, positions;   // (positions: at most)
     int           *token_of, *slot_of;   // by position: token, slot; token -1 where there is none
     Tile          *tiles;
     int           *n_tiles;              // [0]: tiles, [1]: positions

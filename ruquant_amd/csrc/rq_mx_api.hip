@@ -136,6 +136,7 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     s.top = top;
     s.E = (int) E;
     s.tile_tokens = p.tile_tokens;
+    s.positions = (int) p.positions;
     s.token_of = (int *) (ws + p.token_of);
     s.slot_of = (int *) (ws + p.slot_of);
     s.tiles = (Tile *) (ws + p.tile_table);

@@ -239,28 +239,32 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void 
             }
         }
     } else {
-        // 32 tokens x 32 rows at a time through LDS (a region of the wavefront's own), so that a token's outputs leave as one run
-        constexpr int kStride = 36;
-        static_assert(G::kWaves * 32 * kStride * 4 <= G::kBytes, "a region per wavefront");
-        float *mine = reinterpret_cast<float *>(lds) + g.wave * 32 * kStride;
+        // 32 tokens x 64 rows at a time through LDS (a region of the wavefront's own), so that a token's outputs leave as whole lines.
+        // (Lines written in halves cost much: 2048 x 17408 outputs in bf16, 64 bytes a token and store, 38 us, in fp32 30.)
+        constexpr int kStride = 68;
+        static_assert(RB % 2 == 0 && G::kWaves * 32 * kStride * 4 <= G::kBytes, "a region per wavefront");
+        float    *mine = reinterpret_cast<float *>(lds) + g.wave * 32 * kStride;
+        const int dtype = MODE == kDown ? RQ_F32 : a.out_dtype;
         barrier();   // (the ring is not read any more)
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
 #pragma unroll
-            for (int r = 0; r < RB; ++r) {
+            for (int r = 0; r < RB; r += 2) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const v4f v = { g.acc[r][t][4 * q], g.acc[r][t][4 * q + 1], g.acc[r][t][4 * q + 2], g.acc[r][t][4 * q + 3] };
-                    *reinterpret_cast<v4f *>(mine + (lane & 31) * kStride + q * 8 + (lane >> 5) * 4) = v;
+                for (int q = 0; q < 8; ++q) {
+                    const v16f &c = g.acc[r + q / 4][t];
+                    *reinterpret_cast<v4f *>(mine + (lane & 31) * kStride + q * 8 + (lane >> 5) * 4) =
+                        v4f{ c[q % 4 * 4], c[q % 4 * 4 + 1], c[q % 4 * 4 + 2], c[q % 4 * 4 + 3] };
                 }
                 __builtin_amdgcn_wave_barrier();
-                for (int i = 0; i < 4; ++i) {
-                    const int at = i * 8 + (lane >> 3), token = (wc * TB + t) * 32 + at;
+                const int64_t n0 = (int64_t) (block0 + wr * RB + r) * 32;
+                const int     wide = dtype == RQ_F32 ? 4 : 3;   // (log2 of the lanes of a token: 16 bytes each)
+                const int     step = 64 >> wide, at0 = lane >> wide, n = (lane & ((1 << wide) - 1)) << (6 - wide);
+                for (int at = at0; at < 32; at += step) {
+                    const int token = (wc * TB + t) * 32 + at;
                     if (token < tile.count) {
                         const int64_t row = MODE == kDown ? a.row_of[tile.first + token] : tile.first + token;
-                        const v4f     v = *reinterpret_cast<const v4f *>(mine + at * kStride + (lane & 7) * 4);
-                        store_out(MODE == kDown ? RQ_F32 : a.out_dtype, a.y, row * a.ldy, (int64_t) (block0 + wr * RB + r) * 32 + (lane & 7) * 4,
-                                  a.L.N, v);
+                        store_out(dtype, a.y, row * a.ldy, n0 + n, a.L.N, mine + at * kStride + n);
                     }
                 }
                 __builtin_amdgcn_wave_barrier();
@@ -285,14 +289,7 @@ hipError_t launch(const ProductArgs &a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_tiled(int mode, const ProductArgs &a, hipStream_t stream) {
-    static const int v = getenv("RQ_T") ? atoi(getenv("RQ_T")) : 0;
-    if (mode == kDense) {
-        if (v == 1) return launch<kDense, 4, 2, 4, 4>(a, stream);
-        if (v == 2) return launch<kDense, 4, 2, 4, 3>(a, stream);
-        if (v == 3) return launch<kDense, 2, 2, 4, 4>(a, stream);
-        if (v == 4) return launch<kDense, 2, 2, 4, 6>(a, stream);
-        return launch<kDense, 4, 2, 2, 3>(a, stream);
-    }
+    if (mode == kDense) return a.L.steps >= 64 ? launch<kDense, 4, 2, 4, 4>(a, stream) : launch<kDense, 2, 2, 2, 3>(a, stream);
     return mode == kGateUp ? launch<kGateUp, 4, 2, 2, 3>(a, stream) : launch<kDown, 4, 2, 2, 3>(a, stream);
 }
 

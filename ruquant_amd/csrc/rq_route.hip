@@ -129,67 +129,129 @@ hipError_t route(const RouteArgs &a, hipStream_t stream) {
 // One workgroup: counts the experts' slots, lays their tiles out and deals the slots to their places. The order of an expert's
 // slots is that in which they arrive, and no result depends on it: every slot's row is computed by itself.
 constexpr int kSortThreads = 1024;
+constexpr int kSortBatch = 8;   // ids in flight per thread
+// Up to so many positions the slots are dealt in LDS and written in order: from this one workgroup a store of 64 places of memory
+// takes 64 clocks. (16384 slots of 64 experts: 19 us dealt to memory directly.)
+constexpr int kSortLds = 32768;
+
+// sum over the threads in front of and with this one (all of the workgroup take part)
+__device__ __forceinline__ int scan(int v, int *waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 63) waves[wave] = v;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) v += waves[i];
+    return v;
+}
+
 __global__ __launch_bounds__(kSortThreads) void rq_sort_kernel(const SortArgs a) {
-    __shared__ int count[RQ_ROUTE_MAX_E], first[RQ_ROUTE_MAX_E];
+    __shared__ int count[RQ_ROUTE_MAX_E], waves[2][kSortThreads / 64];
     const int t = threadIdx.x;
-    for (int e = t; e < a.E; e += kSortThreads) count[e] = 0;
+    count[t] = 0;   // (E <= 1024)
     __syncthreads();
-    for (int i = t; i < a.slots; i += kSortThreads) {
-        const int e = a.ids[i];
-        if (e >= 0 && e < a.E) atomicAdd(&count[e], 1);
+    for (int i0 = t; i0 < a.slots; i0 += kSortThreads * kSortBatch) {
+        int e[kSortBatch];
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) e[k] = i0 + k * kSortThreads < a.slots ? a.ids[i0 + k * kSortThreads] : -1;
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k)
+            if (e[k] >= 0 && e[k] < a.E) atomicAdd(&count[e[k]], 1);
     }
     __syncthreads();
-    // prefix sums of the positions (in 32s) and of the tiles, an expert a thread (E <= 1024)
+    // the positions (in 32s) and tiles in front of each expert, an expert a thread
     const int mine = t < a.E ? count[t] : 0, room = (mine + 31) & ~31, tiles = (mine + a.tile_tokens - 1) / a.tile_tokens;
-    __shared__ int sum1[kSortThreads], sum2[kSortThreads];
-    sum1[t] = room;
-    sum2[t] = tiles;
-    __syncthreads();
-    for (int o = 1; o < kSortThreads; o <<= 1) {
-        const int v = t >= o ? sum1[t - o] : 0, w = t >= o ? sum2[t - o] : 0;
-        __syncthreads();
-        sum1[t] += v;
-        sum2[t] += w;
-        __syncthreads();
-    }
+    const int at = scan(room, waves[0]) - room, tile0 = scan(tiles, waves[1]) - tiles;
     if (t < a.E) {
-        const int at = sum1[t] - room;
-        first[t] = at;
+        count[t] = at;
         for (int i = 0; i < tiles; ++i) {
-            Tile &to = a.tiles[sum2[t] - tiles + i];
-            to.expert = t;
-            to.first = at + i * a.tile_tokens;
-            to.count = min(a.tile_tokens, mine - i * a.tile_tokens);
+            const Tile to = { t, at + i * a.tile_tokens, min(a.tile_tokens, mine - i * a.tile_tokens), 0 };
+            a.tiles[tile0 + i] = to;
         }
-        for (int i = mine; i < room; ++i) a.token_of[at + i] = -1;
+        if (a.positions > kSortLds)
+            for (int i = mine; i < room; ++i) a.token_of[at + i] = -1;
     }
     if (t == kSortThreads - 1) {
-        a.n_tiles[0] = sum2[t];
-        a.n_tiles[1] = sum1[t];
+        a.n_tiles[0] = tile0 + tiles;
+        a.n_tiles[1] = at + room;
     }
+    extern __shared__ int dealt[];
+    const bool in_lds = a.positions <= kSortLds;
     __syncthreads();
-    for (int i = t; i < a.slots; i += kSortThreads) {
-        const int e = a.ids[i];
-        if (e >= 0 && e < a.E) {
-            const int p = atomicAdd(&first[e], 1);
-            a.slot_of[p] = i;
-            a.token_of[p] = i / a.top;
+    for (int i0 = t; i0 < a.slots; i0 += kSortThreads * kSortBatch) {
+        int e[kSortBatch], p[kSortBatch];
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) e[k] = i0 + k * kSortThreads < a.slots ? a.ids[i0 + k * kSortThreads] : -1;
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) p[k] = e[k] >= 0 && e[k] < a.E ? atomicAdd(&count[e[k]], 1) : -1;
+#pragma unroll
+        for (int k = 0; k < kSortBatch; ++k) {
+            const int i = i0 + k * kSortThreads;
+            if (p[k] < 0) continue;
+            if (in_lds) dealt[p[k]] = i;
+            else a.slot_of[p[k]] = i, a.token_of[p[k]] = i / a.top;
         }
+    }
+    if (!in_lds) return;
+    // (the places behind an expert's last slot)
+    if (t < a.E)
+        for (int i = mine; i < room; ++i) dealt[at + i] = -1;
+    __shared__ int positions;
+    if (t == kSortThreads - 1) positions = at + room;
+    __syncthreads();
+    for (int p = t; p < positions; p += kSortThreads) {
+        const int i = dealt[p];
+        a.slot_of[p] = i;
+        a.token_of[p] = i < 0 ? -1 : i / a.top;
     }
 }
 
-template <int DT>
+// y[m] = sum_j weights[m][j] * rows[m top + j] in the order of j, fp32, four outputs a thread; the slots' rows are loaded four at a time.
+template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void rq_combine_kernel(const float *rows, int64_t N, const int32_t *ids, const float *weights,
                                                          int top, int E, typename Element<DT>::type *y, int64_t ldy) {
-    const int64_t m = blockIdx.x;
-    for (int64_t n = (int64_t) blockIdx.y * 256 + threadIdx.x; n < N; n += (int64_t) gridDim.y * 256) {
-        float sum = 0;
-        for (int j = 0; j < top; ++j) {
-            const int e = ids[m * top + j];
-            if (e >= 0 && e < E) sum += weights[m * top + j] * rows[(m * top + j) * N + n];
+    const int64_t m = blockIdx.x, n = ((int64_t) blockIdx.y * 256 + threadIdx.x) * 4;
+    if (n >= N) return;
+    v4f sum = { 0, 0, 0, 0 };
+    for (int j0 = 0; j0 < top; j0 += 4) {
+        v4f   v[4];
+        float w[4];
+        bool  there[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t slot = m * top + j0 + k;
+            const int     e = j0 + k < top ? ids[slot] : -1;
+            there[k] = e >= 0 && e < E;
+            w[k] = 0;
+            v[k] = v4f{ 0, 0, 0, 0 };
+            if (there[k]) {
+                w[k] = weights[slot];
+                if constexpr (VEC) {
+                    v[k] = *reinterpret_cast<const v4f *>(rows + slot * N + n);
+                } else {
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < N) v[k][i] = rows[slot * N + n + i];
+                }
+            }
         }
-        y[m * ldy + n] = from_float<DT>(sum);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (there[k]) sum += w[k] * v[k];
     }
+    store_out(DT, y, m * ldy, n, N, sum);
+}
+
+template <int DT>
+hipError_t combine(const float *rows, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E, void *y,
+                   int64_t ldy, hipStream_t stream) {
+    const dim3 grid((unsigned) M, (unsigned) ((N + 1023) / 1024));
+    auto      *out = reinterpret_cast<typename Element<DT>::type *>(y);
+    if (N % 4 == 0) hipLaunchKernelGGL((rq_combine_kernel<DT, true>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E, out, ldy);
+    else hipLaunchKernelGGL((rq_combine_kernel<DT, false>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E, out, ldy);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -201,22 +263,20 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t stream) {
 }
 
 hipError_t launch_sort(const SortArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(rq_sort_kernel, dim3(1), dim3(kSortThreads), 0, stream, a);
+    constexpr int kMost = kSortLds * sizeof(int);
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(rq_sort_kernel),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (set != hipSuccess) return set;
+    const int bytes = a.positions <= kSortLds ? a.positions * (int) sizeof(int) : 0;
+    hipLaunchKernelGGL(rq_sort_kernel, dim3(1), dim3(kSortThreads), bytes, stream, a);
     return hipGetLastError();
 }
 
 hipError_t launch_combine(const float *rows, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E,
                           int out_dtype, void *y, int64_t ldy, hipStream_t stream) {
-    const dim3 grid((unsigned) M, (unsigned) ((N + 1023) / 1024));
-    if (out_dtype == RQ_F32) {
-        hipLaunchKernelGGL((rq_combine_kernel<RQ_F32>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E, (float *) y, ldy);
-    } else if (out_dtype == RQ_F16) {
-        hipLaunchKernelGGL((rq_combine_kernel<RQ_F16>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E, (__half *) y, ldy);
-    } else {
-        hipLaunchKernelGGL((rq_combine_kernel<RQ_BF16>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E,
-                           (__hip_bfloat16 *) y, ldy);
-    }
-    return hipGetLastError();
+    if (out_dtype == RQ_F32) return combine<RQ_F32>(rows, N, ids, weights, M, top, E, y, ldy, stream);
+    if (out_dtype == RQ_F16) return combine<RQ_F16>(rows, N, ids, weights, M, top, E, y, ldy, stream);
+    return combine<RQ_BF16>(rows, N, ids, weights, M, top, E, y, ldy, stream);
 }
 
 }  // namespace mx
