@@ -233,6 +233,29 @@ __device__ __forceinline__ void store_h(const ProductArgs &a, const v16f &gate, 
         }
     }
 }
+// Few tokens (rq_mx_decode.hip): up to four that every workgroup quantises for itself, or up to 16 in row form (a_codes set). The
+// experts of up to four tokens in two launches; their h is rows of h_stride bytes of codes by slot, and of h_stride / 16 scales.
+struct DecodeArgs {
+    WeightLayout   L;
+    const uint8_t *w, *w2;
+    const void    *x;
+    int64_t        ldx, M;
+    const uint8_t *a_codes, *a_scales;
+    ActLayout      A;
+    const int32_t *ids;
+    const float   *weights;
+    int            top, E;
+    uint8_t       *h_codes, *h_scales;
+    int64_t        h_stride;
+    int            out_dtype;
+    void          *y;
+    int64_t        ldy;
+};
+// whether these tokens can be quantised that way (most: elements that it is worth for)
+bool decode_takes(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, int64_t most);
+hipError_t launch_decode(int dtype, const DecodeArgs &a, hipStream_t stream);
+hipError_t launch_decode_experts(int dtype, const DecodeArgs &gate_up, const DecodeArgs &down, hipStream_t stream);
+
 // few tokens per tile (tile_tokens 32 or 64): weights go from memory into registers
 hipError_t launch_skinny(int mode, const ProductArgs &a, int tile_tokens, hipStream_t stream);
 // many: both operands through LDS (tile_tokens 128)

@@ -12,6 +12,10 @@ int64_t pad256(int64_t n) { return up_to(n, 256); }
 
 constexpr int64_t kMaxTokens = 1 << 22;   // rows of a call; slots of an experts' call
 
+// Most elements that every workgroup of a product quantises for itself.
+constexpr int64_t kFusedElements = 24576;
+// Most tokens whose experts' weights are streamed slot by slot, without sorting.
+constexpr int64_t kExpertsDecodeTokens = 4;
 // tokens up to which a product streams its weights (rq_mx_skinny.hip)
 constexpr int kSkinnyTokens = 64;
 
@@ -26,7 +30,7 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
     ExpertsPlan p;
     p.slots = M * top;
     const double per = (double) p.slots / (double) E;   // of an expert, on average
-    p.tile_tokens = per <= 16 ? 32 : per <= 40 ? 64 : 128;
+    p.tile_tokens = per <= 16 ? 32 : per <= 40 || M <= kExpertsDecodeTokens ? 64 : 128;
     p.panels = p.tile_tokens > kSkinnyTokens;
     p.tiles = most_tiles(p.slots, E, p.tile_tokens);
     p.positions = most_positions(p.slots, E);
@@ -75,6 +79,26 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
     }
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
+    if (M <= 16) {
+        DecodeArgs d = {};
+        d.L = weight_layout(N, K);
+        d.x = x;
+        d.ldx = ldx;
+        d.M = M;
+        d.w = (const uint8_t *) prepared;
+        d.out_dtype = out_dtype;
+        d.y = y;
+        d.ldy = ldy;
+        if (!decode_takes(in_dtype, x, ldx, M, K, kFusedElements)) {
+            d.A = act_layout(K);
+            uint8_t *codes = (uint8_t *) workspace, *scales = codes + pad256(M * d.A.code_stride);
+            d.a_codes = codes;
+            d.a_scales = scales;
+            const hipError_t e = launch_act_quantize(in_dtype, x, ldx, M, K, codes, scales, st);
+            if (e != hipSuccess) return e;
+        }
+        return launch_decode(in_dtype, d, st);
+    }
     ProductArgs a = {};
     a.L = weight_layout(N, K);
     a.A = act_layout(K);
@@ -130,6 +154,29 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < p.total) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
     uint8_t *ws = (uint8_t *) workspace;
+    if (decode_takes(in_dtype, x, ldx, 1, K, 65536) && (M == 1 || (M <= kExpertsDecodeTokens && ldx * (int64_t) dtype_bytes(in_dtype) % 16 == 0))) {
+        DecodeArgs g = {};
+        g.L = weight_layout(F, K);
+        g.w = (const uint8_t *) gate;
+        g.w2 = (const uint8_t *) up;
+        g.x = x;
+        g.ldx = ldx;
+        g.M = M;
+        g.ids = ids;
+        g.weights = weights;
+        g.top = top;
+        g.E = (int) E;
+        g.h_stride = up_to(F, 256) / 2;
+        g.h_codes = ws + p.h;
+        g.h_scales = ws + p.h_scales;
+        g.out_dtype = out_dtype;
+        g.y = y;
+        g.ldy = ldy;
+        DecodeArgs d = g;
+        d.L = weight_layout(N, F);
+        d.w = (const uint8_t *) down;
+        return launch_decode_experts(in_dtype, g, d, st);
+    }
     SortArgs s;
     s.ids = ids;
     s.slots = (int) p.slots;
