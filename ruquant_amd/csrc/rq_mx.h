@@ -33,7 +33,7 @@ inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // Activations (workspace), in one of two forms:
 //   panels: as a weight of so many rows (the tiled product: its loads are whole runs of 1 KiB);
 //   rows  : rows of K / 2 bytes (K padded to 256: whole 128-byte lines), and per row and 256 inputs 2 x 4 bytes of scales, [block of
-//           a run][run]: the four bytes that a lane needs are one word here too (the skinny product: few rows are read, in any order).
+//           a run][run] (a few tokens, which the lanes of one fragment read).
 // ---------------------------------------------------------------------------------------------------
 struct WeightLayout {
     int64_t N, K;
@@ -74,17 +74,23 @@ __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__hip_bfloat16 v) {
     return __uint_as_float((uint32_t) __builtin_bit_cast(uint16_t, v) << 16);
 }
-__device__ __forceinline__ uint16_t bf16_bits(float f) {   // to the nearest, ties to even; NaN stays NaN
-    const uint32_t u = __float_as_uint(f);
-    return f != f ? 0x7FC0 : (uint16_t) ((u + 0x7FFF + ((u >> 16) & 1)) >> 16);
-}
 template <int DT>
 __device__ __forceinline__ typename Element<DT>::type from_float(float f) {
     if constexpr (DT == RQ_F32) return f;
     else if constexpr (DT == RQ_F16) return __float2half(f);
-    else return __builtin_bit_cast(__hip_bfloat16, bf16_bits(f));
+    else return __builtin_bit_cast(__hip_bfloat16, (__bf16) f);   // (to the nearest, ties to even; one instruction for two)
 }
 
+// The largest of this lane's and its neighbours' in the group of four, and of both lanes l and l + 32 (cross-lane operations of the
+// vector ALU: through LDS each costs a hundred clocks).
+__device__ __forceinline__ uint32_t max_of_four(uint32_t v) {
+    v = max(v, (uint32_t) __builtin_amdgcn_mov_dpp((int) v, 0xB1, 0xF, 0xF, true));
+    return max(v, (uint32_t) __builtin_amdgcn_mov_dpp((int) v, 0x4E, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t of_other_half(uint32_t v, bool upper) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);   // [0]: the lower half's, [1]: the upper half's
+    return upper ? r[0] : r[1];
+}
 // The scale byte of a block by its largest magnitude's bits (sign cleared): 255 for an infinity or NaN.
 __device__ __forceinline__ int block_scale(uint32_t top_bits) {
     const int e = (int) (top_bits >> 23);
@@ -131,27 +137,36 @@ struct Tile {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
+// Rows of the slots in 16 bits, for outputs of 16 bits: whole numbers up to 2^15 of a unit that 32 outputs share, 2^(X - 141), X the
+// exponent of the largest (16 .. 254; 255: one of them is not finite, and all 32 read as NaN). Each output is off by at most 2^-15 of
+// the 32's largest, 1 / 100 of what its last rounding to bf16 costs, and the rows' traffic, which is what their sum takes, is halved.
+constexpr int kRows16 = 3;
+
 struct ProductArgs {
     WeightLayout   L;
     const uint8_t *w, *w2;          // prepared weights; kGateUp: w the gate, w2 the up projection
-    const uint8_t *a_codes, *a_scales;   // rows; panels: both behind a_codes
-    ActLayout      A;
-    WeightLayout   P;                    // of the panels
+    const uint8_t *panels;          // the activations
+    WeightLayout   P;
     int64_t        M;               // tokens (kDense)
     const Tile    *tiles;           // kGateUp, kDown: the tiles, on the device
-    const int     *n_tiles;         //   and how many there are
-    int            most_tiles;      //   at most
-    const int     *row_of;          // position -> row: kGateUp of the activations (row form), kDown of the output
+    int            most_tiles;      //   so many; those past the last one have no tokens
+    const int     *row_of;          // kDown: position -> row of y
     int            out_dtype;
-    void          *y;               // kDense: the result; kDown: fp32 rows of the slots
+    void          *y;               // kDense: the result; kDown: rows of the slots, fp32 or kRows16
     int64_t        ldy;
-    uint8_t       *h_codes, *h_scales;   // kGateUp: activations of the down projection by position, in the form that it reads
-    ActLayout      H;
+    uint8_t       *row_scales;      // kRows16: ldy / 32 a row
+    uint8_t       *h;               // kGateUp: the down projection's activations, panels by position
     WeightLayout   HP;
 };
 template <int DT>
 __device__ __forceinline__ uint32_t pair_bits(float lo, float hi) {   // of a 16-bit type
-    return (uint32_t) __builtin_bit_cast(uint16_t, from_float<DT>(lo)) | (uint32_t) __builtin_bit_cast(uint16_t, from_float<DT>(hi)) << 16;
+    if constexpr (DT == RQ_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, h2{ (_Float16) lo, (_Float16) hi });
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, b2{ (__bf16) lo, (__bf16) hi });
+    }
 }
 // Four consecutive outputs n .. n + 3 of a row (`base` elements in), those in front of N.
 __device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int64_t n, int64_t N, const v4f &v) {
@@ -187,10 +202,27 @@ __device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int6
     store_out(dtype, y, base, n, N, x);
     store_out(dtype, y, base, n + 4, N, z);
 }
+// Eight outputs n .. n + 7 of a row in 16 bits, of 32 that this lane and its three neighbours have (N is padded to 64).
+__device__ __forceinline__ void store_rows16(const ProductArgs &a, int64_t row, int64_t n, const float *v) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    top = max_of_four(top);
+    const int   e = (int) (top >> 23), X = e >= 255 ? 255 : e < 16 ? 16 : e;
+    const float by = X == 255 ? 0.0f : __uint_as_float((uint32_t) (268 - X) << 23);   // 2^(141 - X)
+    // (rounded to a whole number, ties to even, by the addition of 1.5 x 2^23, which leaves it in the low bits)
+    uint32_t q[8], w[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(fminf(__builtin_fmaf(v[i], by, 12582912.0f), 12582912.0f + 32767.0f));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x05040100);
+    if (n >= a.ldy) return;   // (a tile past the padded rows)
+    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y) + row * a.ldy + n) = make_uint4(w[0], w[1], w[2], w[3]);
+    if ((n & 31) == 0) a.row_scales[row * (a.ldy >> 5) + (n >> 5)] = (uint8_t) X;
+}
 // Block b (32 rows) of h = silu(gate) * up for the token in column lane % 32, from both lanes that hold it, as activations of the down
 // projection in row p. Behind the last block that the rows of h have (their padding to 64), the step's remaining scales are set
 // too: the down projection multiplies them by zero codes, and a NaN would show.
-template <bool PANELS>
 __device__ __forceinline__ void store_h(const ProductArgs &a, const v16f &gate, const v16f &up, int lane, bool there, int64_t p, int b) {
     float    h[16];
     uint32_t top = 0;
@@ -199,7 +231,8 @@ __device__ __forceinline__ void store_h(const ProductArgs &a, const v16f &gate, 
         h[i] = gate[i] / (1.0f + expf(-gate[i])) * up[i];
         top = max(top, __float_as_uint(h[i]) & 0x7FFFFFFFu);
     }
-    top = max(top, (uint32_t) __shfl_xor((int) top, 32));
+    const bool upper = lane >= 32;
+    top = max(top, of_other_half(top, upper));
     const int X = block_scale(top);
     uint32_t  c[2];   // rows 8 q + 4 (lane / 32) .. + 3 in half-word q
 #pragma unroll
@@ -209,27 +242,17 @@ __device__ __forceinline__ void store_h(const ProductArgs &a, const v16f &gate, 
         for (int i = 0; i < 8; ++i) v[i] = h[8 * q + i];
         c[q] = X == 255 ? 0u : pack8(v, scale_down(X));
     }
-    const uint32_t o[2] = { (uint32_t) __shfl_xor((int) c[0], 32), (uint32_t) __shfl_xor((int) c[1], 32) };
+    const uint32_t o[2] = { of_other_half(c[0], upper), of_other_half(c[1], upper) };
     if (lane < 32 && there) {
         const uint4 codes = make_uint4((c[0] & 0xFFFF) | o[0] << 16, c[0] >> 16 | (o[0] & 0xFFFF0000u), (c[1] & 0xFFFF) | o[1] << 16,
                                        c[1] >> 16 | (o[1] & 0xFFFF0000u));
-        uint8_t *to;
-        if constexpr (PANELS) {
-            const int64_t block = p >> 5;
-            const int     row = (int) p & 31;
-            *reinterpret_cast<uint4 *>(a.h_codes + (block * a.HP.steps * 2 + (b >> 1)) * 1024 + ((b & 1) * 32 + row) * 16) = codes;
-            to = a.h_codes + a.HP.code_bytes + block * a.HP.chunks * 512;
-            to[panel_scale_at(row, b)] = (uint8_t) X;
-            if (b == a.L.row_blocks - 1) {
-                for (int k = b + 1; k & 3; ++k) to[panel_scale_at(row, k)] = 0;
-            }
-        } else {
-            *reinterpret_cast<uint4 *>(a.h_codes + p * a.H.code_stride + (int64_t) b * 16) = codes;
-            to = a.h_scales + p * a.H.scale_stride;
-            to[act_scale_at(b)] = (uint8_t) X;
-            if (b == a.L.row_blocks - 1) {
-                for (int k = b + 1; k & 3; ++k) to[act_scale_at(k)] = 0;
-            }
+        const int64_t block = p >> 5;
+        const int     row = (int) p & 31;
+        *reinterpret_cast<uint4 *>(a.h + (block * a.HP.steps * 2 + (b >> 1)) * 1024 + ((b & 1) * 32 + row) * 16) = codes;
+        uint8_t *to = a.h + a.HP.code_bytes + block * a.HP.chunks * 512;
+        to[panel_scale_at(row, b)] = (uint8_t) X;
+        if (b == a.L.row_blocks - 1) {
+            for (int k = b + 1; k & 3; ++k) to[panel_scale_at(row, k)] = 0;
         }
     }
 }
@@ -239,6 +262,7 @@ struct DecodeArgs {
     WeightLayout   L;
     const uint8_t *w, *w2;
     const void    *x;
+    bool           aligned;   // every row of x to 16 bytes
     int64_t        ldx, M;
     const uint8_t *a_codes, *a_scales;
     ActLayout      A;
@@ -251,16 +275,17 @@ struct DecodeArgs {
     void          *y;
     int64_t        ldy;
 };
-// whether these tokens can be quantised that way (most: elements that it is worth for)
-bool decode_takes(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, int64_t most);
+// whether a product's tokens are quantised that way
+bool decode_takes(int64_t M, int64_t K, int64_t N);
 hipError_t launch_decode(int dtype, const DecodeArgs &a, hipStream_t stream);
 hipError_t launch_decode_experts(int dtype, const DecodeArgs &gate_up, const DecodeArgs &down, hipStream_t stream);
 
-// few tokens per tile (tile_tokens 32 or 64): weights go from memory into registers
-hipError_t launch_skinny(int mode, const ProductArgs &a, int tile_tokens, hipStream_t stream);
-// many: both operands through LDS (tile_tokens 128)
-hipError_t launch_tiled(int mode, const ProductArgs &a, hipStream_t stream);
-constexpr int kTiledTokens = 128;
+// more tokens: both operands through LDS, in tiles of several forms
+constexpr int kTiledForms = 7, kForm64 = 1, kForm128 = 3, kForm256 = 6;   // (the experts': 128 x 64, 128 x 128, 256 x 128 rows x tokens)
+hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream);
+int tiled_form(const WeightLayout &L, int64_t M);   // for a plain product
+int tiled_tokens(int form);
+int64_t tiled_row_tiles(int mode, int form, int64_t N);
 
 // Sorts the slots by expert, every expert's from a multiple of 32 positions on, and cuts them into tiles of tile_tokens positions.
 struct SortArgs {
@@ -268,7 +293,8 @@ struct SortArgs {
     int            slots, top, E, tile_tokens, positions;   // (positions: at most)
     int           *token_of, *slot_of;   // by position: token, slot; token -1 where there is none
     Tile          *tiles;
-    int           *n_tiles;              // [0]: tiles, [1]: positions
+    int            most_tiles;           // the table's length: the tiles behind the last get a count of 0
+    int           *used;                 // how many positions there are
 };
 hipError_t launch_sort(const SortArgs &a, hipStream_t stream);
 inline int64_t most_positions(int64_t slots, int64_t E) {
@@ -279,8 +305,9 @@ inline int64_t most_tiles(int64_t slots, int64_t E, int tile_tokens) {
     const int64_t some = slots < E ? slots : E;
     return some + slots / tile_tokens;
 }
-// y[m] = sum_j weights[m][j] * rows[m * top + j], over the slots whose id is an expert's
-hipError_t launch_combine(const float *rows, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E,
+// y[m] = sum_j weights[m][j] * rows[m * top + j], over the slots whose id is an expert's. row_scales: rows of kRows16 with ld outputs
+// each; null: fp32 rows of N
+hipError_t launch_combine(const void *rows, const uint8_t *row_scales, int64_t ld, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E,
                           int out_dtype, void *y, int64_t ldy, hipStream_t stream);
 
 struct RouteArgs {

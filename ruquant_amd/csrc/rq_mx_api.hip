@@ -7,51 +7,65 @@ namespace {
 
 bool known_dtype(int dtype) { return dtype == RQ_F32 || dtype == RQ_F16 || dtype == RQ_BF16; }
 bool aligned(const void *p, size_t n) { return (uintptr_t) p % n == 0; }
+bool rows_aligned(const void *x, int64_t ld, int64_t M, int dtype) {
+    return aligned(x, 16) && (M == 1 || ld * (dtype == RQ_F32 ? 4 : 2) % 16 == 0);
+}
 size_t dtype_bytes(int dtype) { return dtype == RQ_F32 ? 4 : 2; }
 int64_t pad256(int64_t n) { return up_to(n, 256); }
 
 constexpr int64_t kMaxTokens = 1 << 22;   // rows of a call; slots of an experts' call
 
-// Most elements that every workgroup of a product quantises for itself.
-constexpr int64_t kFusedElements = 24576;
 // Most tokens whose experts' weights are streamed slot by slot, without sorting.
 constexpr int64_t kExpertsDecodeTokens = 4;
-// tokens up to which a product streams its weights (rq_mx_skinny.hip)
-constexpr int kSkinnyTokens = 64;
+// Most tokens of a product whose weights go from memory into registers (rq_mx_decode.hip).
+constexpr int kDecodeTokens = 16;
 
 struct ExpertsPlan {
-    int     tile_tokens;   // 32, 64: skinny; 128: tiled
-    bool    panels;        // activations in panel form: by position, as the tiled product reads them
-    int64_t slots, positions, tiles;
+    bool    decode;               // slot by slot (rq_mx_decode.hip); otherwise sorted by expert and tiled
+    int     tile_tokens;          // of both products
+    int     form;                 // of the tiles of both
+    bool    rows16;
+    int64_t slots, positions, tiles, ld;   // (ld: of rows16)
     WeightLayout XP, HP;
-    size_t  x, x_scales, h, h_scales, rows, token_of, slot_of, tile_table, n_tiles, total;   // offsets
+    size_t  x, h, h_scales, rows, row_scales, token_of, slot_of, tile_table, used, total;   // offsets
 };
-ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top) {
-    ExpertsPlan p;
+ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top, int out_dtype) {
+    ExpertsPlan p = {};
     p.slots = M * top;
-    const double per = (double) p.slots / (double) E;   // of an expert, on average
-    p.tile_tokens = per <= 16 ? 32 : per <= 40 || M <= kExpertsDecodeTokens ? 64 : 128;
-    p.panels = p.tile_tokens > kSkinnyTokens;
-    p.tiles = most_tiles(p.slots, E, p.tile_tokens);
-    p.positions = most_positions(p.slots, E);
-    p.XP = weight_layout(p.positions, K);
-    p.HP = weight_layout(p.positions, F);
-    const ActLayout X = act_layout(K), H = act_layout(F);
     size_t at = 0;
     auto take = [&](int64_t bytes) {
         const size_t here = at;
         at += (size_t) pad256(bytes);
         return here;
     };
-    p.x = take(p.panels ? p.XP.expert_bytes : M * X.code_stride);
-    p.x_scales = take(p.panels ? 0 : M * X.scale_stride);
-    p.h = take(p.panels ? p.HP.expert_bytes : p.positions * H.code_stride);
-    p.h_scales = take(p.panels ? 0 : p.positions * H.scale_stride);
-    p.rows = take(p.slots * N * 4);
+    p.decode = M <= kExpertsDecodeTokens && K <= 65536;
+    if (p.decode) {
+        p.h = take(p.slots * (up_to(F, 256) / 2));
+        p.h_scales = take(p.slots * (up_to(F, 256) / 32));
+        p.total = at;
+        return p;
+    }
+    // Tiles of 64 tokens up to 96 slots an expert; of 128 above, 256 rows of weights each where those are enough to keep the chip busy.
+    // (us for the whole call, 64 -> 128 tokens x 128 rows -> 128 x 256, by experts x slots an expert: 5120 x 1280 64 x 62: 210 -> 213 -> 226,
+    // 60 x 136: 295 -> 285 -> 258, 64 x 256: 479 -> 444 -> 403, 8 x 125: 50 -> 55 -> 64, 8 x 512: 134 -> 107 -> 120; 2048 x 512 60 x 136: 88 ->
+    // 83 -> 86, 64 x 256: 140 -> 128 -> 134)
+    const int64_t token_tiles = p.slots / 128 + ((p.slots < E ? p.slots : E) + 1) / 2;
+    p.form = p.slots <= 96 * E ? kForm64 : tiled_row_tiles(kGateUp, kForm256, F) * token_tiles >= 768 ? kForm256 : kForm128;
+    p.tile_tokens = tiled_tokens(p.form);
+    p.tiles = most_tiles(p.slots, E, p.tile_tokens);
+    p.positions = most_positions(p.slots, E);
+    p.XP = weight_layout(p.positions, K);
+    p.HP = weight_layout(p.positions, F);
+    p.rows16 = out_dtype != RQ_F32;
+    p.ld = up_to(N, 64);
+    p.x = take(p.XP.expert_bytes);
+    p.h = take(p.HP.expert_bytes);
+    p.rows = take(p.rows16 ? p.slots * p.ld * 2 : p.slots * N * 4);
+    p.row_scales = take(p.rows16 ? p.slots * p.ld / 32 : 0);
     p.token_of = take(p.positions * 4);
     p.slot_of = take(p.positions * 4);
     p.tile_table = take(p.tiles * (int64_t) sizeof(Tile));
-    p.n_tiles = take(8);
+    p.used = take(4);
     p.total = at;
     return p;
 }
@@ -65,7 +79,7 @@ bool good_experts(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top
 extern "C" size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M) {
     if (rq_mx4_prepared_bytes(1, N, K) == 0 || M < 0 || M > kMaxTokens) return 0;
     const ActLayout A = act_layout(K);
-    return (size_t) (M > kSkinnyTokens ? weight_layout(M, K).expert_bytes : pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
+    return (size_t) (M > kDecodeTokens ? weight_layout(M, K).expert_bytes : pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
 }
 
 extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in_dtype, const void *x, int64_t ldx, int64_t M,
@@ -79,17 +93,18 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
     }
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
-    if (M <= 16) {
+    if (M <= kDecodeTokens) {
         DecodeArgs d = {};
         d.L = weight_layout(N, K);
         d.x = x;
+        d.aligned = rows_aligned(x, ldx, M, in_dtype);
         d.ldx = ldx;
         d.M = M;
         d.w = (const uint8_t *) prepared;
         d.out_dtype = out_dtype;
         d.y = y;
         d.ldy = ldy;
-        if (!decode_takes(in_dtype, x, ldx, M, K, kFusedElements)) {
+        if (!decode_takes(M, K, N)) {
             d.A = act_layout(K);
             uint8_t *codes = (uint8_t *) workspace, *scales = codes + pad256(M * d.A.code_stride);
             d.a_codes = codes;
@@ -101,22 +116,15 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
     }
     ProductArgs a = {};
     a.L = weight_layout(N, K);
-    a.A = act_layout(K);
     a.w = (const uint8_t *) prepared;
-    uint8_t *codes = (uint8_t *) workspace, *scales = codes + pad256(M * a.A.code_stride);
-    a.a_codes = codes;
-    a.a_scales = scales;
+    a.panels = (uint8_t *) workspace;
     a.M = M;
     a.out_dtype = out_dtype;
     a.y = y;
     a.ldy = ldy;
-    if (M <= kSkinnyTokens) {
-        const hipError_t e = launch_act_quantize(in_dtype, x, ldx, M, K, codes, scales, st);
-        return e != hipSuccess ? e : launch_skinny(kDense, a, M <= 32 ? 32 : 64, st);
-    }
     a.P = weight_layout(M, K);
-    const hipError_t e = launch_panel_quantize(in_dtype, x, ldx, a.P, nullptr, nullptr, codes, st);
-    return e != hipSuccess ? e : launch_tiled(kDense, a, st);
+    const hipError_t e = launch_panel_quantize(in_dtype, x, ldx, a.P, nullptr, nullptr, (uint8_t *) workspace, st);
+    return e != hipSuccess ? e : launch_tiled(kDense, tiled_form(a.L, M), a, st);
 }
 
 extern "C" int rq_route(int dtype, const void *logits, int64_t ldl, int64_t M, int64_t E, int scoring, const float *bias, int groups,
@@ -137,7 +145,9 @@ extern "C" int rq_route(int dtype, const void *logits, int64_t ldl, int64_t M, i
 
 extern "C" size_t rq_mx4_experts_workspace_bytes(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top) {
     if (!good_experts(E, K, F, N, M, top)) return 0;
-    return experts_plan(E, K, F, N, M, top).total + 256;
+    // (room for either kind of rows)
+    const size_t a = experts_plan(E, K, F, N, M, top, RQ_F32).total, b = experts_plan(E, K, F, N, M, top, RQ_BF16).total;
+    return (a > b ? a : b) + 256;
 }
 
 extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down, int64_t E, int64_t K, int64_t F, int64_t N,
@@ -150,16 +160,17 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
         !aligned(weights, 4) || (M > 1 && (ldx < K || ldy < N))) {
         return RQ_E_ARGUMENT;
     }
-    const ExpertsPlan p = experts_plan(E, K, F, N, M, top);
+    const ExpertsPlan p = experts_plan(E, K, F, N, M, top, out_dtype);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < p.total) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
     uint8_t *ws = (uint8_t *) workspace;
-    if (decode_takes(in_dtype, x, ldx, 1, K, 65536) && (M == 1 || (M <= kExpertsDecodeTokens && ldx * (int64_t) dtype_bytes(in_dtype) % 16 == 0))) {
+    if (p.decode) {
         DecodeArgs g = {};
         g.L = weight_layout(F, K);
         g.w = (const uint8_t *) gate;
         g.w2 = (const uint8_t *) up;
         g.x = x;
+        g.aligned = rows_aligned(x, ldx, M, in_dtype);
         g.ldx = ldx;
         g.M = M;
         g.ids = ids;
@@ -187,40 +198,34 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     s.token_of = (int *) (ws + p.token_of);
     s.slot_of = (int *) (ws + p.slot_of);
     s.tiles = (Tile *) (ws + p.tile_table);
-    s.n_tiles = (int *) (ws + p.n_tiles);
+    s.most_tiles = (int) p.tiles;
+    s.used = (int *) (ws + p.used);
     hipError_t e = launch_sort(s, st);
-    if (e == hipSuccess) {
-        e = p.panels ? launch_panel_quantize(in_dtype, x, ldx, p.XP, s.token_of, s.n_tiles + 1, ws + p.x, st)
-                     : launch_act_quantize(in_dtype, x, ldx, M, K, ws + p.x, ws + p.x_scales, st);
-    }
+    if (e == hipSuccess) e = launch_panel_quantize(in_dtype, x, ldx, p.XP, s.token_of, s.used, ws + p.x, st);
     ProductArgs a = {};
     a.L = weight_layout(F, K);
-    a.A = act_layout(K);
     a.w = (const uint8_t *) gate;
     a.w2 = (const uint8_t *) up;
-    a.a_codes = ws + p.x;
-    a.a_scales = ws + p.x_scales;
-    a.tiles = s.tiles;
-    a.n_tiles = s.n_tiles;
-    a.most_tiles = (int) p.tiles;
-    a.row_of = s.token_of;
-    a.h_codes = ws + p.h;
-    a.h_scales = ws + p.h_scales;
-    a.H = act_layout(F);
+    a.panels = ws + p.x;
     a.P = p.XP;
+    a.tiles = s.tiles;
+    a.most_tiles = (int) p.tiles;
+    a.h = ws + p.h;
     a.HP = p.HP;
-    if (e == hipSuccess) e = p.panels ? launch_tiled(kGateUp, a, st) : launch_skinny(kGateUp, a, p.tile_tokens, st);
+    if (e == hipSuccess) e = launch_tiled(kGateUp, p.form, a, st);
     ProductArgs d = a;
     d.L = weight_layout(N, F);
-    d.A = a.H;
-    d.P = p.HP;
     d.w = (const uint8_t *) down;
-    d.a_codes = a.h_codes;
-    d.a_scales = a.h_scales;
+    d.panels = a.h;
+    d.P = p.HP;
     d.row_of = s.slot_of;
+    d.out_dtype = p.rows16 ? kRows16 : RQ_F32;
     d.y = ws + p.rows;
-    d.ldy = N;
-    if (e == hipSuccess) e = p.panels ? launch_tiled(kDown, d, st) : launch_skinny(kDown, d, p.tile_tokens, st);
-    if (e == hipSuccess) e = launch_combine((const float *) (ws + p.rows), N, ids, weights, M, top, (int) E, out_dtype, y, ldy, st);
+    d.ldy = p.rows16 ? p.ld : N;
+    d.row_scales = ws + p.row_scales;
+    if (e == hipSuccess) e = launch_tiled(kDown, p.form, d, st);
+    if (e == hipSuccess) {
+        e = launch_combine(ws + p.rows, p.rows16 ? d.row_scales : nullptr, d.ldy, N, ids, weights, M, top, (int) E, out_dtype, y, ldy, st);
+    }
     return e;
 }

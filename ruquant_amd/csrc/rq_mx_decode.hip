@@ -11,8 +11,8 @@ namespace rq {
 namespace mx {
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kWaves = 8;   // of the experts' kernels
+constexpr int kDecodeUnits = 512;   // most runs of 16 rows that are a workgroup each
 
 // This lane's part of a 16-row fragment of a step: row lane % 16, block lane / 16 of the step's four.
 struct Lane {
@@ -59,12 +59,15 @@ struct Tokens {
 
 // Eight elements of a token from k on (zeros past its end)
 template <int DT>
-__device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, int K, int u, float (&v)[8]) {
+__device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, bool aligned, int K, int u, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0;
     if (u * 8 >= K) return;
     const typename Element<DT>::type *p = x + u * 8;
-    if constexpr (DT == RQ_F32) {
+    if (!aligned) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_float(p[i]);
+    } else if constexpr (DT == RQ_F32) {
         const v4f a = *reinterpret_cast<const v4f *>(p), b = *reinterpret_cast<const v4f *>(p + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
@@ -82,8 +85,7 @@ __device__ __forceinline__ void store_unit(uint8_t *codes, uint8_t *scales, int 
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max(top, (uint32_t) __shfl_xor((int) top, 1));
-    top = max(top, (uint32_t) __shfl_xor((int) top, 2));
+    top = max_of_four(top);
     const int X = block_scale(top);
     *reinterpret_cast<uint32_t *>(codes + u * 4) = X == 255 ? 0u : pack8(v, scale_down(X));
     if ((u & 3) == 0) scales[u >> 2] = (uint8_t) X;
@@ -91,17 +93,18 @@ __device__ __forceinline__ void store_unit(uint8_t *codes, uint8_t *scales, int 
 
 // MAT weights of NR runs of 16 rows against T tokens: this wavefront's share of the inputs. DEPTH steps of the weights are on their
 // way while the tokens are quantised. ROWS: the tokens are in memory in row form instead (up to 16).
-template <int DT, bool ROWS, int MAT, int NR, int DEPTH>
+template <int DT, bool ROWS, int W, int MAT, int NR, int DEPTH>
 __device__ __forceinline__ void stream(const Rows (&rows)[MAT][NR], const Lane &l, const DecodeArgs &a, const typename Element<DT>::type *x, int T,
                                        uint8_t *lds, v4f (&acc)[MAT][NR]) {
+    constexpr int kThreads = 64 * W;
     const int    K = (int) a.L.K, steps = (K + 127) / 128, units = steps * 16;
     const Tokens tokens(lds, T, steps);
     const int    wave = threadIdx.x >> 6, u0 = threadIdx.x;
-    const int    s0 = steps * wave / kWaves, s1 = steps * (wave + 1) / kWaves;
+    const int    s0 = steps * wave / W, s1 = steps * (wave + 1) / W;
     float        v[2][8];
     if constexpr (!ROWS) {   // (the first two units of the first token: all there is of a short one)
-        if (u0 < units) load_unit<DT>(x, K, u0, v[0]);
-        if (u0 + kThreads < units) load_unit<DT>(x, K, u0 + kThreads, v[1]);
+        if (u0 < units) load_unit<DT>(x, a.aligned, K, u0, v[0]);
+        if (u0 + kThreads < units) load_unit<DT>(x, a.aligned, K, u0 + kThreads, v[1]);
         __builtin_amdgcn_sched_barrier(0);
     }
     const int      t = min(l.row, T - 1);   // (columns past the tokens repeat the last one)
@@ -133,8 +136,8 @@ __device__ __forceinline__ void stream(const Rows (&rows)[MAT][NR], const Lane &
             uint8_t *codes = tokens.codes + k * tokens.code_stride, *scales = tokens.scales + k * tokens.scale_stride;
             for (int u = k == 0 ? u0 + 2 * kThreads : u0; u < units; u += 2 * kThreads) {
                 const bool more = u + kThreads < units;
-                load_unit<DT>(x + k * a.ldx, K, u, v[0]);
-                if (more) load_unit<DT>(x + k * a.ldx, K, u + kThreads, v[1]);
+                load_unit<DT>(x + k * a.ldx, a.aligned, K, u, v[0]);
+                if (more) load_unit<DT>(x + k * a.ldx, a.aligned, K, u + kThreads, v[1]);
                 store_unit(codes, scales, u, v[0]);
                 if (more) store_unit(codes, scales, u + kThreads, v[1]);
             }
@@ -167,8 +170,8 @@ __device__ __forceinline__ void put_part(v4f *part, const v4f (&acc)[CELLS], con
     }
 }
 
-template <int DT, bool ROWS, int NR>
-__global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_kernel(const DecodeArgs a) {
+template <int DT, bool ROWS, int W, int NR>
+__global__ __launch_bounds__(64 * W, 4) void rq_mx_decode_kernel(const DecodeArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const Lane l;
     const int  wave = threadIdx.x >> 6, unit0 = blockIdx.x * NR;
@@ -179,16 +182,16 @@ __global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_kernel(const DecodeA
 #pragma unroll
     for (int r = 0; r < NR; ++r) acc[0][r] = v4f{ 0, 0, 0, 0 };
     const int T = (int) a.M;
-    stream<DT, ROWS, 1, NR, 8 / NR>(rows, l, a, reinterpret_cast<const typename Element<DT>::type *>(a.x), T, lds, acc);
+    stream<DT, ROWS, W, 1, NR, 8 / NR>(rows, l, a, reinterpret_cast<const typename Element<DT>::type *>(a.x), T, lds, acc);
     __syncthreads();   // (the tokens are not read any more)
     v4f *part = reinterpret_cast<v4f *>(lds);
     put_part<NR>(part, acc[0], l, T, wave);
     __syncthreads();
     const int cells = NR * T * 4;
-    for (int c = threadIdx.x; c < cells; c += kThreads) {
+    for (int c = threadIdx.x; c < cells; c += 64 * W) {
         v4f sum = part[c];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) sum += part[w * cells + c];
+        for (int w = 1; w < W; ++w) sum += part[w * cells + c];
         const int t = (c >> 2) % T, r = (c >> 2) / T;
         store_out(a.out_dtype, a.y, t * a.ldy, (int64_t) (unit0 + r) * 16 + (c & 3) * 4, a.L.N, sum);
     }
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_kernel(const DecodeA
 
 // One block of 32 rows of h of the slot blockIdx.y: gate and up, silu(gate) * up, quantised.
 template <int DT>
-__global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_gate_up_kernel(const DecodeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 4) void rq_mx_decode_gate_up_kernel(const DecodeArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int slot = blockIdx.y, e = a.ids[slot];
     if (e < 0 || e >= a.E) return;
@@ -213,7 +216,7 @@ __global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_gate_up_kernel(const
 #pragma unroll
         for (int r = 0; r < 2; ++r) acc[m][r] = v4f{ 0, 0, 0, 0 };
     const typename Element<DT>::type *x = reinterpret_cast<const typename Element<DT>::type *>(a.x) + (int64_t) (slot / a.top) * a.ldx;
-    stream<DT, false, 2, 2, 3>(rows, l, a, x, 1, lds, acc);
+    stream<DT, false, kWaves, 2, 2, 3>(rows, l, a, x, 1, lds, acc);
     __syncthreads();
     v4f      *part = reinterpret_cast<v4f *>(lds);
     const v4f all[4] = { acc[0][0], acc[0][1], acc[1][0], acc[1][1] };
@@ -235,8 +238,7 @@ __global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_gate_up_kernel(const
             h[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
             top = max(top, __float_as_uint(h[i]) & 0x7FFFFFFFu);
         }
-        top = max(top, (uint32_t) __shfl_xor((int) top, 1));
-        top = max(top, (uint32_t) __shfl_xor((int) top, 2));
+        top = max_of_four(top);
         const int X = block_scale(top), b = blockIdx.x, blocks = gridDim.x;
         reinterpret_cast<uint32_t *>(a.h_codes + (int64_t) slot * a.h_stride + b * 16)[threadIdx.x] = X == 255 ? 0u : pack8(h, scale_down(X));
         if (threadIdx.x == 0) {
@@ -251,8 +253,8 @@ __global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_gate_up_kernel(const
 // 16 rows of the output of token blockIdx.y: the wavefronts share out its slots, or parts of their inputs where there are fewer slots
 // than wavefronts, weigh their sums, and join them in the order of the wavefronts.
 template <int DT>
-__global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_down_kernel(const DecodeArgs a) {
-    constexpr int kDepth = 8;
+__global__ __launch_bounds__(64 * kWaves, 4) void rq_mx_decode_down_kernel(const DecodeArgs a) {
+    constexpr int kDepth = 5;   // (8: its registers leave one workgroup per compute unit)
     const Lane l;
     const int  wave = threadIdx.x >> 6, unit = blockIdx.x, m = blockIdx.y;
     const int  split = a.top >= kWaves ? 1 : kWaves / a.top, shares = a.top * split;
@@ -299,29 +301,34 @@ __global__ __launch_bounds__(kThreads, 4) void rq_mx_decode_down_kernel(const De
 }
 
 // LDS of the tokens, or of the partial sums behind them
-int lds_bytes(int64_t T, int64_t K, int cells) {
-    const int64_t tokens = T * ((K + 127) / 128) * 68, sums = (int64_t) kWaves * cells * T * 64;
+int lds_bytes(int64_t T, int64_t K, int cells, int waves) {
+    const int64_t tokens = T * ((K + 127) / 128) * 68, sums = (int64_t) waves * cells * T * 64;
     return (int) (tokens > sums ? tokens : sums);
 }
 
 template <int DT, bool ROWS>
 hipError_t decode(const DecodeArgs &a, hipStream_t stream) {
-    // 32 rows a workgroup where there are enough for the chip, 16 where there are not
+    // 32 rows and four wavefronts a workgroup where that is enough of them for the chip, 16 and eight where it is not (K = 5120, N = 5120,
+    // one token: 5.8 us with four, 5.1 with eight, 7.4 with sixteen; N = 17408 the same with four and eight)
     const int units = (int) ((a.L.N + 15) / 16);
     const int64_t K = ROWS ? 0 : a.L.K;
-    if (units > 2 * 256) {
-        hipLaunchKernelGGL((rq_mx_decode_kernel<DT, ROWS, 2>), dim3((units + 1) / 2), dim3(kThreads), lds_bytes(a.M, K, 2), stream, a);
+    if (units > kDecodeUnits) {
+        hipLaunchKernelGGL((rq_mx_decode_kernel<DT, ROWS, 4, 2>), dim3((units + 1) / 2), dim3(256), lds_bytes(a.M, K, 2, 4), stream, a);
     } else {
-        hipLaunchKernelGGL((rq_mx_decode_kernel<DT, ROWS, 1>), dim3(units), dim3(kThreads), lds_bytes(a.M, K, 1), stream, a);
+        hipLaunchKernelGGL((rq_mx_decode_kernel<DT, ROWS, 8, 1>), dim3(units), dim3(512), lds_bytes(a.M, K, 1, 8), stream, a);
     }
     return hipGetLastError();
 }
 
 }  // namespace
 
-bool decode_takes(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, int64_t most) {
-    const int64_t bytes = dtype == RQ_F32 ? 4 : 2;
-    return M <= 4 && M * K <= most && (uintptr_t) x % 16 == 0 && (M == 1 || ldx * bytes % 16 == 0);
+bool decode_takes(int64_t M, int64_t K, int64_t N) {
+    if (M > 4 || M * K > 65536) return false;
+    // Every workgroup reads and rounds all of the tokens, against a launch of 2 us that does it once. (us, by every workgroup -> once:
+    // N = 5120: K = 5120 2 tokens 5.9 -> 7.3, 4 tokens 7.7 -> 7.6, K = 17408 1 token 13.3 -> 14.5; N = 17408, K = 5120: 2 tokens
+    // 12.6 -> 12.8, 4 tokens 15.9 -> 13.2)
+    const int64_t units = (N + 15) / 16, workgroups = units > kDecodeUnits ? (units + 1) / 2 : units;
+    return M * K * workgroups <= 6000000;
 }
 
 hipError_t launch_decode(int dtype, const DecodeArgs &a, hipStream_t stream) {
@@ -331,16 +338,16 @@ hipError_t launch_decode(int dtype, const DecodeArgs &a, hipStream_t stream) {
 
 hipError_t launch_decode_experts(int dtype, const DecodeArgs &gate_up, const DecodeArgs &down, hipStream_t stream) {
     const dim3 grid(gate_up.L.row_blocks, (unsigned) (gate_up.M * gate_up.top));
-    const int  bytes = lds_bytes(1, gate_up.L.K, 4);
-    if (dtype == RQ_F32) hipLaunchKernelGGL((rq_mx_decode_gate_up_kernel<RQ_F32>), grid, dim3(kThreads), bytes, stream, gate_up);
-    else if (dtype == RQ_F16) hipLaunchKernelGGL((rq_mx_decode_gate_up_kernel<RQ_F16>), grid, dim3(kThreads), bytes, stream, gate_up);
-    else hipLaunchKernelGGL((rq_mx_decode_gate_up_kernel<RQ_BF16>), grid, dim3(kThreads), bytes, stream, gate_up);
+    const int  bytes = lds_bytes(1, gate_up.L.K, 4, kWaves);
+    if (dtype == RQ_F32) hipLaunchKernelGGL((rq_mx_decode_gate_up_kernel<RQ_F32>), grid, dim3(64 * kWaves), bytes, stream, gate_up);
+    else if (dtype == RQ_F16) hipLaunchKernelGGL((rq_mx_decode_gate_up_kernel<RQ_F16>), grid, dim3(64 * kWaves), bytes, stream, gate_up);
+    else hipLaunchKernelGGL((rq_mx_decode_gate_up_kernel<RQ_BF16>), grid, dim3(64 * kWaves), bytes, stream, gate_up);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 out((unsigned) ((down.L.N + 15) / 16), (unsigned) down.M);
-    if (down.out_dtype == RQ_F32) hipLaunchKernelGGL((rq_mx_decode_down_kernel<RQ_F32>), out, dim3(kThreads), 0, stream, down);
-    else if (down.out_dtype == RQ_F16) hipLaunchKernelGGL((rq_mx_decode_down_kernel<RQ_F16>), out, dim3(kThreads), 0, stream, down);
-    else hipLaunchKernelGGL((rq_mx_decode_down_kernel<RQ_BF16>), out, dim3(kThreads), 0, stream, down);
+    if (down.out_dtype == RQ_F32) hipLaunchKernelGGL((rq_mx_decode_down_kernel<RQ_F32>), out, dim3(64 * kWaves), 0, stream, down);
+    else if (down.out_dtype == RQ_F16) hipLaunchKernelGGL((rq_mx_decode_down_kernel<RQ_F16>), out, dim3(64 * kWaves), 0, stream, down);
+    else hipLaunchKernelGGL((rq_mx_decode_down_kernel<RQ_BF16>), out, dim3(64 * kWaves), 0, stream, down);
     return hipGetLastError();
 }
 

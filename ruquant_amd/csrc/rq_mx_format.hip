@@ -53,8 +53,7 @@ __global__ __launch_bounds__(kThreads) void rq_mx_quantize_kernel(const typename
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max(top, (uint32_t) __shfl_xor((int) top, 1));
-    top = max(top, (uint32_t) __shfl_xor((int) top, 2));
+    top = max_of_four(top);
     const int      X = block_scale(top);
     const uint32_t c = X == 255 ? 0u : pack8(v, scale_down(X));
     if (!ACT || (int64_t) u * 4 < code_stride) *reinterpret_cast<uint32_t *>(codes + (int64_t) m * code_stride + (int64_t) u * 4) = c;
@@ -91,8 +90,7 @@ __global__ __launch_bounds__(kThreads) void rq_mx_panel_quantize_kernel(const ty
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
-        top = max(top, (uint32_t) __shfl_xor((int) top, 1));
-        top = max(top, (uint32_t) __shfl_xor((int) top, 2));
+        top = max_of_four(top);
         const int X = block_scale(top);
         if (part * 4 + j < 2 * L.steps) *reinterpret_cast<uint32_t *>(codes + j * 1024) = X == 255 ? 0u : pack8(v[j], scale_down(X));
         word |= (uint32_t) X << (8 * j);

@@ -1,4 +1,6 @@
 // MXFP4 product for many tokens: tiles of rows x tokens, both operands through LDS.
+#include <type_traits>
+
 #include "rq_mx.h"
 
 namespace rq {
@@ -34,8 +36,11 @@ struct Tiled {
     static constexpr int kWaves = 2 * WC, kThreads = 64 * kWaves;
     static constexpr int kABlocks = 2 * RB, kBBlocks = WC * TB;
     static constexpr int kSlot = (kABlocks + kBBlocks) * 2048;   // one step of both operands
-    static constexpr int kScales = R * kSlot;                    // behind the ring: one chunk of their scales
-    static constexpr int kBytes = kScales + (kABlocks + kBBlocks) * 512;
+    // Behind the ring the scales, a chunk a slot. A short ring has one slot: the next chunk is fetched by the second step of a chunk, when
+    // its own has been read. A longer one would wait for that too early: there a chunk is fetched with its first step.
+    static constexpr bool kAhead = R > 4;
+    static constexpr int  kScaleSlots = kAhead ? (R + 5) / 4 : 1, kScaleSlot = (kABlocks + kBBlocks) * 512;
+    static constexpr int  kScales = R * kSlot, kBytes = kScales + kScaleSlots * kScaleSlot;
     // 1 KiB each, of a wavefront per step; runs of the scales per chunk (some are fetched twice so that all fetch as many)
     static constexpr int kARuns = 2 * kABlocks / kWaves, kBRuns = 2 * kBBlocks / kWaves, kRuns = kARuns + kBRuns;
     static constexpr int kScaleRuns = (kABlocks + kBBlocks) / 2, kScales1 = (kScaleRuns + kWaves - 1) / kWaves;
@@ -58,9 +63,11 @@ struct Tiled {
         if (i < kARuns) load_run(a_src[i] + (int64_t) t * 2048, lane16, to + (wave * kARuns + i) * 1024);
         else load_run(b_src[i - kARuns] + (int64_t) t * 2048, lane16, to + (2 * kABlocks + wave * kBRuns + i - kARuns) * 1024);
     }
+    static __device__ __forceinline__ int scale_slot(int c) { return kAhead ? c % kScaleSlots * kScaleSlot : 0; }
     __device__ __forceinline__ void fetch_scales(int c) {
 #pragma unroll
-        for (int i = 0; i < kScales1; ++i) load_run(s_src[i] + (int64_t) c * 512, lds0 + kScales + (i * kWaves + wave) % kScaleRuns * 1024);
+        for (int i = 0; i < kScales1; ++i)
+            load_run(s_src[i] + (int64_t) c * 512, lds0 + kScales + scale_slot(c) + (i * kWaves + wave) % kScaleRuns * 1024);
     }
     __device__ __forceinline__ void read_a(int slot, int i) {
 #pragma unroll
@@ -70,71 +77,82 @@ struct Tiled {
 #pragma unroll
         for (int h = 0; h < 2; ++h) B[i][h] = *reinterpret_cast<const v4i *>(b_lds + slot * kSlot + (2 * i + h) * 1024);
     }
-    // the scales of inputs 256 half .. + 255 of the chunk in LDS
-    __device__ __forceinline__ void read_sa(int half, int i) { sA[i] = *reinterpret_cast<const int *>(as_lds + i * 512 + half * 256); }
-    __device__ __forceinline__ void read_sb(int (&sB)[TB], int half, int i) const {
-        sB[i] = *reinterpret_cast<const int *>(bs_lds + i * 512 + half * 256);
+    // the scales of inputs 256 part .. + 255
+    __device__ __forceinline__ void read_sa(int part, int i) {
+        sA[i] = *reinterpret_cast<const int *>(as_lds + scale_slot(part >> 1) + i * 512 + (part & 1) * 256);
+    }
+    __device__ __forceinline__ void read_sb(int (&sB)[TB], int part, int i) const {
+        sB[i] = *reinterpret_cast<const int *>(bs_lds + scale_slot(part >> 1) + i * 512 + (part & 1) * 256);
     }
 
     // Step t = 4 c + J: its products from A and B, behind each row block's the read of its fragments of step t + 1, between them the
     // reads of step t + 1's activations into N and the fetch of step t + R - 1 into the slot of step t - 1 (whose reads the products
     // of step t - 1 have waited for, in every wavefront that has passed this step's barrier). The scales are read every second
-    // step; those of the next chunk are fetched by the second step of a chunk, last of its loads, and read by the fourth. MORE: all
-    // of those steps exist.
-    template <int J, bool MORE>
+    // step, those of the next chunk by the fourth of this one. (Ahead: chunk c is fetched by step 4 c - R + 1, into a slot whose last
+    // reads, of chunk c - S, the products of step 4 (c - S) + 2 have waited for; 4 S >= R + 2.) MORE: all of those steps exist.
+    template <bool ACTIVE, int J, bool MORE>
     __device__ __forceinline__ void step(int t, int slot, const v4i (&B)[TB][2], v4i (&N)[TB][2], int (&sB)[TB], int (&sN)[TB]) {
         const int  next = slot + 1 == R ? 0 : slot + 1, last = slot == 0 ? R - 1 : slot - 1;
         const bool get = MORE || t + R - 1 < steps;
         // step t + 1 has arrived; those behind it need not have
-        if (MORE || t + R - 2 < steps) wait_loads<(R - 3) * kRuns + (MORE && J == 2 ? kScales1 : 0)>();
+        constexpr int kChunks = kAhead ? ((J + R - 2) >> 2) - ((J + 1) >> 2) : MORE && J == 2;   // chunks' scales among those
+        if (MORE || t + R - 2 < steps) wait_loads<(R - 3) * kRuns + kChunks * kScales1>();
         else wait_loads<0>();
         barrier();
+        if (kAhead && (J + R - 1) % 4 == 0 && get) fetch_scales((t + R - 1) >> 2);
         if (!MORE && get) {
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) fetch_run(t + R - 1, last, i);
         }
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
+            if constexpr (ACTIVE) {
 #pragma unroll
-            for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1)>(A[r][0], B[b][0], acc[r][b], sA[r], sB[b]);
-            // (past the last step: what the ring holds, for nobody)
+                for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1)>(A[r][0], B[b][0], acc[r][b], sA[r], sB[b]);
+                // (past the last step: what the ring holds, for nobody)
 #pragma unroll
-            for (int i = r * TB / RB; i < (r + 1) * TB / RB; ++i) {
-                read_b(N, next, i);
-                if (J & 1) read_sb(sN, J == 1, i);
+                for (int i = r * TB / RB; i < (r + 1) * TB / RB; ++i) {
+                    read_b(N, next, i);
+                    if (J & 1) read_sb(sN, (t >> 1) + 1, i);
+                }
             }
             if (MORE) {
 #pragma unroll
                 for (int i = r * kRuns / RB; i < (r + 1) * kRuns / RB; ++i) fetch_run(t + R - 1, last, i);
             }
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (ACTIVE) {
 #pragma unroll
-            for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1) + 1>(A[r][1], B[b][1], acc[r][b], sA[r], sB[b]);
-            read_a(next, r);
-            if (J & 1) read_sa(J == 1, r);
+                for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1) + 1>(A[r][1], B[b][1], acc[r][b], sA[r], sB[b]);
+                read_a(next, r);
+                if (J & 1) read_sa((t >> 1) + 1, r);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (J & 1) {
+        if constexpr (ACTIVE && (J & 1)) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) sB[i] = sN[i];
         }
-        if (J == 1 && (MORE || t + 3 < steps)) fetch_scales((t >> 2) + 1);
+        if (!kAhead && J == 1 && (MORE || t + 3 < steps)) fetch_scales((t >> 2) + 1);
     }
 
+    // ACTIVE: this wavefront has tokens; otherwise it moves its share and keeps the barriers
+    template <bool ACTIVE>
     __device__ __forceinline__ void loop() {
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
             for (int t = 0; t < TB; ++t) acc[r][t] = v16f{ 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 };
-        fetch_scales(0);
+        if (!kAhead) fetch_scales(0);
 #pragma unroll
         for (int t = 0; t < R - 1; ++t) {
             if (t < steps) {
+                if (kAhead && t % 4 == 0) fetch_scales(t >> 2);
 #pragma unroll
                 for (int i = 0; i < kRuns; ++i) fetch_run(t, t, i);
             }
         }
-        if (steps >= R - 1) wait_loads<(R - 2) * kRuns>();
+        if (steps >= R - 1) wait_loads<(R - 2) * kRuns + (kAhead ? (R - 2) / 4 : 0) * kScales1>();
         else wait_loads<0>();
         barrier();
         v4i B[TB][2], N[TB][2];
@@ -146,19 +164,19 @@ struct Tiled {
         int  t = 0, slot = 0;
         auto next = [&]() __attribute__((always_inline)) { ++t, slot = slot + 1 == R ? 0 : slot + 1; };
         while (t + R + 2 < steps) {
-            step<0, true>(t, slot, B, N, sB, sN), next();
-            step<1, true>(t, slot, N, B, sB, sN), next();
-            step<2, true>(t, slot, B, N, sB, sN), next();
-            step<3, true>(t, slot, N, B, sB, sN), next();
+            step<ACTIVE, 0, true>(t, slot, B, N, sB, sN), next();
+            step<ACTIVE, 1, true>(t, slot, N, B, sB, sN), next();
+            step<ACTIVE, 2, true>(t, slot, B, N, sB, sN), next();
+            step<ACTIVE, 3, true>(t, slot, N, B, sB, sN), next();
         }
         while (true) {
-            step<0, false>(t, slot, B, N, sB, sN), next();
+            step<ACTIVE, 0, false>(t, slot, B, N, sB, sN), next();
             if (t >= steps) break;
-            step<1, false>(t, slot, N, B, sB, sN), next();
+            step<ACTIVE, 1, false>(t, slot, N, B, sB, sN), next();
             if (t >= steps) break;
-            step<2, false>(t, slot, B, N, sB, sN), next();
+            step<ACTIVE, 2, false>(t, slot, B, N, sB, sN), next();
             if (t >= steps) break;
-            step<3, false>(t, slot, N, B, sB, sN), next();
+            step<ACTIVE, 3, false>(t, slot, N, B, sB, sN), next();
             if (t >= steps) break;
         }
         wait_loads<0>();   // (none of this wavefront's loads lands in LDS behind this)
@@ -166,7 +184,7 @@ struct Tiled {
 };
 
 template <int MODE, int RB, int TB, int WC, int R>
-__global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void rq_mx_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles) {
+__global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB <= 4 ? 3 : 2) void rq_mx_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles) {
     using G = Tiled<MODE, RB, TB, WC, R>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     // Workgroups go to the XCDs in turn. Each XCD takes a run of the tiles in an order in which the token tiles run fastest, so that
@@ -180,14 +198,16 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void 
         tile.first = token_tile * G::kTileTokens;
         tile.count = (int) (a.M - tile.first < G::kTileTokens ? a.M - tile.first : G::kTileTokens);
     } else {
-        if (token_tile >= *a.n_tiles) return;
         tile = a.tiles[token_tile];
+        if (tile.count == 0) return;   // (past the last)
     }
     G g;
     g.lane = threadIdx.x & 63;
     g.wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    g.wr = g.wave / WC;
-    g.wc = g.wave % WC;
+    // (a wavefront's number mod 4 is its SIMD: the two that a tile with half of its tokens leaves idle, or the four, are of all of them; with
+    // four wavefronts the workgroups take turns)
+    g.wr = g.wave & 1;
+    g.wc = WC == 2 ? ((g.wave >> 1) ^ (int) (blockIdx.x >> 3)) & 1 : g.wave >> 1;
     g.lane16 = g.lane * 16;
     g.steps = a.L.steps;
     g.lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void *) lds;
@@ -216,7 +236,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void 
 #pragma unroll
     for (int i = 0; i < G::kBRuns; ++i) {
         const int run = g.wave * G::kBRuns + i;
-        g.b_src[i] = uniform(a.a_codes + (int64_t) token_place(run >> 1) * a.P.steps * 2048 + (run & 1) * 1024);
+        g.b_src[i] = uniform(a.panels + (int64_t) token_place(run >> 1) * a.P.steps * 2048 + (run & 1) * 1024);
     }
 #pragma unroll
     for (int i = 0; i < G::kScales1; ++i) {   // of two row blocks, or of two token blocks
@@ -224,9 +244,10 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void 
         const bool rows = run < RB;
         const int  r = 2 * run + (g.lane >> 5);
         g.s_src[i] = (rows ? matrix(r) + a.L.code_bytes + (int64_t) place(r) * a.L.chunks * 512
-                           : a.a_codes + a.P.code_bytes + (int64_t) token_place(r - 2 * RB) * a.P.chunks * 512) + (g.lane & 31) * 16;
+                           : a.panels + a.P.code_bytes + (int64_t) token_place(r - 2 * RB) * a.P.chunks * 512) + (g.lane & 31) * 16;
     }
-    g.loop();
+    if (g.wc * TB * 32 < tile.count) g.template loop<true>();
+    else g.template loop<false>();
     const int lane = g.lane, wr = g.wr, wc = g.wc;
     if constexpr (MODE == kGateUp) {
 #pragma unroll
@@ -235,38 +256,55 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 4 ? 3 : 2) void 
 #pragma unroll
             for (int q = 0; q < RB / 2; ++q) {
                 const int b = block0 + wr * (RB / 2) + q;
-                if (b < a.L.row_blocks) store_h<true>(a, g.acc[q][t], g.acc[RB / 2 + q][t], lane, token < tile.count, tile.first + token, b);
+                if (b < a.L.row_blocks) store_h(a, g.acc[q][t], g.acc[RB / 2 + q][t], lane, token < tile.count, tile.first + token, b);
             }
         }
     } else {
         // 32 tokens x 64 rows at a time through LDS (a region of the wavefront's own), so that a token's outputs leave as whole lines.
         // (Lines written in halves cost much: 2048 x 17408 outputs in bf16, 64 bytes a token and store, 38 us, in fp32 30.)
         constexpr int kStride = 68;
-        static_assert(RB % 2 == 0 && G::kWaves * 32 * kStride * 4 <= G::kBytes, "a region per wavefront");
+        static_assert(G::kWaves * 32 * kStride * 4 <= G::kBytes, "a region per wavefront");
         float    *mine = reinterpret_cast<float *>(lds) + g.wave * 32 * kStride;
-        const int dtype = MODE == kDown ? RQ_F32 : a.out_dtype;
+        const int dtype = a.out_dtype;   // (kDown: RQ_F32 or kRows16)
+        // (the rows of this wavefront's tokens, a token a lane)
+        int64_t row_at[TB];
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            const int token = (wc * TB + t) * 32 + (lane & 31);
+            row_at[t] = MODE == kDown ? (token < tile.count ? a.row_of[tile.first + token] : 0) : tile.first + token;
+        }
         barrier();   // (the ring is not read any more)
+        if (wc * TB * 32 >= tile.count) return;
+        // LANES of a token write 16 bytes each
+        auto store = [&](auto lanes, int t, int r) __attribute__((always_inline)) {
+            constexpr int kLanes = decltype(lanes)::value, kTokens = 64 / kLanes;
+            const int     n = lane % kLanes * (dtype == RQ_F32 ? 4 : 8), first = (wc * TB + t) * 32;
+            const int64_t n0 = (int64_t) (block0 + wr * RB + r) * 32 + n;
+#pragma unroll
+            for (int i = 0; i < 32 / kTokens; ++i) {
+                const int     at = i * kTokens + lane / kLanes;
+                const int64_t row = MODE == kDown ? __shfl((int) row_at[t], at) : tile.first + first + at;
+                if (first + at < tile.count) {
+                    if (MODE == kDown && dtype == kRows16) store_rows16(a, row, n0, mine + at * kStride + n);
+                    else store_out(dtype, a.y, row * a.ldy, n0, a.L.N, mine + at * kStride + n);
+                }
+            }
+        };
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
 #pragma unroll
             for (int r = 0; r < RB; r += 2) {
+                constexpr int kTwo = RB > 1 ? 2 : 1;   // row blocks at a time
+                static_assert(RB % kTwo == 0, "row blocks in pairs");
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
+                for (int q = 0; q < 4 * kTwo; ++q) {
                     const v16f &c = g.acc[r + q / 4][t];
                     *reinterpret_cast<v4f *>(mine + (lane & 31) * kStride + q * 8 + (lane >> 5) * 4) =
                         v4f{ c[q % 4 * 4], c[q % 4 * 4 + 1], c[q % 4 * 4 + 2], c[q % 4 * 4 + 3] };
                 }
                 __builtin_amdgcn_wave_barrier();
-                const int64_t n0 = (int64_t) (block0 + wr * RB + r) * 32;
-                const int     wide = dtype == RQ_F32 ? 4 : 3;   // (log2 of the lanes of a token: 16 bytes each)
-                const int     step = 64 >> wide, at0 = lane >> wide, n = (lane & ((1 << wide) - 1)) << (6 - wide);
-                for (int at = at0; at < 32; at += step) {
-                    const int token = (wc * TB + t) * 32 + at;
-                    if (token < tile.count) {
-                        const int64_t row = MODE == kDown ? a.row_of[tile.first + token] : tile.first + token;
-                        store_out(dtype, a.y, row * a.ldy, n0 + n, a.L.N, mine + at * kStride + n);
-                    }
-                }
+                if (dtype == RQ_F32) store(std::integral_constant<int, 8 * kTwo>{}, t, r);
+                else store(std::integral_constant<int, 4 * kTwo>{}, t, r);
                 __builtin_amdgcn_wave_barrier();
             }
         }
@@ -286,11 +324,60 @@ hipError_t launch(const ProductArgs &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int MODE>
+hipError_t launch_form(int form, const ProductArgs &a, hipStream_t stream) {
+    if constexpr (MODE == kDense) {
+        switch (form) {
+            case 0: return launch<MODE, 1, 1, 2, 8>(a, stream);
+            case 1: return launch<MODE, 2, 1, 2, 6>(a, stream);
+            case 2: return launch<MODE, 2, 2, 2, 6>(a, stream);
+            case 3: return launch<MODE, 2, 2, 2, 3>(a, stream);
+            case 4: return launch<MODE, 2, 2, 4, 5>(a, stream);
+            default: return launch<MODE, 4, 2, 4, 4>(a, stream);
+        }
+    } else {
+        if (form == kForm64) return launch<MODE, 2, 1, 2, 6>(a, stream);
+        if (form == kForm128) return launch<MODE, 2, 2, 2, 3>(a, stream);
+        return launch<MODE, 4, 2, 2, 3>(a, stream);
+    }
+}
+
+// The forms, and what their tiles take in microseconds: a step of 128 inputs with one tile on a compute unit, a step of every tile of
+// many, and what stands in front of and behind the steps. Measured over K = 1024, 5120, 17408, N = 512 to 17408 and 20 to 2048 tokens:
+// the form that these numbers choose is 1.7 % slower than the fastest of nine on average, 30 % at worst (deep rings cover the latency
+// of few tiles, large tiles spare LDS and L2 where there are many).
+struct Form {
+    int    rows, tokens, resident;   // a tile; tiles that a compute unit holds
+    double alone, full, fixed;
+};
+constexpr Form kForms[kTiledForms] = { { 64, 64, 2, .098, .155, 2.0 },   { 128, 64, 2, .131, .212, 2.2 },  { 128, 128, 1, .187, .358, 2.6 },
+                                       { 128, 128, 2, .405, .310, 2.2 }, { 128, 256, 1, .295, .635, 4.0 }, { 256, 256, 1, .470, .866, 6.0 },
+                                       { 256, 128, 2, 0, 0, 0 } };   // (the last one for the experts only)
+
 }  // namespace
 
-hipError_t launch_tiled(int mode, const ProductArgs &a, hipStream_t stream) {
-    if (mode == kDense) return a.L.steps >= 64 ? launch<kDense, 4, 2, 4, 4>(a, stream) : launch<kDense, 2, 2, 2, 3>(a, stream);
-    return mode == kGateUp ? launch<kGateUp, 4, 2, 2, 3>(a, stream) : launch<kDown, 4, 2, 2, 3>(a, stream);
+int tiled_tokens(int form) { return kForms[form].tokens; }
+int64_t tiled_row_tiles(int mode, int form, int64_t N) {
+    const int rows = mode == kGateUp ? kForms[form].rows / 2 : kForms[form].rows;
+    return (N + rows - 1) / rows;
+}
+int tiled_form(const WeightLayout &L, int64_t M) {
+    int    best = 0;
+    double least = 0;
+    for (int i = 0; i + 1 < kTiledForms; ++i) {
+        const Form   &f = kForms[i];
+        const int64_t tiles = tiled_row_tiles(kDense, i, L.N) * ((M + f.tokens - 1) / f.tokens);
+        const int64_t load = (tiles + 255) / 256, rounds = (load + f.resident - 1) / f.resident;   // of the busiest compute unit
+        const double  alone = f.alone * (double) rounds, full = load > 1 ? f.full * (double) load : 0;
+        const double  price = (double) rounds * f.fixed + (double) L.steps * (full > alone ? full : alone);
+        if (i == 0 || price < least) best = i, least = price;
+    }
+    return best;
+}
+
+hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream) {
+    if (mode == kDense) return launch_form<kDense>(form, a, stream);
+    return mode == kGateUp ? launch_form<kGateUp>(form, a, stream) : launch_form<kDown>(form, a, stream);
 }
 
 }  // namespace mx

@@ -26,22 +26,27 @@ def _dtype(t, what):
 
 def _rows(x, what):
     """(rows, length, row stride) of a matrix on the GPU whose rows' elements are consecutive"""
-    if not x.is_cuda or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
-        raise RqError("%s: a matrix on the GPU with consecutive elements in its rows, got %s on %s with strides %s"
-                      % (what, tuple(x.shape), x.device, x.stride()))
-    M, K = x.shape
-    return M, K, x.stride(0) if M > 1 else K
+    # (a decode step's calls are a few microseconds each on the GPU: every attribute that is asked for shows)
+    if x.dim() == 2 and x.is_cuda:
+        M, K = x.shape
+        ld, one = x.stride()
+        if one == 1 or K == 1:
+            return M, K, ld if M > 1 else K
+    raise RqError("%s: a matrix on the GPU with consecutive elements in its rows, got %s on %s with strides %s"
+                  % (what, tuple(x.shape), x.device, x.stride()))
 
 
-def _same_device(x, **others):
+def _elsewhere(index, **others):
+    """The error for a tensor or weight that is not on GPU `index`"""
     for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise RqError("%s is on %s, the activations are on %s" % (name, t.device, x.device))
+        if t is not None and t.get_device() != index:
+            raise RqError("%s is on GPU %d, the activations are on %d" % (name, t.get_device(), index))
 
 
 def _check_codes(codes, scales):
-    if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() < 2 or codes.shape[:-1] != scales.shape[:-1]
-            or codes.shape[-1] != 16 * scales.shape[-1] or not codes.is_cuda or codes.device != scales.device):
+    shape, blocks = codes.shape, scales.shape
+    if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or len(shape) < 2 or shape[:-1] != blocks[:-1]
+            or shape[-1] != 16 * blocks[-1] or not codes.is_cuda or codes.get_device() != scales.get_device()):
         raise RqError("codes [.., K / 2] and scales [.., K / 32] are uint8 tensors on one GPU, got %s %s on %s and %s %s on %s"
                       % (codes.dtype, tuple(codes.shape), codes.device, scales.dtype, tuple(scales.shape), scales.device))
 
@@ -59,11 +64,12 @@ def mx_quantize(x):
     dt = _dtype(x.dtype, "mx_quantize")
     if K % 32 or K == 0:
         raise RqError("mx_quantize: rows of whole blocks of 32, got %d" % K)
-    codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((M, K // 32), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((M, K // 2), dtype=torch.uint8)
+    scales = x.new_empty((M, K // 32), dtype=torch.uint8)
     if M:
-        _check(_on_device_of(x, load_library().rq_mx4_quantize, dt, x.data_ptr(), ldx, M, K, codes.data_ptr(), scales.data_ptr()),
-               "rq_mx4_quantize")
+        rc = _on_device_of(x, load_library().rq_mx4_quantize, dt, x.data_ptr(), ldx, M, K, codes.data_ptr(), scales.data_ptr())
+        if rc != 0:
+            _check(rc, "rq_mx4_quantize")
     return codes, scales
 
 
@@ -72,11 +78,13 @@ def mx_dequantize(codes, scales, dtype=torch.float32):
     _check_codes(codes, scales)
     dt = _dtype(dtype, "mx_dequantize")
     K = 2 * codes.shape[-1]
-    out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=codes.device)
+    out = codes.new_empty((*codes.shape[:-1], K), dtype=dtype)
     if out.numel():
         codes, scales = _aligned(codes, 4), scales.contiguous()
-        _check(_on_device_of(codes, load_library().rq_mx4_dequantize, dt, codes.data_ptr(), scales.data_ptr(), out.numel() // K, K,
-                             out.data_ptr(), K), "rq_mx4_dequantize")
+        rc = _on_device_of(codes, load_library().rq_mx4_dequantize, dt, codes.data_ptr(), scales.data_ptr(), out.numel() // K, K,
+                           out.data_ptr(), K)
+        if rc != 0:
+            _check(rc, "rq_mx4_dequantize")
     return out
 
 
@@ -91,6 +99,7 @@ class MXWeight:
         self.E = codes.shape[0] if codes.dim() == 3 else 1
         self.N, self.K = codes.shape[-2], 2 * codes.shape[-1]
         self.device = codes.device
+        self._index = codes.get_device()
         L = load_library()
         n = L.rq_mx4_prepared_bytes(self.E, self.N, self.K)
         if n == 0:
@@ -99,36 +108,50 @@ class MXWeight:
         self.prepared = _device_bytes(n, self.device)
         _check(_on_device_of(codes, L.rq_mx4_prepare, codes.data_ptr(), scales.data_ptr(), self.E, self.N, self.K,
                              self.prepared.data_ptr(), n), "rq_mx4_prepare")
+        self._ptr = self.prepared.data_ptr()
+
+    def get_device(self):
+        return self._index
 
     def workspace(self, M):
         return _device_bytes(load_library().rq_mx4_workspace_bytes(self.K, self.N, M), self.device)
 
 
-def _output(out, M, N, x, what):
-    if out is None:
-        return torch.empty((M, N), dtype=x.dtype, device=x.device), N
-    if out.shape != (M, N) or not out.is_cuda or (out.stride(1) != 1 and N != 1) or (M > 1 and out.stride(0) < N):
-        raise RqError("%s: out has to be [%d, %d] on the GPU with consecutive elements in its rows, got %s with strides %s"
-                      % (what, M, N, tuple(out.shape), out.stride()))
-    return out, out.stride(0) if M > 1 else N
+def _output(out, M, N, what):
+    """row stride and type of `out`, checked"""
+    if out.shape == (M, N) and out.is_cuda:
+        ld, one = out.stride()
+        if (one == 1 or N == 1) and (M == 1 or ld >= N):
+            return ld if M > 1 else N, _dtype(out.dtype, what)
+    raise RqError("%s: out has to be [%d, %d] on the GPU with consecutive elements in its rows, got %s with strides %s"
+                  % (what, M, N, tuple(out.shape), out.stride()))
 
 
 def mx_mul_mat(weight, x, out=None, workspace=None):
     """y[M, N] = x^[M, K] . W^T, x^ = x rounded as by mx_quantize, sums in fp32, rounded once to out's type (x's by default)."""
     M, K, ldx = _rows(x, "mx_mul_mat")
+    N = weight.N
     if weight.E != 1 or K != weight.K:
-        raise RqError("mx_mul_mat: activations of %d inputs against a weight of E=%d N=%d K=%d" % (K, weight.E, weight.N, weight.K))
-    dt = _dtype(x.dtype, "mx_mul_mat")
-    out, ldy = _output(out, M, weight.N, x, "mx_mul_mat")
-    odt = _dtype(out.dtype, "mx_mul_mat's out")
-    _same_device(x, weight=weight, out=out, workspace=workspace)
+        raise RqError("mx_mul_mat: activations of %d inputs against a weight of E=%d N=%d K=%d" % (K, weight.E, N, weight.K))
+    odt = dt = _dtype(x.dtype, "mx_mul_mat")
+    ldy = N
+    if out is None:
+        out = x.new_empty((M, N))
+    else:
+        ldy, odt = _output(out, M, N, "mx_mul_mat")
     if M == 0:
         return out
     L = load_library()
+    index = x.get_device()
     if workspace is None:
-        workspace = _device_bytes(L.rq_mx4_workspace_bytes(K, weight.N, M), x.device)
-    rc = _on_device_of(x, L.rq_mx4_mul_mat, weight.prepared.data_ptr(), K, weight.N, dt, x.data_ptr(), ldx, M, odt, out.data_ptr(),
-                       ldy, workspace.data_ptr(), workspace.numel())
+        n = L.rq_mx4_workspace_bytes(K, N, M)
+        workspace = x.new_empty((n,), dtype=torch.uint8)
+    else:
+        n = workspace.numel() * workspace.element_size()
+        _elsewhere(index, workspace=workspace)
+    if weight._index != index or out.get_device() != index:
+        _elsewhere(index, weight=weight, out=out)
+    rc = _on_device_of(x, L.rq_mx4_mul_mat, weight._ptr, K, N, dt, x.data_ptr(), ldx, M, odt, out.data_ptr(), ldy, workspace.data_ptr(), n)
     if rc != 0:
         _check(rc, "rq_mx4_mul_mat")
     return out
@@ -146,11 +169,12 @@ def route(logits, top, scoring="softmax", bias=None, groups=1, top_groups=1, ren
         raise RqError("route: scoring %r is none of %s" % (scoring, sorted(SCORINGS)))
     if groups < 1 or E % groups or not 1 <= top_groups <= groups or not 1 <= top <= top_groups * (E // groups):
         raise RqError("route: %d of %d experts from %d of %d groups" % (top, E, top_groups, groups))
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()):
-        raise RqError("route: bias is fp32 [%d], got %s %s" % (E, bias.dtype, tuple(bias.shape)))
-    _same_device(logits, bias=bias)
-    ids = torch.empty((M, top), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((M, top), dtype=torch.float32, device=logits.device)
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous():
+            raise RqError("route: bias is fp32 [%d], got %s %s" % (E, bias.dtype, tuple(bias.shape)))
+        _elsewhere(logits.get_device(), bias=bias)
+    ids = logits.new_empty((M, top), dtype=torch.int32)
+    weights = logits.new_empty((M, top), dtype=torch.float32)
     if M:
         rc = _on_device_of(logits, load_library().rq_route, dt, logits.data_ptr(), ldl, M, E, SCORINGS[scoring],
                            None if bias is None else bias.data_ptr(), groups, top_groups, top, int(renormalize), float(scale),
@@ -180,19 +204,24 @@ def expert_ffn(gate, up, down, x, ids, weights, out=None, workspace=None):
             or not ids.is_contiguous() or not weights.is_contiguous()):
         raise RqError("expert_ffn: ids int32 and weights fp32 [%d, top], contiguous, got %s %s and %s %s"
                       % (M, ids.dtype, tuple(ids.shape), weights.dtype, tuple(weights.shape)))
-    dt = _dtype(x.dtype, "expert_ffn")
-    out, ldy = _output(out, M, N, x, "expert_ffn")
-    odt = _dtype(out.dtype, "expert_ffn's out")
-    _same_device(x, gate=gate, up=up, down=down, ids=ids, weights=weights, out=out, workspace=workspace)
+    odt = dt = _dtype(x.dtype, "expert_ffn")
+    ldy = N
+    if out is None:
+        out = x.new_empty((M, N))
+    else:
+        ldy, odt = _output(out, M, N, "expert_ffn")
     if M == 0:
         return out
     L = load_library()
-    top = ids.shape[1]
+    index, top = x.get_device(), ids.shape[1]
     if workspace is None:
-        workspace = _device_bytes(L.rq_mx4_experts_workspace_bytes(E, K, F, N, M, top), x.device)
-    rc = _on_device_of(x, L.rq_mx4_experts, gate.prepared.data_ptr(), up.prepared.data_ptr(), down.prepared.data_ptr(), E, K, F, N, dt,
-                       x.data_ptr(), ldx, M, ids.data_ptr(), weights.data_ptr(), top, odt, out.data_ptr(), ldy, workspace.data_ptr(),
-                       workspace.numel())
+        n = L.rq_mx4_experts_workspace_bytes(E, K, F, N, M, top)
+        workspace = x.new_empty((n,), dtype=torch.uint8)
+    else:
+        n = workspace.numel() * workspace.element_size()
+    _elsewhere(index, gate=gate, up=up, down=down, ids=ids, weights=weights, out=out, workspace=workspace)
+    rc = _on_device_of(x, L.rq_mx4_experts, gate._ptr, up._ptr, down._ptr, E, K, F, N, dt, x.data_ptr(), ldx, M, ids.data_ptr(),
+                       weights.data_ptr(), top, odt, out.data_ptr(), ldy, workspace.data_ptr(), n)
     if rc != 0:
         _check(rc, "rq_mx4_experts")
     return out

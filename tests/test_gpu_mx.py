@@ -287,7 +287,7 @@ def _experts(E, F, K, N, seed):
 
 
 def _check_experts(y, x64, mats, ids, w, dtype):
-    want, bound = ref.experts(x64, mats, ids, w)
+    want, bound = ref.experts(x64, mats, ids, w, dtype != torch.float32)
     bound = bound + ROUNDING[dtype] * 1.01 * np.abs(want) + (2.0 ** -25 if dtype == torch.float16 else 0)
     off = np.abs(_host(y) - want)
     assert (off <= bound).all(), "off by %g times the bound" % (off / bound).max()
@@ -335,6 +335,50 @@ def test_experts_skip_ids_that_are_none(M):
     _check_experts(rq.expert_ffn(gate, up, down, x, _gpu(one), _gpu(w)), x64, mats, one, w, torch.float32)
     none = torch.full((M, top), -1, dtype=torch.int32, device=DEV)
     assert (rq.expert_ffn(gate, up, down, x, none, _gpu(w)) == 0).all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 30])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_experts_read_any_rows(M, dtype):
+    """x with a row stride and a start that are not multiples of 16 bytes"""
+    E, K, F, N, top = 4, 96, 64, 40, 2
+    _, (gate, up, down) = _experts(E, F, K, N, 7)
+    x, _ = _activations(M, K, 2, DTYPES[dtype])
+    room = torch.zeros((M, K + 3), dtype=DTYPES[dtype], device=DEV)
+    room[:, 1:1 + K] = x
+    ids = torch.arange(2 * M, device=DEV, dtype=torch.int32).view(M, 2) % E
+    w = torch.rand((M, top), device=DEV)
+    assert torch.equal(rq.expert_ffn(gate, up, down, room[:, 1:1 + K], ids, w), rq.expert_ffn(gate, up, down, x, ids, w))
+    dense = rq.MXWeight(*(_gpu(a) for a in _weights((50,), K, 3)))
+    assert torch.equal(rq.mx_mul_mat(dense, room[:, 1:1 + K]), rq.mx_mul_mat(dense, x))
+
+
+def test_experts_with_many_slots():
+    """more places than are sorted on the chip at once; every token's row as with its experts one at a time"""
+    M, E, top, K, F, N = 3000, 5, 12, 64, 32, 33
+    mats, (gate, up, down) = _experts(E, F, K, N, 5)
+    x, x64 = _activations(M, K, 8, torch.float32)
+    x, x64 = x / 16, x64 / 16
+    rng = np.random.default_rng(1)
+    ids = rng.integers(-1, E, size=(M, top)).astype(np.int32)
+    w = rng.random((M, top)).astype(np.float32)
+    _check_experts(rq.expert_ffn(gate, up, down, x, _gpu(ids), _gpu(w)), x64, mats, ids, w, torch.float32)
+
+
+@pytest.mark.parametrize("M", [2, 40])
+def test_experts_with_nan_and_infinity(M):
+    """a token that holds one is NaN, the others keep their bits"""
+    E, K, F, N, top = 4, 128, 64, 72, 2
+    _, (gate, up, down) = _experts(E, F, K, N, 7)
+    ids = torch.arange(2 * M, device=DEV, dtype=torch.int32).view(M, 2) % E
+    w = torch.rand((M, top), device=DEV)
+    for dtype in DTYPES.values():
+        x, _ = _activations(M, K, 2, dtype)
+        want = rq.expert_ffn(gate, up, down, x / 16, ids, w)
+        bad = x / 16
+        bad[M - 1, 5] = float("inf")
+        y = rq.expert_ffn(gate, up, down, bad, ids, w)
+        assert torch.isnan(y[M - 1]).all() and torch.equal(y[:M - 1], want[:M - 1])
 
 
 @pytest.mark.parametrize("M", [1, 9, 70, 300])
