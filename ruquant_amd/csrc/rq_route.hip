@@ -5,107 +5,170 @@ namespace rq {
 namespace mx {
 namespace {
 
-constexpr int kRouteThreads = 256;
+constexpr int   kRouteThreads = 256;
 constexpr float kLowest = -3.402823466e38f;
 
-// A wavefront per token, expert e in lane e / V, slot e % V, V = values per lane.
+// Over the wavefront by cross-lane operations of the vector ALU: quads, rows of 16, then rows 1 and 3 take their neighbour's, rows 2 and 3
+// the lower half's, and lane 63 has all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v, int other) {
+    return __builtin_amdgcn_update_dpp(other, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_max(int v) {
+    constexpr int kLeast = -2147483647 - 1;   // (so that each step is one instruction)
+    v = max(v, moved<0xB1, 0xF>(v, kLeast));
+    v = max(v, moved<0x4E, 0xF>(v, kLeast));
+    v = max(v, moved<0x141, 0xF>(v, kLeast));
+    v = max(v, moved<0x140, 0xF>(v, kLeast));
+    v = max(v, moved<0x142, 0xA>(v, kLeast));
+    v = max(v, moved<0x143, 0xC>(v, kLeast));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double added(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t) moved<CTRL, ROWS>((int) (uint32_t) b, 0), hi = (uint32_t) moved<CTRL, ROWS>((int) (uint32_t) (b >> 32), 0);
+    return v + __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = added<0xB1, 0xF>(v);
+    v = added<0x4E, 0xF>(v);
+    v = added<0x141, 0xF>(v);
+    v = added<0x140, 0xF>(v);
+    v = added<0x142, 0xA>(v);
+    v = added<0x143, 0xC>(v);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) b, 63), hi = (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) (b >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
+// floats as whole numbers of the same order (no NaN, no -0)
+__device__ __forceinline__ int ordered(float f) {
+    const int b = __float_as_int(f);
+    return b ^ ((b >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7FFFFFFF)); }
+constexpr int kNever = -2147483647 - 1;   // in front of every number: what cannot be chosen
+
+// A wavefront per token, experts V lane .. V lane + V - 1 in a lane. The choice is `top` rounds of a maximum over the wavefront, of whole
+// numbers that have the order of the choices: the lowest lane and place that holds it is the lowest index. Bound by the vector ALU
+// from some thousand tokens on (30 instructions a round), by its latency below.
 template <int DT, int V>
-__global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs a) {
-    const int     lane = threadIdx.x & 63;
-    const int64_t m = (int64_t) blockIdx.x * (kRouteThreads / 64) + (threadIdx.x >> 6);
+__global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs a, const bool vec) {
+    using T = typename Element<DT>::type;
+    const int     lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t m = (int64_t) blockIdx.x * (kRouteThreads / 64) + wave;
     if (m >= a.M) return;
-    const typename Element<DT>::type *x = reinterpret_cast<const typename Element<DT>::type *>(a.logits) + m * a.ldl;
-    float s[V], c[V];
+    const T *x = reinterpret_cast<const T *>(a.logits) + m * a.ldl + lane * V;
+    const int mine = min(max(a.E - lane * V, 0), V);   // experts of this lane
+    float s[V];
+    int   c[V];
+    if (V > 1 && vec) {   // (whole lanes)
+        if constexpr (DT == RQ_F32) {
+            typedef float F __attribute__((ext_vector_type(V)));
+            F f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int   e = lane * V + j;
-        const float f = e < a.E ? to_float(x[e]) : -INFINITY;
-        s[j] = f != f ? -INFINITY : f;
+            for (int j = 0; j < V; ++j) f[j] = -INFINITY;
+            if (mine) f = *reinterpret_cast<const F *>(x);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = f[j];
+        } else {
+            typedef uint16_t H __attribute__((ext_vector_type(V)));
+            H h;
+            if (mine) h = *reinterpret_cast<const H *>(x);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = mine ? to_float(__builtin_bit_cast(T, (uint16_t) h[j])) : -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = j < mine ? to_float(x[j]) : -INFINITY;
     }
-    if (a.scoring == 0) {
-        float top = s[0];
 #pragma unroll
-        for (int j = 1; j < V; ++j) top = fmaxf(top, s[j]);
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        double sum = 0;
+    for (int j = 0; j < V; ++j) s[j] = s[j] != s[j] ? -INFINITY : s[j];
+    if (a.scoring == 0) {
+        int most = kNever;
+#pragma unroll
+        for (int j = 0; j < V; ++j) most = max(most, ordered(s[j]));
+        const float top = unordered(wave_max(most));
+        double      sum = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             s[j] = s[j] == -INFINITY ? 0.0f : s[j] == top ? 1.0f : expf(s[j] - top);
             sum += (double) s[j];
         }
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-        const float by = (float) sum;
+        const float by = (float) wave_sum(sum);
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = by > 0 ? s[j] / by : 0.0f;
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = 1.0f / (1.0f + expf(-s[j]));
     }
-    // what the choice goes by: numbers from the lowest finite one up; what cannot be chosen is minus infinity
+    // what the choice goes by: numbers from the lowest finite one up
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int e = lane * V + j;
-        float     v = s[j];
-        if (a.bias && e < a.E) v += a.bias[e];
-        c[j] = e >= a.E ? -INFINITY : v > kLowest ? v : kLowest;   // (a NaN is not greater)
+        float v = s[j];
+        if (a.bias && j < mine) v += a.bias[lane * V + j];
+        c[j] = j < mine ? ordered(v > kLowest ? v : kLowest) : kNever;   // (a NaN is not greater)
     }
     if (a.groups > 1) {
-        // the groups' worth, a group per lane: its two largest values, found one expert at a time
-        const int size = a.E / a.groups;
-        float worth = -INFINITY;
-        float one = -INFINITY, two = -INFINITY;
-        for (int i = 0; i < size; ++i) {
-            const int e = lane * size + i;
-            float     v = -INFINITY;
+        // 2^share lanes a group find its two largest; the groups' sums are compared by all of their lanes
+        __shared__ int all[kRouteThreads / 64][64 * V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float t = __shfl(c[j], (e / V) & 63);
-                if (e % V == j) v = t;
+        for (int j = 0; j < V; ++j) all[wave][lane * V + j] = c[j];
+        __builtin_amdgcn_wave_barrier();
+        const int size = a.E / a.groups, share = 31 - __clz(64 / a.groups), group = lane >> share, first = lane & ((1 << share) - 1);
+        int       one = kNever, two = kNever;
+        if (group < a.groups) {
+            for (int i = first; i < size; i += 1 << share) {
+                const int v = all[wave][group * size + i];
+                two = max(two, min(one, v));
+                one = max(one, v);
             }
-            if (v > one) two = one, one = v;
-            else if (v > two) two = v;
         }
-        if (lane < a.groups) {
-            worth = size > 1 ? one + two : one;
-            worth = worth > kLowest ? worth : kLowest;
+        for (int o = 1; o < 1 << share; o <<= 1) {
+            const int p = __shfl_xor(one, o), q = __shfl_xor(two, o);
+            two = max(min(one, p), max(two, q));
+            one = max(one, p);
         }
-        // its place among the groups: how many are worth more, or as much in front of it
-        int place = 0;
+        float worth = size > 1 ? unordered(one) + unordered(two) : unordered(one);
+        worth = worth > kLowest ? worth : kLowest;
+        int place = 0;   // groups that are worth more, or as much in front of it
         for (int g = 0; g < a.groups; ++g) {
-            const float v = __shfl(worth, g);
-            place += v > worth || (v == worth && g < lane);
+            const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(worth), g << share));
+            place += v > worth || (v == worth && g < group);
         }
-        const int kept = lane < a.groups && place < a.top_groups;
+        const unsigned long long kept = __ballot(group < a.groups && place < a.top_groups);
+        const float              per = 1.0f / (float) size;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int e = lane * V + j;
-            const int k = __shfl(kept, (e / size) & 63);
-            if (!k || e >= a.E) c[j] = -INFINITY;
+            const int of = (int) (((float) (lane * V + j) + 0.5f) * per);   // (exact: under 1024, and half a unit away from whole numbers)
+            if (!((kept >> (min(of, a.groups - 1) << share)) & 1)) c[j] = kNever;
         }
     }
     float chosen = 0, total = 0;
     int   id = 0;
     for (int i = 0; i < a.top; ++i) {
-        float best = c[0];
-        int   at = 0;
+        int most = c[0];
 #pragma unroll
-        for (int j = 1; j < V; ++j) {
-            if (c[j] > best) best = c[j], at = j;
-        }
-        float all = best;
-        for (int o = 32; o; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
-        const int   from = __ffsll((unsigned long long) __ballot(best == all)) - 1;   // the lowest lane
-        float       w = s[0];
+        for (int j = 1; j < V; ++j) most = max(most, c[j]);
+        const int best = wave_max(most);
+        // (the lane and the place are the wavefront's, so the scalar unit finds them)
+        unsigned long long has[V], any = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) has[j] = __ballot(c[j] == best), any |= has[j];
+        const int from = __builtin_ctzll(any);
+        int       at = 0;
+        float     w = s[0];
+#pragma unroll
+        for (int j = V - 1; j > 0; --j) at = (has[j] >> from) & 1 ? j : at;
+        at = (has[0] >> from) & 1 ? 0 : at;
 #pragma unroll
         for (int j = 1; j < V; ++j) w = at == j ? s[j] : w;
-        w = __shfl(w, from);
-        const int e = __shfl(lane * V + at, from);
-        if (lane == from) {
+        const float picked = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from));
+        const int   e = from * V + at;
 #pragma unroll
-            for (int j = 0; j < V; ++j) c[j] = at == j ? -INFINITY : c[j];
-        }
-        total += w;
-        if (lane == i) chosen = w, id = e;
+        for (int j = 0; j < V; ++j) c[j] = lane == (at == j ? from : -1) ? kNever : c[j];
+        total += picked;
+        if (lane == i) chosen = picked, id = e;
     }
     if (lane < a.top) {
         const float w = a.renormalize ? (total > 0 ? chosen / total : 0.0f) : chosen;
@@ -114,15 +177,20 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
     }
 }
 
+template <int DT, int V>
+void route_with(const RouteArgs &a, hipStream_t stream) {
+    const int64_t bytes = (DT == RQ_F32 ? 4 : 2) * V, align = bytes < 16 ? bytes : 16;
+    const bool    vec = a.E % V == 0 && (uintptr_t) a.logits % align == 0 && (a.M == 1 || a.ldl * (DT == RQ_F32 ? 4 : 2) % align == 0);
+    const dim3    grid((unsigned) ((a.M + kRouteThreads / 64 - 1) / (kRouteThreads / 64)));
+    hipLaunchKernelGGL((rq_route_kernel<DT, V>), grid, dim3(kRouteThreads), 0, stream, a, vec);
+}
 template <int DT>
 hipError_t route(const RouteArgs &a, hipStream_t stream) {
-    const dim3 grid((unsigned) ((a.M + kRouteThreads / 64 - 1) / (kRouteThreads / 64)));
-    const int  v = (a.E + 63) / 64;
-    if (v <= 1) hipLaunchKernelGGL((rq_route_kernel<DT, 1>), grid, dim3(kRouteThreads), 0, stream, a);
-    else if (v <= 2) hipLaunchKernelGGL((rq_route_kernel<DT, 2>), grid, dim3(kRouteThreads), 0, stream, a);
-    else if (v <= 4) hipLaunchKernelGGL((rq_route_kernel<DT, 4>), grid, dim3(kRouteThreads), 0, stream, a);
-    else if (v <= 8) hipLaunchKernelGGL((rq_route_kernel<DT, 8>), grid, dim3(kRouteThreads), 0, stream, a);
-    else hipLaunchKernelGGL((rq_route_kernel<DT, 16>), grid, dim3(kRouteThreads), 0, stream, a);
+    if (a.E <= 64) route_with<DT, 1>(a, stream);
+    else if (a.E <= 128) route_with<DT, 2>(a, stream);
+    else if (a.E <= 256) route_with<DT, 4>(a, stream);
+    else if (a.E <= 512) route_with<DT, 8>(a, stream);
+    else route_with<DT, 16>(a, stream);
     return hipGetLastError();
 }
 
