@@ -47,7 +47,8 @@ int rq_mx4_prepare(const void *codes_dev, const void *scales_dev, int64_t E, int
 
 /* y[m][n] = sum_k x^[m][k] w[n][k], x^ the activations after rq_mx4_quantize's rounding, sums in fp32, rounded once to out_dtype.
  * x: M rows, stride ldx elements, any alignment of its type; y: row stride ldy elements. workspace: 256-byte aligned,
- * rq_mx4_workspace_bytes, need not be initialised, not shared by calls that can overlap. */
+ * rq_mx4_workspace_bytes, need not be initialised, not shared by calls that can overlap; where that is 256 (a few tokens, which
+ * the product quantises as it reads them) it is not looked at and may be null. */
 size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M);
 int rq_mx4_mul_mat(const void *prepared_dev, int64_t K, int64_t N, int in_dtype, const void *x_dev, int64_t ldx, int64_t M,
                    int out_dtype, void *y_dev, int64_t ldy, void *workspace_dev, size_t workspace_bytes, rq_stream_t stream);

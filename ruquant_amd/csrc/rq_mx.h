@@ -1,6 +1,8 @@
 // Shared definitions of the MXFP4 operators: layouts, element conversions and launch arguments.
 #pragma once
 
+#include <atomic>
+
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -118,6 +120,18 @@ __device__ __forceinline__ v16f mfma(const v4i &a, const v4i &b, const v16f &c, 
     const v8i A = { a[0], a[1], a[2], a[3], 0, 0, 0, 0 };
     const v8i B = { b[0], b[1], b[2], b[3], 0, 0, 0, 0 };
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, J, sa, J, sb);
+}
+
+// Lets a kernel have so much dynamic LDS, once per device; `allowed` has a bit for each.
+inline hipError_t allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &allowed) {
+    int        dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (allowed.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // ---- launches ---------------------------------------------------------------------------------------

@@ -78,6 +78,7 @@ bool good_experts(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top
 
 extern "C" size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M) {
     if (rq_mx4_prepared_bytes(1, N, K) == 0 || M < 0 || M > kMaxTokens) return 0;
+    if (decode_takes(M, K, N)) return 256;   // (not looked at)
     const ActLayout A = act_layout(K);
     return (size_t) (M > kDecodeTokens ? weight_layout(M, K).expert_bytes : pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
 }
@@ -91,7 +92,7 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
         (M > 1 && (ldx < K || ldy < N))) {
         return RQ_E_ARGUMENT;
     }
-    if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return RQ_E_WORKSPACE;
+    if (!decode_takes(M, K, N) && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
     if (M <= kDecodeTokens) {
         DecodeArgs d = {};

@@ -316,9 +316,10 @@ hipError_t launch(const ProductArgs &a, hipStream_t stream) {
     using G = Tiled<MODE, RB, TB, WC, R>;
     const int row_tiles = (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
     const int token_tiles = MODE == kDense ? (int) ((a.M + G::kTileTokens - 1) / G::kTileTokens) : a.most_tiles;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, G::kBytes);
-    if (set != hipSuccess) return set;
+    if ((int64_t) row_tiles * token_tiles > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    static std::atomic<uint64_t> allowed{ 0 };   // devices on which the kernel may have its LDS
+    const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R>), G::kBytes, allowed);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE, RB, TB, WC, R>), dim3((unsigned) row_tiles * token_tiles), dim3(G::kThreads), G::kBytes, stream,
                        a, row_tiles, token_tiles);
     return hipGetLastError();

@@ -358,10 +358,9 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t stream) {
 }
 
 hipError_t launch_sort(const SortArgs &a, hipStream_t stream) {
-    constexpr int kMost = kSortLds * sizeof(int);
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(rq_sort_kernel),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
-    if (set != hipSuccess) return set;
+    static std::atomic<uint64_t> allowed{ 0 };
+    const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_sort_kernel), kSortLds * (int) sizeof(int), allowed);
+    if (e != hipSuccess) return e;
     const int bytes = a.positions <= kSortLds ? a.positions * (int) sizeof(int) : 0;
     hipLaunchKernelGGL(rq_sort_kernel, dim3(1), dim3(kSortThreads), bytes, stream, a);
     return hipGetLastError();

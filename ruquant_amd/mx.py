@@ -144,14 +144,16 @@ def mx_mul_mat(weight, x, out=None, workspace=None):
     L = load_library()
     index = x.get_device()
     if workspace is None:
-        n = L.rq_mx4_workspace_bytes(K, N, M)
-        workspace = x.new_empty((n,), dtype=torch.uint8)
+        n, at = L.rq_mx4_workspace_bytes(K, N, M), None
+        if n > 256:   # (256: nothing that the call looks at)
+            workspace = x.new_empty((n,), dtype=torch.uint8)
+            at = workspace.data_ptr()
     else:
-        n = workspace.numel() * workspace.element_size()
+        n, at = workspace.numel() * workspace.element_size(), workspace.data_ptr()
         _elsewhere(index, workspace=workspace)
     if weight._index != index or out.get_device() != index:
         _elsewhere(index, weight=weight, out=out)
-    rc = _on_device_of(x, L.rq_mx4_mul_mat, weight._ptr, K, N, dt, x.data_ptr(), ldx, M, odt, out.data_ptr(), ldy, workspace.data_ptr(), n)
+    rc = _on_device_of(x, L.rq_mx4_mul_mat, weight._ptr, K, N, dt, x.data_ptr(), ldx, M, odt, out.data_ptr(), ldy, at, n)
     if rc != 0:
         _check(rc, "rq_mx4_mul_mat")
     return out

@@ -460,8 +460,8 @@ def test_refusals():
         lambda: rq.mx_mul_mat(W, x, out=torch.zeros((2, 5), device=DEV)), lambda: rq.mx_mul_mat(W, x, out=torch.zeros((2, 4), device="cpu")),
         lambda: rq.mx_mul_mat(W, x, out=torch.zeros((2, 4), dtype=torch.int32, device=DEV)),
         lambda: rq.mx_mul_mat(W, x, out=torch.zeros((1, 4), device=DEV).expand(2, 4)),
-        lambda: rq.mx_mul_mat(W, x, workspace=torch.empty(256, dtype=torch.uint8, device=DEV)[:16]),
-        lambda: rq.mx_mul_mat(W, x, workspace=torch.empty(1 << 20, dtype=torch.uint8, device=DEV)[1:]),
+        lambda: rq.mx_mul_mat(W, x.repeat(20, 1), workspace=torch.empty(256, dtype=torch.uint8, device=DEV)[:16]),
+        lambda: rq.mx_mul_mat(W, x.repeat(20, 1), workspace=torch.empty(1 << 20, dtype=torch.uint8, device=DEV)[1:]),
         lambda: rq.route(x, 0), lambda: rq.route(x, 65), lambda: rq.route(x, 33), lambda: rq.route(x, 2, scoring="relu"),
         lambda: rq.route(x, 2, groups=5), lambda: rq.route(x, 2, groups=4, top_groups=5), lambda: rq.route(x, 17, groups=4),
         lambda: rq.route(x, 2, bias=torch.zeros(63, device=DEV)), lambda: rq.route(x, 2, bias=torch.zeros(64, device=DEV).half()),
@@ -478,3 +478,11 @@ def test_refusals():
             pytest.fail("call %d was not refused" % i)
     assert rq.mx_mul_mat(W, x[:0]).shape == (0, 4) and rq.expert_ffn(gate, gate, down, x[:0], ids[:0], w[:0]).shape == (0, 64)
     assert rq.route(x[:0], 3)[0].shape == (0, 3)
+
+
+def test_example_runs():
+    """The mixture layer of examples/: rounding weights and activations to four bits (a unit in 8 to 16 of a block's largest) leaves its output
+    within a third of the fp32 one, and not nearer than a thirtieth."""
+    from examples.mixture_layer import main
+    off = main(["--tokens", "1,5,70,200", "--hidden", "512", "--expert", "160", "--experts", "8", "--top", "3"])
+    assert len(off) == 4 and all(1 / 30 < v < 1 / 3 for v in off), off
