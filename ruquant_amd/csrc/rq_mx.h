@@ -159,6 +159,7 @@ constexpr int kRows16 = 3;
 struct ProductArgs {
     WeightLayout   L;
     const uint8_t *w, *w2;          // prepared weights; kGateUp: w the gate, w2 the up projection
+    int            first_block, row_tiles;   // kDense: the row blocks of this launch start here
     const uint8_t *panels;          // the activations
     WeightLayout   P;
     int64_t        M;               // tokens (kDense)
@@ -296,8 +297,8 @@ hipError_t launch_decode_experts(int dtype, const DecodeArgs &gate_up, const Dec
 
 // more tokens: both operands through LDS, in tiles of several forms
 constexpr int kTiledForms = 7, kForm64 = 1, kForm128 = 3, kForm256 = 6;   // (the experts': 128 x 64, 128 x 128, 256 x 128 rows x tokens)
-hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream);
-int tiled_form(const WeightLayout &L, int64_t M);   // for a plain product
+hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream);   // the experts'
+hipError_t launch_tiled_product(const ProductArgs &a, hipStream_t stream);               // a plain one, planned by its size
 int tiled_tokens(int form);
 int64_t tiled_row_tiles(int mode, int form, int64_t N);
 

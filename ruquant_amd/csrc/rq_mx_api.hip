@@ -125,7 +125,7 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
     a.ldy = ldy;
     a.P = weight_layout(M, K);
     const hipError_t e = launch_panel_quantize(in_dtype, x, ldx, a.P, nullptr, nullptr, (uint8_t *) workspace, st);
-    return e != hipSuccess ? e : launch_tiled(kDense, tiled_form(a.L, M), a, st);
+    return e != hipSuccess ? e : launch_tiled_product(a, st);
 }
 
 extern "C" int rq_route(int dtype, const void *logits, int64_t ldl, int64_t M, int64_t E, int scoring, const float *bias, int groups,

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     g.as_lds = lds + G::kScales + g.wr * RB * 512 + g.lane * 4;
     g.bs_lds = lds + G::kScales + (G::kABlocks + g.wc * TB) * 512 + g.lane * 4;
     constexpr int  kBlocks = G::kTileRows / 32;   // row blocks of the tile, per matrix
-    const int      block0 = row_tile * kBlocks;
+    const int      block0 = (MODE == kDense ? a.first_block : 0) + row_tile * kBlocks;
     const uint8_t *w = a.w + (int64_t) tile.expert * a.L.expert_bytes;
     const uint8_t *w2 = MODE == kGateUp ? a.w2 + (int64_t) tile.expert * a.L.expert_bytes : w;
     // row block i of the tile, in the order of its wavefronts: its matrix and place; blocks past the weight's repeat its last one
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
 template <int MODE, int RB, int TB, int WC, int R>
 hipError_t launch(const ProductArgs &a, hipStream_t stream) {
     using G = Tiled<MODE, RB, TB, WC, R>;
-    const int row_tiles = (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
+    const int row_tiles = MODE == kDense ? a.row_tiles : (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
     const int token_tiles = MODE == kDense ? (int) ((a.M + G::kTileTokens - 1) / G::kTileTokens) : a.most_tiles;
     if ((int64_t) row_tiles * token_tiles > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     static std::atomic<uint64_t> allowed{ 0 };   // devices on which the kernel may have its LDS
@@ -362,22 +362,55 @@ int64_t tiled_row_tiles(int mode, int form, int64_t N) {
     const int rows = mode == kGateUp ? kForms[form].rows / 2 : kForms[form].rows;
     return (N + rows - 1) / rows;
 }
-int tiled_form(const WeightLayout &L, int64_t M) {
-    int    best = 0;
-    double least = 0;
-    for (int i = 0; i + 1 < kTiledForms; ++i) {
-        const Form   &f = kForms[i];
-        const int64_t tiles = tiled_row_tiles(kDense, i, L.N) * ((M + f.tokens - 1) / f.tokens);
-        const int64_t load = (tiles + 255) / 256, rounds = (load + f.resident - 1) / f.resident;   // of the busiest compute unit
-        const double  alone = f.alone * (double) rounds, full = load > 1 ? f.full * (double) load : 0;
-        const double  price = (double) rounds * f.fixed + (double) L.steps * (full > alone ? full : alone);
-        if (i == 0 || price < least) best = i, least = price;
+namespace {
+
+double price(int form, int64_t tiles, int64_t steps) {
+    const Form   &f = kForms[form];
+    const int64_t load = (tiles + 255) / 256, rounds = (load + f.resident - 1) / f.resident;   // of the busiest compute unit
+    const double  alone = f.alone * (double) rounds, full = load > 1 ? f.full * (double) load : 0;
+    return (double) rounds * f.fixed + (double) steps * (full > alone ? full : alone);
+}
+
+}  // namespace
+
+// A product is one launch in the form of the least price, or two: as many row tiles as fill whole rounds of the chip in one form, and the
+// rows behind them, which would leave most of it idle for a round, in another. (17408 x 5120 at 2048 tokens: 544 tiles of 256 x 256 are
+// two rounds and 32 tiles.)
+hipError_t launch_tiled_product(const ProductArgs &a, hipStream_t stream) {
+    constexpr int    kPlain = kTiledForms - 1;
+    constexpr double kLaunch = 2.0;
+    const int64_t    rows = (int64_t) a.L.row_blocks * 32, steps = a.L.steps;
+    auto token_tiles = [&](int f) { return (a.M + kForms[f].tokens - 1) / kForms[f].tokens; };
+    auto row_tiles = [&](int f, int64_t n) { return (n + kForms[f].rows - 1) / kForms[f].rows; };
+    double  least = 0;
+    int     form = -1, rest = -1;
+    int64_t main_tiles = 0;
+    for (int f = 0; f < kPlain; ++f) {
+        const int64_t tokens = token_tiles(f), all = row_tiles(f, rows);
+        const double  whole = price(f, all * tokens, steps);
+        if (form < 0 || whole < least) least = whole, form = f, rest = -1, main_tiles = all;
+        const int64_t round = 256 * kForms[f].resident, rounds = all * tokens / round;
+        for (int64_t k = rounds; k > 0 && k > rounds - 2; --k) {
+            const int64_t n = k * round / tokens;   // row tiles
+            if (n == 0 || n >= all) continue;
+            const double some = price(f, n * tokens, steps) + kLaunch;
+            for (int g = 0; g < kPlain; ++g) {
+                const double p = some + price(g, row_tiles(g, rows - n * kForms[f].rows) * token_tiles(g), steps);
+                if (p < least) least = p, form = f, rest = g, main_tiles = n;
+            }
+        }
     }
-    return best;
+    ProductArgs one = a;
+    one.first_block = 0;
+    one.row_tiles = (int) main_tiles;
+    hipError_t e = launch_form<kDense>(form, one, stream);
+    if (e != hipSuccess || rest < 0) return e;
+    one.first_block = (int) (main_tiles * kForms[form].rows / 32);
+    one.row_tiles = (int) row_tiles(rest, rows - main_tiles * kForms[form].rows);
+    return launch_form<kDense>(rest, one, stream);
 }
 
 hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream) {
-    if (mode == kDense) return launch_form<kDense>(form, a, stream);
     return mode == kGateUp ? launch_form<kGateUp>(form, a, stream) : launch_form<kDown>(form, a, stream);
 }
 
