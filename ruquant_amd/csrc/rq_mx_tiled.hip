@@ -36,21 +36,19 @@ struct Tiled {
     static constexpr int kWaves = 2 * WC, kThreads = 64 * kWaves;
     static constexpr int kABlocks = 2 * RB, kBBlocks = WC * TB;
     static constexpr int kSlot = (kABlocks + kBBlocks) * 2048;   // one step of both operands
-    // Behind the ring the scales, a chunk a slot. A short ring has one slot: the next chunk is fetched by the second step of a chunk, when
-    // its own has been read. A longer one would wait for that too early: there a chunk is fetched with its first step.
-    static constexpr bool kAhead = R > 4;
-    static constexpr int  kScaleSlots = kAhead ? (R + 5) / 4 : 1, kScaleSlot = (kABlocks + kBBlocks) * 512;
-    static constexpr int  kScales = R * kSlot, kBytes = kScales + kScaleSlots * kScaleSlot;
-    // 1 KiB each, of a wavefront per step; runs of the scales per chunk (some are fetched twice so that all fetch as many)
+    // Behind the ring the scales, a part (two steps) a slot: row blocks, then token blocks, 256 bytes each, moved four at a time.
+    static constexpr int kScaleRuns = (kABlocks + kBBlocks + 3) / 4, kScaleSlot = kScaleRuns * 1024, kScaleSlots = (R + 1) / 2;
+    static constexpr int kScales = R * kSlot, kBytes = kScales + kScaleSlots * kScaleSlot;
+    // 1 KiB each, of a wavefront per step, and of a part's scales (some are fetched twice so that all fetch as many)
     static constexpr int kARuns = 2 * kABlocks / kWaves, kBRuns = 2 * kBBlocks / kWaves, kRuns = kARuns + kBRuns;
-    static constexpr int kScaleRuns = (kABlocks + kBBlocks) / 2, kScales1 = (kScaleRuns + kWaves - 1) / kWaves;
-    static_assert(2 * kABlocks % kWaves == 0 && 2 * kBBlocks % kWaves == 0 && kBBlocks % 2 == 0, "split of the loads");
+    static constexpr int kPartRuns = (kScaleRuns + kWaves - 1) / kWaves;
+    static_assert(2 * kABlocks % kWaves == 0 && 2 * kBBlocks % kWaves == 0, "split of the loads");
     static constexpr int kTileRows = MODE == kGateUp ? 32 * RB : 64 * RB;            // (of each matrix)
     static constexpr int kTileTokens = 32 * WC * TB;
 
     // what this wavefront moves
     const uint8_t *a_src[kARuns], *b_src[kBRuns];   // wave-uniform
-    const uint8_t *s_src[kScales1];                 // the lane's
+    const uint8_t *s_src[kPartRuns];                // the lane's
     uint32_t       lds0, lane16;
     int            wave, wr, wc, lane, steps;
     const uint8_t *a_lds, *b_lds, *as_lds, *bs_lds;   // this lane's places in slot 0
@@ -63,11 +61,11 @@ struct Tiled {
         if (i < kARuns) load_run(a_src[i] + (int64_t) t * 2048, lane16, to + (wave * kARuns + i) * 1024);
         else load_run(b_src[i - kARuns] + (int64_t) t * 2048, lane16, to + (2 * kABlocks + wave * kBRuns + i - kARuns) * 1024);
     }
-    static __device__ __forceinline__ int scale_slot(int c) { return kAhead ? c % kScaleSlots * kScaleSlot : 0; }
-    __device__ __forceinline__ void fetch_scales(int c) {
+    static __device__ __forceinline__ int scale_slot(int part) { return part % kScaleSlots * kScaleSlot; }
+    __device__ __forceinline__ void fetch_scales(int part) {
 #pragma unroll
-        for (int i = 0; i < kScales1; ++i)
-            load_run(s_src[i] + (int64_t) c * 512, lds0 + kScales + scale_slot(c) + (i * kWaves + wave) % kScaleRuns * 1024);
+        for (int i = 0; i < kPartRuns; ++i)
+            load_run(s_src[i] + (int64_t) part * 256, lds0 + kScales + scale_slot(part) + (i * kWaves + wave) % kScaleRuns * 1024);
     }
     __device__ __forceinline__ void read_a(int slot, int i) {
 #pragma unroll
@@ -77,29 +75,26 @@ struct Tiled {
 #pragma unroll
         for (int h = 0; h < 2; ++h) B[i][h] = *reinterpret_cast<const v4i *>(b_lds + slot * kSlot + (2 * i + h) * 1024);
     }
-    // the scales of inputs 256 part .. + 255
-    __device__ __forceinline__ void read_sa(int part, int i) {
-        sA[i] = *reinterpret_cast<const int *>(as_lds + scale_slot(part >> 1) + i * 512 + (part & 1) * 256);
-    }
+    __device__ __forceinline__ void read_sa(int part, int i) { sA[i] = *reinterpret_cast<const int *>(as_lds + scale_slot(part) + i * 256); }
     __device__ __forceinline__ void read_sb(int (&sB)[TB], int part, int i) const {
-        sB[i] = *reinterpret_cast<const int *>(bs_lds + scale_slot(part >> 1) + i * 512 + (part & 1) * 256);
+        sB[i] = *reinterpret_cast<const int *>(bs_lds + scale_slot(part) + i * 256);
     }
 
-    // Step t = 4 c + J: its products from A and B, behind each row block's the read of its fragments of step t + 1, between them the
-    // reads of step t + 1's activations into N and the fetch of step t + R - 1 into the slot of step t - 1 (whose reads the products
-    // of step t - 1 have waited for, in every wavefront that has passed this step's barrier). The scales are read every second
-    // step, those of the next chunk by the fourth of this one. (Ahead: chunk c is fetched by step 4 c - R + 1, into a slot whose last
-    // reads, of chunk c - S, the products of step 4 (c - S) + 2 have waited for; 4 S >= R + 2.) MORE: all of those steps exist.
+    // Step t (t % 2 == J): its products from A and B, behind each row block's the read of its fragments of step t + 1, between them the
+    // reads of step t + 1's activations into N and the fetch of step t + R - 1 into the slot of step t - 1. Who has passed this step's
+    // barrier has issued the products of step t - 1, which waited for that slot's reads. The scales of part q are read by step 2 q - 1
+    // and waited for by the products of step 2 q; part p is fetched with step 2 p, behind the barrier of step 2 p - R + 1, into the slot of part
+    // p - S, whose reads are past from the barrier of step 2 (p - S) + 1 on: 2 S >= R. MORE: all of those steps exist.
     template <bool ACTIVE, int J, bool MORE>
     __device__ __forceinline__ void step(int t, int slot, const v4i (&B)[TB][2], v4i (&N)[TB][2], int (&sB)[TB], int (&sN)[TB]) {
         const int  next = slot + 1 == R ? 0 : slot + 1, last = slot == 0 ? R - 1 : slot - 1;
         const bool get = MORE || t + R - 1 < steps;
         // step t + 1 has arrived; those behind it need not have
-        constexpr int kChunks = kAhead ? ((J + R - 2) >> 2) - ((J + 1) >> 2) : MORE && J == 2;   // chunks' scales among those
-        if (MORE || t + R - 2 < steps) wait_loads<(R - 3) * kRuns + kChunks * kScales1>();
+        constexpr int kParts = (J + R - 2) / 2 - (J + 1) / 2;   // first steps of a part, which bring its scales, among those
+        if (MORE || t + R - 2 < steps) wait_loads<(R - 3) * kRuns + kParts * kPartRuns>();
         else wait_loads<0>();
         barrier();
-        if (kAhead && (J + R - 1) % 4 == 0 && get) fetch_scales((t + R - 1) >> 2);
+        if ((J + R - 1) % 2 == 0 && get) fetch_scales((t + R - 1) >> 1);
         if (!MORE && get) {
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) fetch_run(t + R - 1, last, i);
@@ -108,12 +103,12 @@ struct Tiled {
         for (int r = 0; r < RB; ++r) {
             if constexpr (ACTIVE) {
 #pragma unroll
-                for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1)>(A[r][0], B[b][0], acc[r][b], sA[r], sB[b]);
+                for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * J>(A[r][0], B[b][0], acc[r][b], sA[r], sB[b]);
                 // (past the last step: what the ring holds, for nobody)
 #pragma unroll
                 for (int i = r * TB / RB; i < (r + 1) * TB / RB; ++i) {
                     read_b(N, next, i);
-                    if (J & 1) read_sb(sN, (t >> 1) + 1, i);
+                    if (J == 1) read_sb(sN, (t >> 1) + 1, i);
                 }
             }
             if (MORE) {
@@ -123,17 +118,16 @@ struct Tiled {
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (ACTIVE) {
 #pragma unroll
-                for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * (J & 1) + 1>(A[r][1], B[b][1], acc[r][b], sA[r], sB[b]);
+                for (int b = 0; b < TB; ++b) acc[r][b] = mfma<2 * J + 1>(A[r][1], B[b][1], acc[r][b], sA[r], sB[b]);
                 read_a(next, r);
-                if (J & 1) read_sa((t >> 1) + 1, r);
+                if (J == 1) read_sa((t >> 1) + 1, r);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (ACTIVE && (J & 1)) {
+        if constexpr (ACTIVE && J == 1) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) sB[i] = sN[i];
         }
-        if (!kAhead && J == 1 && (MORE || t + 3 < steps)) fetch_scales((t >> 2) + 1);
     }
 
     // ACTIVE: this wavefront has tokens; otherwise it moves its share and keeps the barriers
@@ -143,16 +137,15 @@ struct Tiled {
         for (int r = 0; r < RB; ++r)
 #pragma unroll
             for (int t = 0; t < TB; ++t) acc[r][t] = v16f{ 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 };
-        if (!kAhead) fetch_scales(0);
 #pragma unroll
         for (int t = 0; t < R - 1; ++t) {
             if (t < steps) {
-                if (kAhead && t % 4 == 0) fetch_scales(t >> 2);
+                if (t % 2 == 0) fetch_scales(t >> 1);
 #pragma unroll
                 for (int i = 0; i < kRuns; ++i) fetch_run(t, t, i);
             }
         }
-        if (steps >= R - 1) wait_loads<(R - 2) * kRuns + (kAhead ? (R - 2) / 4 : 0) * kScales1>();
+        if (steps >= R - 1) wait_loads<(R - 2) * kRuns + (R - 2) / 2 * kPartRuns>();
         else wait_loads<0>();
         barrier();
         v4i B[TB][2], N[TB][2];
@@ -163,20 +156,14 @@ struct Tiled {
         for (int i = 0; i < TB; ++i) read_b(B, 0, i), read_sb(sB, 0, i);
         int  t = 0, slot = 0;
         auto next = [&]() __attribute__((always_inline)) { ++t, slot = slot + 1 == R ? 0 : slot + 1; };
-        while (t + R + 2 < steps) {
+        while (t + R < steps) {
             step<ACTIVE, 0, true>(t, slot, B, N, sB, sN), next();
             step<ACTIVE, 1, true>(t, slot, N, B, sB, sN), next();
-            step<ACTIVE, 2, true>(t, slot, B, N, sB, sN), next();
-            step<ACTIVE, 3, true>(t, slot, N, B, sB, sN), next();
         }
         while (true) {
             step<ACTIVE, 0, false>(t, slot, B, N, sB, sN), next();
             if (t >= steps) break;
             step<ACTIVE, 1, false>(t, slot, N, B, sB, sN), next();
-            if (t >= steps) break;
-            step<ACTIVE, 2, false>(t, slot, B, N, sB, sN), next();
-            if (t >= steps) break;
-            step<ACTIVE, 3, false>(t, slot, N, B, sB, sN), next();
             if (t >= steps) break;
         }
         wait_loads<0>();   // (none of this wavefront's loads lands in LDS behind this)
@@ -213,8 +200,8 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     g.lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void *) lds;
     g.a_lds = lds + g.wr * RB * 2048 + g.lane * 16;
     g.b_lds = lds + (2 * G::kABlocks + g.wc * TB * 2) * 1024 + g.lane * 16;
-    g.as_lds = lds + G::kScales + g.wr * RB * 512 + g.lane * 4;
-    g.bs_lds = lds + G::kScales + (G::kABlocks + g.wc * TB) * 512 + g.lane * 4;
+    g.as_lds = lds + G::kScales + g.wr * RB * 256 + g.lane * 4;
+    g.bs_lds = lds + G::kScales + (G::kABlocks + g.wc * TB) * 256 + g.lane * 4;
     constexpr int  kBlocks = G::kTileRows / 32;   // row blocks of the tile, per matrix
     const int      block0 = (MODE == kDense ? a.first_block : 0) + row_tile * kBlocks;
     const uint8_t *w = a.w + (int64_t) tile.expert * a.L.expert_bytes;
@@ -239,12 +226,10 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
         g.b_src[i] = uniform(a.panels + (int64_t) token_place(run >> 1) * a.P.steps * 2048 + (run & 1) * 1024);
     }
 #pragma unroll
-    for (int i = 0; i < G::kScales1; ++i) {   // of two row blocks, or of two token blocks
-        const int  run = (i * G::kWaves + g.wave) % G::kScaleRuns;
-        const bool rows = run < RB;
-        const int  r = 2 * run + (g.lane >> 5);
-        g.s_src[i] = (rows ? matrix(r) + a.L.code_bytes + (int64_t) place(r) * a.L.chunks * 512
-                           : a.panels + a.P.code_bytes + (int64_t) token_place(r - 2 * RB) * a.P.chunks * 512) + (g.lane & 31) * 16;
+    for (int i = 0; i < G::kPartRuns; ++i) {   // of four blocks, row blocks first (past the last one it again)
+        const int r = min((i * G::kWaves + g.wave) % G::kScaleRuns * 4 + (g.lane >> 4), G::kABlocks + G::kBBlocks - 1);
+        g.s_src[i] = (r < G::kABlocks ? matrix(r) + a.L.code_bytes + (int64_t) place(r) * a.L.chunks * 512
+                                      : a.panels + a.P.code_bytes + (int64_t) token_place(r - G::kABlocks) * a.P.chunks * 512) + (g.lane & 15) * 16;
     }
     if (g.wc * TB * 32 < tile.count) g.template loop<true>();
     else g.template loop<false>();

@@ -184,6 +184,24 @@ def test_product_rows_do_not_depend_on_the_others(M):
     assert torch.equal(rq.mx_mul_mat(W, other)[-1], y[-1])
 
 
+@pytest.mark.parametrize("M,K,N", [(300, 1024, 70000), (520, 2080, 70000), (1000, 640, 40000), (200, 1376, 90000), (65, 8192, 70000),
+                                   (2000, 384, 20000), (300, 17408, 9000)])
+def test_product_of_many_tiles_is_that_of_few(M, K, N):
+    """Every tile adds up the inputs in the same order, so a product whose tiles go over the chip in several rounds has the same bits as that
+    of its tokens some at a time, and as itself again: nothing of a tile's neighbours, or of a wavefront that is behind, shows."""
+    g = torch.Generator(device=DEV).manual_seed(M + K)
+    codes = torch.empty((N, K // 2), dtype=torch.uint8, device=DEV).random_(0, 256, generator=g)
+    scales = torch.empty((N, K // 32), dtype=torch.uint8, device=DEV).random_(116, 124, generator=g)
+    W = rq.MXWeight(codes, scales)
+    x = torch.randn((M, K), device=DEV, generator=g)
+    y = rq.mx_mul_mat(W, x)
+    for _ in range(3):
+        assert torch.equal(rq.mx_mul_mat(W, x), y)
+    for i in range(0, M, 100):   # (at least 17 tokens: fewer add up in another order)
+        part = x[min(i, M - 60):i + 100]
+        assert torch.equal(rq.mx_mul_mat(W, part), y[min(i, M - 60):i + 100])
+
+
 @pytest.mark.parametrize("M", [1, 18, 130])
 def test_product_with_nan_and_infinity(M):
     """a NaN in a token makes its row NaN and no other; a NaN scale of a weight makes its row's outputs NaN and no other"""
@@ -379,6 +397,24 @@ def test_experts_with_nan_and_infinity(M):
         bad[M - 1, 5] = float("inf")
         y = rq.expert_ffn(gate, up, down, bad, ids, w)
         assert torch.isnan(y[M - 1]).all() and torch.equal(y[:M - 1], want[:M - 1])
+
+
+@pytest.mark.parametrize("E,top,M,K,F,N", [(32, 6, 2000, 1024, 640, 2048), (8, 2, 3000, 2048, 256, 1024), (60, 4, 600, 1376, 352, 1000)])
+def test_experts_of_many_tiles_are_repeatable(E, top, M, K, F, N):
+    """The same bits again and again, and for a part of the tokens (whose tiles are others)."""
+    g = torch.Generator(device=DEV).manual_seed(M)
+    weight = lambda *shape: rq.MXWeight(  # noqa: E731
+        torch.empty((*shape[:-1], shape[-1] // 2), dtype=torch.uint8, device=DEV).random_(0, 256, generator=g),
+        torch.empty((*shape[:-1], shape[-1] // 32), dtype=torch.uint8, device=DEV).random_(117, 121, generator=g))
+    gate, up, down = weight(E, F, K), weight(E, F, K), weight(E, N, F)
+    x = torch.randn((M, K), device=DEV, generator=g).bfloat16()
+    ids = torch.randn((M, E), device=DEV, generator=g).topk(top, dim=1).indices.int()
+    w = torch.rand((M, top), device=DEV, generator=g)
+    y = rq.expert_ffn(gate, up, down, x, ids, w)
+    for _ in range(4):
+        assert torch.equal(rq.expert_ffn(gate, up, down, x, ids, w), y)
+    for i in range(0, M, 500):
+        assert torch.equal(rq.expert_ffn(gate, up, down, x[i:i + 500], ids[i:i + 500], w[i:i + 500]), y[i:i + 500])
 
 
 @pytest.mark.parametrize("M", [1, 9, 70, 300])
