@@ -151,9 +151,10 @@ struct Tile {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
-// Rows of the slots in 16 bits, for outputs of 16 bits: whole numbers up to 2^15 of a unit that 32 outputs share, 2^(X - 141), X the
-// exponent of the largest (16 .. 254; 255: one of them is not finite, and all 32 read as NaN). Each output is off by at most 2^-15 of
-// the 32's largest, 1 / 100 of what its last rounding to bf16 costs, and the rows' traffic, which is what their sum takes, is halved.
+// Rows of the slots in 16 bits, for outputs in bf16: fp16 numbers of a unit that 32 outputs share, 2^(X - 141), X the exponent of the
+// largest finite one (16 .. 254), which lies under 2^15 of it. An output is off by at most 2^-11 of itself, 1 / 8 of what its last rounding
+// to bf16 costs (and by no more than 2^-40 of the largest, under 2^-29 of it); infinities and NaN stay what they are. The rows' traffic,
+// which is what their sum takes, is halved. Outputs in fp16 have as many bits as such rows, so theirs are in fp32.
 constexpr int kRows16 = 3;
 
 struct ProductArgs {
@@ -223,14 +224,20 @@ __device__ __forceinline__ void store_rows16(const ProductArgs &a, int64_t row, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
     top = max_of_four(top);
-    const int   e = (int) (top >> 23), X = e >= 255 ? 255 : e < 16 ? 16 : e;
-    const float by = X == 255 ? 0.0f : __uint_as_float((uint32_t) (268 - X) << 23);   // 2^(141 - X)
-    // (rounded to a whole number, ties to even, by the addition of 1.5 x 2^23, which leaves it in the low bits)
-    uint32_t q[8], w[4];
+    if (top >= 0x7F800000u) {   // (the four alike) the largest finite one's
+        top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(fminf(__builtin_fmaf(v[i], by, 12582912.0f), 12582912.0f + 32767.0f));
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t u = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+            top = max(top, u < 0x7F800000u ? u : 0u);
+        }
+        top = max_of_four(top);
+    }
+    const int   X = max((int) (top >> 23), 16);
+    const float by = __uint_as_float((uint32_t) (268 - X) << 23);   // 2^(141 - X)
+    uint32_t    w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x05040100);
+    for (int i = 0; i < 4; ++i) w[i] = pair_bits<RQ_F16>(v[2 * i] * by, v[2 * i + 1] * by);
     if (n >= a.ldy) return;   // (a tile past the padded rows)
     *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y) + row * a.ldy + n) = make_uint4(w[0], w[1], w[2], w[3]);
     if ((n & 31) == 0) a.row_scales[row * (a.ldy >> 5) + (n >> 5)] = (uint8_t) X;

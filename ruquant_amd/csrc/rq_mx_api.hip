@@ -56,7 +56,7 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
     p.positions = most_positions(p.slots, E);
     p.XP = weight_layout(p.positions, K);
     p.HP = weight_layout(p.positions, F);
-    p.rows16 = out_dtype != RQ_F32;
+    p.rows16 = out_dtype == RQ_BF16;
     p.ld = up_to(N, 64);
     p.x = take(p.XP.expert_bytes);
     p.h = take(p.HP.expert_bytes);

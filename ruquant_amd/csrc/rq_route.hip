@@ -318,11 +318,14 @@ __global__ __launch_bounds__(256) void rq_combine_kernel(const void *rows, const
             if (!there[k]) continue;
             if constexpr (ROWS16) {
                 // (2^(X - 141) is a normal number from X = 16 on in two factors only: 2^(X - 127) and 2^-14)
-                const float unit = X[k] == 255 ? NAN : __uint_as_float((uint32_t) X[k] << 23);
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                const float unit = __uint_as_float((uint32_t) X[k] << 23);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sum[2 * i] += w[k] * ((float) (int16_t) (v[k][i] & 0xFFFF) * 6.103515625e-05f * unit);
-                    sum[2 * i + 1] += w[k] * ((float) (v[k][i] >> 16) * 6.103515625e-05f * unit);
+                    const int two = v[k][i];   // (of an element of a vector itself, the compiler casts element 0)
+                    const h2  h = __builtin_bit_cast(h2, two);
+                    sum[2 * i] += w[k] * ((float) h[0] * 6.103515625e-05f * unit);
+                    sum[2 * i + 1] += w[k] * ((float) h[1] * 6.103515625e-05f * unit);
                 }
             } else {
 #pragma unroll

@@ -73,7 +73,8 @@ def experts(x, mats, ids, w, rows16):
     Its h differs from that in 64 bits by what fp32 sums allow, d; a block's scale and elements are those of numbers up to d away,
     so its rounding may fall on a neighbouring code. The bound follows every element: |h^ - h^'| is at most the distance between
     the roundings of h - d and h + d under the scales that a block of such numbers can have. rows16: an expert's outputs may be held
-    as whole numbers of a unit that 32 of them share, off by at most 2^-15 of the largest."""
+    as fp16 numbers of a unit that 32 of them share, the largest from 2^14 units up: off by at most 2^-11 of themselves, or by 2^-25
+    units, which is under 2^-39 of the largest."""
     (gc, gs), (uc, us), (dc, ds) = mats
     E = gc.shape[0]
     xq = values(*quantize(x))
@@ -109,8 +110,10 @@ def experts(x, mats, ids, w, rows16):
         wj = w[t, j].astype(np.float64)[:, None]
         off = near @ np.abs(down).T + 2 * (h.shape[1] / 32 + 16) * eps * (np.abs(hq) @ np.abs(down).T)
         if rows16:
-            pad = np.pad(np.abs(o) + off, ((0, 0), (0, -o.shape[1] % 32)))
-            off = off + 2.0 ** -15 * pad.reshape(len(t), -1, 32).max(axis=2).repeat(32, axis=1)[:, :o.shape[1]]
+            size = np.abs(o) + off
+            pad = np.pad(size, ((0, 0), (0, -o.shape[1] % 32)))
+            largest = pad.reshape(len(t), -1, 32).max(axis=2).repeat(32, axis=1)[:, :o.shape[1]]
+            off = off + np.maximum(2.0 ** -11 * size, 2.0 ** -39 * largest)
         np.add.at(y, t, wj * o)
         # (and the weighted sum over the token's experts, every term rounded twice per addition)
         np.add.at(bound, t, np.abs(wj) * (off + 2 * (ids.shape[1] + 1) * eps * np.abs(o)))

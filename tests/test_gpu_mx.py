@@ -305,7 +305,7 @@ def _experts(E, F, K, N, seed):
 
 
 def _check_experts(y, x64, mats, ids, w, dtype):
-    want, bound = ref.experts(x64, mats, ids, w, dtype != torch.float32)
+    want, bound = ref.experts(x64, mats, ids, w, dtype == torch.bfloat16)
     bound = bound + ROUNDING[dtype] * 1.01 * np.abs(want) + (2.0 ** -25 if dtype == torch.float16 else 0)
     off = np.abs(_host(y) - want)
     assert (off <= bound).all(), "off by %g times the bound" % (off / bound).max()
@@ -397,6 +397,32 @@ def test_experts_with_nan_and_infinity(M):
         bad[M - 1, 5] = float("inf")
         y = rq.expert_ffn(gate, up, down, bad, ids, w)
         assert torch.isnan(y[M - 1]).all() and torch.equal(y[:M - 1], want[:M - 1])
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("M", [2, 40, 300])
+def test_experts_outputs_stand_for_themselves(M, dtype):
+    """an output whose weights hold a NaN is NaN, one 2^20 times its neighbours is itself, and neither shows in the outputs beside it"""
+    E, K, F, N = 4, 128, 64, 72
+    mats, (gate, up, down) = _experts(E, F, K, N, 7)
+    ids = torch.arange(M, device=DEV, dtype=torch.int32).view(M, 1) % E
+    w = torch.rand((M, 1), device=DEV) + 0.5
+    x, _ = _activations(M, K, 2, DTYPES[dtype])
+    want = rq.expert_ffn(gate, up, down, x / 16, ids, w)
+    codes, scales = mats[2][0].copy(), mats[2][1].copy()
+    scales[:, 3, 1] = 255
+    codes[:, 70], scales[:, 70] = codes[:, 69], scales[:, 69] + 20
+    y = rq.expert_ffn(gate, up, rq.MXWeight(_gpu(codes), _gpu(scales)), x / 16, ids, w)
+    assert torch.isnan(y[:, 3]).all()
+    if dtype != "fp16":   # (whose range ends in front of it)
+        assert torch.equal(y[:, 70], want[:, 69] * 2.0 ** 20)
+    # A neighbour may be held to 2^-40 of the large one, which can turn its last rounding, one unit in the last place (2^-7 at most).
+    y, want = y.double(), want.double()
+    off, large = (y - want).abs(), (want[:, 69] * 2.0 ** 20).abs()
+    apart = torch.arange(N, device=DEV)
+    assert (off[:, (apart < 64) & (apart != 3)] == 0).all()
+    beside = (apart >= 64) & (apart != 70)
+    assert (off[:, beside] <= 2.0 ** -7 * want[:, beside].abs() + 2.0 ** -39 * large[:, None]).all()
 
 
 @pytest.mark.parametrize("E,top,M,K,F,N", [(32, 6, 2000, 1024, 640, 2048), (8, 2, 3000, 2048, 256, 1024), (60, 4, 600, 1376, 352, 1000)])
