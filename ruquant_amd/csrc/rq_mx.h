@@ -139,9 +139,9 @@ inline hipError_t allow_lds(const void *kernel, int bytes, std::atomic<uint64_t>
 hipError_t launch_act_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, uint8_t *scales,
                                hipStream_t stream);
 // x -> activations in panel form: row r of the panels is row row_of[r] of x (none if negative), or row r if row_of is null. *rows
-// (on the device; null: L.N) of them are looked at. What the panels hold behind the last row is left as it is.
+// (on the device; null: L.N) of them are looked at. What the panels hold behind the last row is left as it is. Sets zero[0 .. zeros - 1] to 0.
 hipError_t launch_panel_quantize(int dtype, const void *x, int64_t ldx, const WeightLayout &L, const int *row_of, const int *rows,
-                                 uint8_t *panels, hipStream_t stream);
+                                 uint8_t *panels, int *zero, int zeros, hipStream_t stream);
 
 // How a product's tokens are cut into tiles. A plain product has one segment of M tokens; the experts' products have one
 // per expert, and the device knows how long they are.
@@ -164,6 +164,9 @@ struct ProductArgs {
     const uint8_t *panels;          // the activations
     WeightLayout   P;
     int64_t        M;               // tokens (kDense)
+    int            splits, split_steps;   // kDense: workgroups that share a tile, and the steps of 128 inputs of each
+    float         *sums;            //   splits > 1: what they leave
+    int           *arrived;         //   and how many have, by wavefront's outputs: zero before the launch
     const Tile    *tiles;           // kGateUp, kDown: the tiles, on the device
     int            most_tiles;      //   so many; those past the last one have no tokens
     const int     *row_of;          // kDown: position -> row of y
@@ -305,7 +308,16 @@ hipError_t launch_decode_experts(int dtype, const DecodeArgs &gate_up, const Dec
 // more tokens: both operands through LDS, in tiles of several forms
 constexpr int kTiledForms = 7, kForm64 = 1, kForm128 = 3, kForm256 = 6;   // (the experts': 128 x 64, 128 x 128, 256 x 128 rows x tokens)
 hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream);   // the experts'
-hipError_t launch_tiled_product(const ProductArgs &a, hipStream_t stream);               // a plain one, planned by its size
+// a plain one, planned by its size
+struct ProductPlan {
+    int     form, rest;           // rest: of the rows behind main_tiles row tiles, or -1
+    int64_t main_tiles;
+    int     splits, split_steps;
+    int     arrived;              // counters, and bytes of sums, that splits > 1 takes
+    int64_t sums_bytes;
+};
+ProductPlan plan_product(int64_t M, int64_t N, int64_t K);
+hipError_t launch_tiled_product(const ProductPlan &plan, const ProductArgs &a, hipStream_t stream);
 int tiled_tokens(int form);
 int64_t tiled_row_tiles(int mode, int form, int64_t N);
 

@@ -17,8 +17,13 @@ constexpr int64_t kMaxTokens = 1 << 22;   // rows of a call; slots of an experts
 
 // Most tokens whose experts' weights are streamed slot by slot, without sorting.
 constexpr int64_t kExpertsDecodeTokens = 4;
-// Most tokens of a product whose weights go from memory into registers (rq_mx_decode.hip).
-constexpr int kDecodeTokens = 16;
+// Products whose weights go from memory into registers (rq_mx_decode.hip): up to 16 tokens, fewer where the sizes make each more costly than
+// the tiles' start. (us, here -> in tiles, at the fewest tokens that go to those: K = 17408: N = 64 9 tokens 11.6 -> 11.0, N = 5120 4 tokens
+// 17.8 -> 16.6, N = 17408 2 tokens 29.2 -> 28.6; K = 8992, N = 5120 8 tokens 12.5 -> 12.7; K = 5120: N = 5120 14 tokens 10.5 -> 10.7, N = 9000
+// 10 tokens 11.1 -> 10.8, N = 17408 6 tokens 14.9 -> 14.8; K = 1024, N = 17408: here up to 16 tokens, 7.8 -> 8.1)
+bool few_tokens(int64_t M, int64_t K, int64_t N) { return M <= 16 && M * K * (N + 4096) <= 614400000; }
+// ... and that each workgroup rounds for itself, so that no workspace is looked at
+bool alone(int64_t M, int64_t K, int64_t N) { return few_tokens(M, K, N) && decode_takes(M, K, N); }
 
 struct ExpertsPlan {
     bool    decode;               // slot by slot (rq_mx_decode.hip); otherwise sorted by expert and tiled
@@ -78,9 +83,11 @@ bool good_experts(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top
 
 extern "C" size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M) {
     if (rq_mx4_prepared_bytes(1, N, K) == 0 || M < 0 || M > kMaxTokens) return 0;
-    if (decode_takes(M, K, N)) return 256;   // (not looked at)
+    if (alone(M, K, N)) return 256;   // (not looked at)
     const ActLayout A = act_layout(K);
-    return (size_t) (M > kDecodeTokens ? weight_layout(M, K).expert_bytes : pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
+    if (few_tokens(M, K, N)) return (size_t) (pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
+    const ProductPlan plan = plan_product(M, N, K);
+    return (size_t) (pad256(weight_layout(M, K).expert_bytes) + plan.sums_bytes + pad256(plan.arrived * 4)) + 256;
 }
 
 extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in_dtype, const void *x, int64_t ldx, int64_t M,
@@ -92,9 +99,9 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
         (M > 1 && (ldx < K || ldy < N))) {
         return RQ_E_ARGUMENT;
     }
-    if (!decode_takes(M, K, N) && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return RQ_E_WORKSPACE;
+    if (!alone(M, K, N) && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
-    if (M <= kDecodeTokens) {
+    if (few_tokens(M, K, N)) {
         DecodeArgs d = {};
         d.L = weight_layout(N, K);
         d.x = x;
@@ -105,7 +112,7 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
         d.out_dtype = out_dtype;
         d.y = y;
         d.ldy = ldy;
-        if (!decode_takes(M, K, N)) {
+        if (!alone(M, K, N)) {
             d.A = act_layout(K);
             uint8_t *codes = (uint8_t *) workspace, *scales = codes + pad256(M * d.A.code_stride);
             d.a_codes = codes;
@@ -124,8 +131,12 @@ extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in
     a.y = y;
     a.ldy = ldy;
     a.P = weight_layout(M, K);
-    const hipError_t e = launch_panel_quantize(in_dtype, x, ldx, a.P, nullptr, nullptr, (uint8_t *) workspace, st);
-    return e != hipSuccess ? e : launch_tiled_product(a, st);
+    const ProductPlan plan = plan_product(M, N, K);
+    uint8_t          *sums = (uint8_t *) workspace + pad256(a.P.expert_bytes);
+    a.sums = (float *) sums;
+    a.arrived = (int *) (sums + plan.sums_bytes);
+    const hipError_t e = launch_panel_quantize(in_dtype, x, ldx, a.P, nullptr, nullptr, (uint8_t *) workspace, a.arrived, plan.arrived, st);
+    return e != hipSuccess ? e : launch_tiled_product(plan, a, st);
 }
 
 extern "C" int rq_route(int dtype, const void *logits, int64_t ldl, int64_t M, int64_t E, int scoring, const float *bias, int groups,
@@ -202,7 +213,7 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     s.most_tiles = (int) p.tiles;
     s.used = (int *) (ws + p.used);
     hipError_t e = launch_sort(s, st);
-    if (e == hipSuccess) e = launch_panel_quantize(in_dtype, x, ldx, p.XP, s.token_of, s.used, ws + p.x, st);
+    if (e == hipSuccess) e = launch_panel_quantize(in_dtype, x, ldx, p.XP, s.token_of, s.used, ws + p.x, nullptr, 0, st);
     ProductArgs a = {};
     a.L = weight_layout(F, K);
     a.w = (const uint8_t *) gate;

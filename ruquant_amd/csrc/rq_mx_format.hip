@@ -67,7 +67,8 @@ __global__ __launch_bounds__(kThreads) void rq_mx_quantize_kernel(const typename
 // lines and writes two lines of codes; a thread's four scales are one word.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(kThreads) void rq_mx_panel_quantize_kernel(const typename Element<DT>::type *x, int64_t ldx, WeightLayout L,
-                                                                        const int *row_of, const int *rows, uint8_t *panels) {
+                                                                        const int *row_of, const int *rows, uint8_t *panels, int *zero, int zeros) {
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < zeros; i += gridDim.x * kThreads) zero[i] = 0;
     const int     parts = 2 * L.chunks;
     const int     block = blockIdx.x / parts, part = blockIdx.x - block * parts;
     const int     row = threadIdx.x >> 3, u = threadIdx.x & 7;
@@ -193,13 +194,13 @@ hipError_t quantize(const void *x_, int64_t ldx, int64_t M, int64_t K, uint8_t *
 
 template <int DT>
 hipError_t panel_quantize(const void *x_, int64_t ldx, const WeightLayout &L, const int *row_of, const int *rows, uint8_t *panels,
-                          hipStream_t stream) {
+                          int *zero, int zeros, hipStream_t stream) {
     using T = typename Element<DT>::type;
     const T   *x = reinterpret_cast<const T *>(x_);
     const bool vec = (uintptr_t) x % 16 == 0 && ldx * (int64_t) sizeof(T) % 16 == 0;
     const dim3 grid((unsigned) ((L.N + 31) / 32 * 2 * L.chunks));
-    if (vec) hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, true>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels);
-    else hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, false>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels);
+    if (vec) hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, true>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels, zero, zeros);
+    else hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, false>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels, zero, zeros);
     return hipGetLastError();
 }
 
@@ -237,10 +238,10 @@ hipError_t launch_act_quantize(int dtype, const void *x, int64_t ldx, int64_t M,
 }
 
 hipError_t launch_panel_quantize(int dtype, const void *x, int64_t ldx, const WeightLayout &L, const int *row_of, const int *rows,
-                                 uint8_t *panels, hipStream_t stream) {
-    if (dtype == RQ_F32) return panel_quantize<RQ_F32>(x, ldx, L, row_of, rows, panels, stream);
-    if (dtype == RQ_F16) return panel_quantize<RQ_F16>(x, ldx, L, row_of, rows, panels, stream);
-    return panel_quantize<RQ_BF16>(x, ldx, L, row_of, rows, panels, stream);
+                                 uint8_t *panels, int *zero, int zeros, hipStream_t stream) {
+    if (dtype == RQ_F32) return panel_quantize<RQ_F32>(x, ldx, L, row_of, rows, panels, zero, zeros, stream);
+    if (dtype == RQ_F16) return panel_quantize<RQ_F16>(x, ldx, L, row_of, rows, panels, zero, zeros, stream);
+    return panel_quantize<RQ_BF16>(x, ldx, L, row_of, rows, panels, zero, zeros, stream);
 }
 
 }  // namespace mx

@@ -170,15 +170,22 @@ struct Tiled {
     }
 };
 
-template <int MODE, int RB, int TB, int WC, int R>
+// SPLIT: a.splits workgroups share a tile's inputs, a.split_steps steps each. Each wavefront leaves its sums, as they lie in its registers,
+// in the workspace and counts itself in; the last of those that hold the same outputs adds them up, in the order of the inputs, so
+// that the bits do not depend on who is last. The sums go past the XCDs' caches (atomic stores and loads of the device's scope) and
+// are waited for before the count, so who sees the last count sees all sums. (With fences instead, which write a whole L2 back for every
+// wavefront: 512 outputs of 17408 inputs, 64 tokens, 4 parts 13.7 us, 16 parts 17.2, 2048 outputs, 8 parts 29.4; so 13.6, 16.1, 16.4.
+// Unshared 22.0 and 22.5.)
+template <int MODE, int RB, int TB, int WC, int R, bool SPLIT>
 __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB <= 4 ? 3 : 2) void rq_mx_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles) {
     using G = Tiled<MODE, RB, TB, WC, R>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     // Workgroups go to the XCDs in turn. Each XCD takes a run of the tiles in an order in which the token tiles run fastest, so that
     // those that share rows of the weight share an L2.
-    const int total = row_tiles * token_tiles;
+    const int total = row_tiles * token_tiles * (SPLIT ? a.splits : 1);
     const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
-    const int v = xcd * each + min(xcd, more) + (int) (blockIdx.x >> 3);
+    const int place_of = xcd * each + min(xcd, more) + (int) (blockIdx.x >> 3);
+    const int v = SPLIT ? place_of / a.splits : place_of, part = SPLIT ? place_of - v * a.splits : 0;
     const int row_tile = v / token_tiles, token_tile = v - row_tile * token_tiles;
     Tile tile = { 0, 0, 0, 0 };
     if constexpr (MODE == kDense) {
@@ -196,7 +203,8 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     g.wr = g.wave & 1;
     g.wc = WC == 2 ? ((g.wave >> 1) ^ (int) (blockIdx.x >> 3)) & 1 : g.wave >> 1;
     g.lane16 = g.lane * 16;
-    g.steps = a.L.steps;
+    const int step0 = SPLIT ? part * a.split_steps : 0;   // (a multiple of two: the scales' parts)
+    g.steps = SPLIT ? min(a.split_steps, a.L.steps - step0) : a.L.steps;
     g.lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void *) lds;
     g.a_lds = lds + g.wr * RB * 2048 + g.lane * 16;
     g.b_lds = lds + (2 * G::kABlocks + g.wc * TB * 2) * 1024 + g.lane * 16;
@@ -215,7 +223,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
 #pragma unroll
     for (int i = 0; i < G::kARuns; ++i) {
         const int run = g.wave * G::kARuns + i;
-        g.a_src[i] = uniform(matrix(run >> 1) + (int64_t) place(run >> 1) * a.L.steps * 2048 + (run & 1) * 1024);
+        g.a_src[i] = uniform(matrix(run >> 1) + (int64_t) place(run >> 1) * a.L.steps * 2048 + (run & 1) * 1024 + (int64_t) step0 * 2048);
     }
     // the tile's token blocks; those past the last repeat it, and those past the activations the activations' last
     const int token0 = tile.first >> 5, token_blocks = min((tile.count + 31) >> 5, a.P.row_blocks - token0);
@@ -223,13 +231,13 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
 #pragma unroll
     for (int i = 0; i < G::kBRuns; ++i) {
         const int run = g.wave * G::kBRuns + i;
-        g.b_src[i] = uniform(a.panels + (int64_t) token_place(run >> 1) * a.P.steps * 2048 + (run & 1) * 1024);
+        g.b_src[i] = uniform(a.panels + (int64_t) token_place(run >> 1) * a.P.steps * 2048 + (run & 1) * 1024 + (int64_t) step0 * 2048);
     }
 #pragma unroll
     for (int i = 0; i < G::kPartRuns; ++i) {   // of four blocks, row blocks first (past the last one it again)
         const int r = min((i * G::kWaves + g.wave) % G::kScaleRuns * 4 + (g.lane >> 4), G::kABlocks + G::kBBlocks - 1);
         g.s_src[i] = (r < G::kABlocks ? matrix(r) + a.L.code_bytes + (int64_t) place(r) * a.L.chunks * 512
-                                      : a.panels + a.P.code_bytes + (int64_t) token_place(r - G::kABlocks) * a.P.chunks * 512) + (g.lane & 15) * 16;
+                                      : a.panels + a.P.code_bytes + (int64_t) token_place(r - G::kABlocks) * a.P.chunks * 512) + (g.lane & 15) * 16 + step0 * 128;
     }
     if (g.wc * TB * 32 < tile.count) g.template loop<true>();
     else g.template loop<false>();
@@ -260,6 +268,35 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
         }
         barrier();   // (the ring is not read any more)
         if (wc * TB * 32 >= tile.count) return;
+        if constexpr (SPLIT) {
+            constexpr int kPairs = RB * TB * 8;   // 512 bytes each
+            const int     outputs = v * G::kWaves + 2 * wc + wr;   // (of the tile's: which wavefront has them differs by workgroup)
+            auto         *sums = reinterpret_cast<uint64_t *>(a.sums) + (int64_t) outputs * a.splits * kPairs * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+                const float    lo = g.acc[i / 8 / TB][i / 8 % TB][i % 8 * 2], hi = g.acc[i / 8 / TB][i / 8 % TB][i % 8 * 2 + 1];
+                const uint64_t x = (uint64_t) __float_as_uint(hi) << 32 | __float_as_uint(lo);
+                __hip_atomic_store(sums + (part * kPairs + i) * 64, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            wait_loads<0>();   // (stores count alike: all of them are where every XCD sees them)
+            int before = 0;
+            if (lane == 0) before = __hip_atomic_fetch_add(a.arrived + outputs, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (__builtin_amdgcn_readfirstlane(before) != a.splits - 1) return;
+            asm volatile("" : : : "memory");
+            for (int p = 0; p < a.splits; ++p) {
+                uint64_t x[kPairs];
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i)
+                    x[i] = __hip_atomic_load(sums + (p * kPairs + i) * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i) {
+                    v16f       &c = g.acc[i / 8 / TB][i / 8 % TB];
+                    const float lo = __uint_as_float((uint32_t) x[i]), hi = __uint_as_float((uint32_t) (x[i] >> 32));
+                    c[i % 8 * 2] = p ? c[i % 8 * 2] + lo : lo;
+                    c[i % 8 * 2 + 1] = p ? c[i % 8 * 2 + 1] + hi : hi;
+                }
+            }
+        }
         // LANES of a token write 16 bytes each
         auto store = [&](auto lanes, int t, int r) __attribute__((always_inline)) {
             constexpr int kLanes = decltype(lanes)::value, kTokens = 64 / kLanes;
@@ -296,17 +333,18 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     }
 }
 
-template <int MODE, int RB, int TB, int WC, int R>
+template <int MODE, int RB, int TB, int WC, int R, bool SPLIT = false>
 hipError_t launch(const ProductArgs &a, hipStream_t stream) {
     using G = Tiled<MODE, RB, TB, WC, R>;
     const int row_tiles = MODE == kDense ? a.row_tiles : (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
     const int token_tiles = MODE == kDense ? (int) ((a.M + G::kTileTokens - 1) / G::kTileTokens) : a.most_tiles;
-    if ((int64_t) row_tiles * token_tiles > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    const int64_t groups = (int64_t) row_tiles * token_tiles * (SPLIT ? a.splits : 1);
+    if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     static std::atomic<uint64_t> allowed{ 0 };   // devices on which the kernel may have its LDS
-    const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R>), G::kBytes, allowed);
+    const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R, SPLIT>), G::kBytes, allowed);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE, RB, TB, WC, R>), dim3((unsigned) row_tiles * token_tiles), dim3(G::kThreads), G::kBytes, stream,
-                       a, row_tiles, token_tiles);
+    hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE, RB, TB, WC, R, SPLIT>), dim3((unsigned) groups), dim3(G::kThreads), G::kBytes, stream, a,
+                       row_tiles, token_tiles);
     return hipGetLastError();
 }
 
@@ -314,7 +352,7 @@ template <int MODE>
 hipError_t launch_form(int form, const ProductArgs &a, hipStream_t stream) {
     if constexpr (MODE == kDense) {
         switch (form) {
-            case 0: return launch<MODE, 1, 1, 2, 8>(a, stream);
+            case 0: return a.splits > 1 ? launch<MODE, 1, 1, 2, 8, true>(a, stream) : launch<MODE, 1, 1, 2, 8>(a, stream);
             case 1: return launch<MODE, 2, 1, 2, 6>(a, stream);
             case 2: return launch<MODE, 2, 2, 2, 6>(a, stream);
             case 3: return launch<MODE, 2, 2, 2, 3>(a, stream);
@@ -360,20 +398,19 @@ double price(int form, int64_t tiles, int64_t steps) {
 
 // A product is one launch in the form of the least price, or two: as many row tiles as fill whole rounds of the chip in one form, and the
 // rows behind them, which would leave most of it idle for a round, in another. (17408 x 5120 at 2048 tokens: 544 tiles of 256 x 256 are
-// two rounds and 32 tiles.)
-hipError_t launch_tiled_product(const ProductArgs &a, hipStream_t stream) {
+// two rounds and 32 tiles.) Or, where the tiles are few and the inputs many, one whose tiles several workgroups share.
+ProductPlan plan_product(int64_t M, int64_t N, int64_t K) {
     constexpr int    kPlain = kTiledForms - 1;
     constexpr double kLaunch = 2.0;
-    const int64_t    rows = (int64_t) a.L.row_blocks * 32, steps = a.L.steps;
-    auto token_tiles = [&](int f) { return (a.M + kForms[f].tokens - 1) / kForms[f].tokens; };
+    const int64_t    rows = up_to(N, 64), steps = up_to(K, 128) / 128;
+    auto token_tiles = [&](int f) { return (M + kForms[f].tokens - 1) / kForms[f].tokens; };
     auto row_tiles = [&](int f, int64_t n) { return (n + kForms[f].rows - 1) / kForms[f].rows; };
-    double  least = 0;
-    int     form = -1, rest = -1;
-    int64_t main_tiles = 0;
+    double      least = 0;
+    ProductPlan plan = { -1, -1, 0, 1, 0, 0, 0 };
     for (int f = 0; f < kPlain; ++f) {
         const int64_t tokens = token_tiles(f), all = row_tiles(f, rows);
         const double  whole = price(f, all * tokens, steps);
-        if (form < 0 || whole < least) least = whole, form = f, rest = -1, main_tiles = all;
+        if (plan.form < 0 || whole < least) least = whole, plan = { f, -1, all, 1, (int) steps, 0, 0 };
         const int64_t round = 256 * kForms[f].resident, rounds = all * tokens / round;
         for (int64_t k = rounds; k > 0 && k > rounds - 2; --k) {
             const int64_t n = k * round / tokens;   // row tiles
@@ -381,18 +418,37 @@ hipError_t launch_tiled_product(const ProductArgs &a, hipStream_t stream) {
             const double some = price(f, n * tokens, steps) + kLaunch;
             for (int g = 0; g < kPlain; ++g) {
                 const double p = some + price(g, row_tiles(g, rows - n * kForms[f].rows) * token_tiles(g), steps);
-                if (p < least) least = p, form = f, rest = g, main_tiles = n;
+                if (p < least) least = p, plan = { f, g, n, 1, (int) steps, 0, 0 };
             }
         }
     }
+    // (64 x 64 tiles only: larger ones have fewer wavefronts to join as much, and were never faster. The join's time from K = 17408 and 5120,
+    // N = 256 to 9000 and 17 to 512 tokens.)
+    const int64_t tiles = row_tiles(0, rows) * token_tiles(0);
+    for (int64_t parts = 2; parts <= 16; ++parts) {
+        const int64_t some = up_to((steps + parts - 1) / parts, 2), n = (steps + some - 1) / some;
+        const double  p = price(0, tiles * n, some) + 0.6 + 0.3 * (double) n + 0.008 * (double) (tiles * n);
+        if (n > 1 && p < least) least = p, plan = { 0, -1, row_tiles(0, rows), (int) n, (int) some, 0, 0 };
+    }
+    if (plan.splits > 1) {
+        plan.arrived = (int) tiles * 4;   // wavefronts, of 32 x 32 outputs
+        plan.sums_bytes = tiles * 4 * plan.splits * 4096;
+    }
+    return plan;
+}
+
+hipError_t launch_tiled_product(const ProductPlan &plan, const ProductArgs &a, hipStream_t stream) {
     ProductArgs one = a;
     one.first_block = 0;
-    one.row_tiles = (int) main_tiles;
-    hipError_t e = launch_form<kDense>(form, one, stream);
-    if (e != hipSuccess || rest < 0) return e;
-    one.first_block = (int) (main_tiles * kForms[form].rows / 32);
-    one.row_tiles = (int) row_tiles(rest, rows - main_tiles * kForms[form].rows);
-    return launch_form<kDense>(rest, one, stream);
+    one.row_tiles = (int) plan.main_tiles;
+    one.splits = plan.splits;
+    one.split_steps = plan.split_steps;
+    hipError_t e = launch_form<kDense>(plan.form, one, stream);
+    if (e != hipSuccess || plan.rest < 0) return e;
+    const int64_t done = plan.main_tiles * kForms[plan.form].rows;
+    one.first_block = (int) (done / 32);
+    one.row_tiles = (int) (((int64_t) a.L.row_blocks * 32 - done + kForms[plan.rest].rows - 1) / kForms[plan.rest].rows);
+    return launch_form<kDense>(plan.rest, one, stream);
 }
 
 hipError_t launch_tiled(int mode, int form, const ProductArgs &a, hipStream_t stream) {

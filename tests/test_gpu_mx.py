@@ -202,6 +202,47 @@ def test_product_of_many_tiles_is_that_of_few(M, K, N):
         assert torch.equal(rq.mx_mul_mat(W, part), y[min(i, M - 60):i + 100])
 
 
+SHARED = [(4, 17408, 5000), (17, 17408, 1), (33, 8992, 70), (64, 16384, 512), (65, 17376, 257), (130, 9056, 600)]
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("M,K,N", SHARED)
+def test_product_whose_tiles_are_shared(M, K, N, dtype):
+    """Few outputs of many inputs, each of which several workgroups sum up: as defined, and the same bits again and again, whoever is last
+    and whatever the workspace held."""
+    x, x64 = _activations(M, K, M + K + N, DTYPES[dtype])
+    codes, scales = _weights((N,), K, M + N)
+    W = rq.MXWeight(_gpu(codes), _gpu(scales))
+    ws = W.workspace(M)
+    assert ws.numel() > -(-M // 32) * 32 * (-(-K // 512) * 512) * 17 // 32 + 2 * 64 * 64 * 4   # (more than the activations: the sums)
+    y = rq.mx_mul_mat(W, x, workspace=ws).clone()
+    _check_product(y, x64, codes, scales, DTYPES[dtype])
+    for i in range(12):
+        ws.fill_(i % 2 * 255)
+        assert torch.equal(rq.mx_mul_mat(W, x, workspace=ws), y)
+
+
+def test_product_whose_tiles_are_shared_in_a_graph():
+    M, K, N = 40, 16384, 512
+    codes, scales = _weights((N,), K, 3)
+    W = rq.MXWeight(_gpu(codes), _gpu(scales))
+    x, _ = _activations(M, K, 8, torch.bfloat16)
+    want = rq.mx_mul_mat(W, x).clone()
+    y, ws = torch.empty_like(want), W.workspace(M)
+    rq.mx_mul_mat(W, x, out=y, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            rq.mx_mul_mat(W, x, out=y, workspace=ws)
+    for i in range(5):
+        y.zero_()
+        ws.fill_(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
 @pytest.mark.parametrize("M", [1, 18, 130])
 def test_product_with_nan_and_infinity(M):
     """a NaN in a token makes its row NaN and no other; a NaN scale of a weight makes its row's outputs NaN and no other"""
