@@ -51,7 +51,9 @@ constexpr int kNever = -2147483647 - 1;   // in front of every number: what cann
 
 // A wavefront per token, experts V lane .. V lane + V - 1 in a lane. The choice is `top` rounds of a maximum over the wavefront, of whole
 // numbers that have the order of the choices: the lowest lane and place that holds it is the lowest index. Bound by the vector ALU
-// from some thousand tokens on (30 instructions a round), by its latency below.
+// from some thousand tokens on (600 instructions a token of 256 experts, 8 of them from 4 of 8 groups, 30 a round: 16384 tokens 20 us; their
+// 17.8 MB would take 3.6), by its latency below (a token of 64 experts 2.2 us). The sums of exponentials are in 64 bits, so that no order
+// of addition changes a choice between two equal scores.
 template <int DT, int V>
 __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs a, const bool vec) {
     using T = typename Element<DT>::type;
@@ -195,7 +197,8 @@ hipError_t route(const RouteArgs &a, hipStream_t stream) {
 }
 
 // One workgroup: counts the experts' slots, lays their tiles out and deals the slots to their places. The order of an expert's
-// slots is that in which they arrive, and no result depends on it: every slot's row is computed by itself.
+// slots is that in which they arrive, and no result depends on it: every slot's row is computed by itself. A chain of passes over the ids by
+// one compute unit: 16384 slots 13.2 us, 148 slots 5.9, of calls of 400 and 97.
 constexpr int kSortThreads = 1024;
 constexpr int kSortBatch = 8;   // ids in flight per thread
 // Up to so many positions the slots are dealt in LDS and written in order: from this one workgroup a store of 64 places of memory
@@ -278,7 +281,8 @@ __global__ __launch_bounds__(kSortThreads) void rq_sort_kernel(const SortArgs a)
 }
 
 // y[m] = sum_j weights[m][j] * rows[m top + j] in the order of j, fp32; the slots' rows are loaded four at a time, 16 bytes a thread and
-// slot: four outputs of fp32 rows, eight of 16-bit ones.
+// slot: four outputs of fp32 rows, eight of 16-bit ones. Bound by memory: 2048 tokens x 8 rows of 5120 in 16 bits, 31 us for 194 MB,
+// half of them from the memory-side cache that the down projection has just filled.
 template <int DT, bool ROWS16, bool VEC>
 __global__ __launch_bounds__(256) void rq_combine_kernel(const void *rows, const uint8_t *row_scales, int64_t ld, int64_t N, const int32_t *ids,
                                                          const float *weights, int top, int E, typename Element<DT>::type *y, int64_t ldy) {
