@@ -317,6 +317,7 @@ struct ProductPlan {
     int64_t sums_bytes;
 };
 ProductPlan plan_product(int64_t M, int64_t N, int64_t K);
+int64_t     product_sums_bytes(int64_t M, int64_t N, int64_t K);   // for sums and counters of up to M tokens
 hipError_t launch_tiled_product(const ProductPlan &plan, const ProductArgs &a, hipStream_t stream);
 int tiled_tokens(int form);
 int64_t tiled_row_tiles(int mode, int form, int64_t N);

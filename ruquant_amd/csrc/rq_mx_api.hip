@@ -69,7 +69,7 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
     p.row_scales = take(p.rows16 ? p.slots * p.ld / 32 : 0);
     p.token_of = take(p.positions * 4);
     p.slot_of = take(p.positions * 4);
-    p.tile_table = take(p.tiles * (int64_t) sizeof(Tile));
+    p.tile_table = take(most_tiles(p.slots, E, tiled_tokens(kForm64)) * (int64_t) sizeof(Tile));   // (room for the smallest, so that it grows with M)
     p.used = take(4);
     p.total = at;
     return p;
@@ -86,8 +86,7 @@ extern "C" size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M) {
     if (alone(M, K, N)) return 256;   // (not looked at)
     const ActLayout A = act_layout(K);
     if (few_tokens(M, K, N)) return (size_t) (pad256(M * A.code_stride) + pad256(M * A.scale_stride)) + 256;
-    const ProductPlan plan = plan_product(M, N, K);
-    return (size_t) (pad256(weight_layout(M, K).expert_bytes) + plan.sums_bytes + pad256(plan.arrived * 4)) + 256;
+    return (size_t) (pad256(weight_layout(M, K).expert_bytes) + pad256(product_sums_bytes(M, N, K))) + 256;
 }
 
 extern "C" int rq_mx4_mul_mat(const void *prepared, int64_t K, int64_t N, int in_dtype, const void *x, int64_t ldx, int64_t M,

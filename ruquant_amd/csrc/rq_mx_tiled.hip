@@ -409,6 +409,14 @@ double price(int form, int64_t tiles, int64_t steps) {
 
 }  // namespace
 
+constexpr int64_t kUnsplitSteps = 24, kMostSplits = 16, kMostParts = 512;
+// At least what any plan for up to M tokens takes.
+int64_t product_sums_bytes(int64_t M, int64_t N, int64_t K) {
+    if (K <= kUnsplitSteps * 128) return 0;
+    const int64_t parts = up_to(N, 64) / 64 * (up_to(M, 64) / 64) * kMostSplits;
+    return (parts < kMostParts ? parts : kMostParts) * (4 * 4096 + 16);   // (16: the counters of a tile's wavefronts)
+}
+
 // A product is one launch in the form of the least price, or two: as many row tiles as fill whole rounds of the chip in one form, and the
 // rows behind them, which would leave most of it idle for a round, in another. (17408 x 5120 at 2048 tokens: 544 tiles of 256 x 256 are
 // two rounds and 32 tiles.) Or, where the tiles are few and the inputs many, one whose tiles several workgroups share.
@@ -436,9 +444,9 @@ ProductPlan plan_product(int64_t M, int64_t N, int64_t K) {
         }
     }
     // (64 x 64 tiles only: larger ones have fewer wavefronts to join as much, and were never faster. The join's time from K = 17408 and 5120,
-    // N = 256 to 9000 and 17 to 512 tokens.)
+    // N = 256 to 9000 and 17 to 512 tokens; by it up to kUnsplitSteps never pay.)
     const int64_t tiles = row_tiles(0, rows) * token_tiles(0);
-    for (int64_t parts = 2; parts <= 16; ++parts) {
+    for (int64_t parts = 2; steps > kUnsplitSteps && parts <= kMostSplits && tiles * parts <= kMostParts; ++parts) {
         const int64_t some = up_to((steps + parts - 1) / parts, 2), n = (steps + some - 1) / some;
         const double  p = price(0, tiles * n, some) + 0.6 + 0.3 * (double) n + 0.008 * (double) (tiles * n);
         if (n > 1 && p < least) least = p, plan = { 0, -1, row_tiles(0, rows), (int) n, (int) some, 0, 0 };

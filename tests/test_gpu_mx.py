@@ -214,12 +214,23 @@ def test_product_whose_tiles_are_shared(M, K, N, dtype):
     codes, scales = _weights((N,), K, M + N)
     W = rq.MXWeight(_gpu(codes), _gpu(scales))
     ws = W.workspace(M)
-    assert ws.numel() > -(-M // 32) * 32 * (-(-K // 512) * 512) * 17 // 32 + 2 * 64 * 64 * 4   # (more than the activations: the sums)
     y = rq.mx_mul_mat(W, x, workspace=ws).clone()
     _check_product(y, x64, codes, scales, DTYPES[dtype])
     for i in range(12):
         ws.fill_(i % 2 * 255)
         assert torch.equal(rq.mx_mul_mat(W, x, workspace=ws), y)
+
+
+def test_one_workspace_serves_every_number_of_tokens():
+    K, N, most = 8992, 300, 700
+    codes, scales = _weights((N,), K, 3)
+    W = rq.MXWeight(_gpu(codes), _gpu(scales))
+    x, _ = _activations(most, K, 8, torch.bfloat16)
+    room = torch.full((W.workspace(most).numel() + 4096,), 7, dtype=torch.uint8, device=DEV)
+    ws = room[:-4096]
+    for M in (700, 400, 260, 128, 64, 33, 17, 16, 12, 5, 2, 1):
+        assert torch.equal(rq.mx_mul_mat(W, x[:M], workspace=ws), rq.mx_mul_mat(W, x[:M]))
+    assert (room[-4096:] == 7).all()
 
 
 def test_product_whose_tiles_are_shared_in_a_graph():

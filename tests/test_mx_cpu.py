@@ -40,6 +40,18 @@ def test_sizes():
         assert ex(*bad) == 0, bad
 
 
+def test_workspaces_grow_with_the_tokens():
+    """so that the most tokens' workspace serves every call"""
+    L = rq.load_library()
+    tokens = list(range(1, 300)) + list(range(300, 9000, 97))
+    for K, N in ((32, 1), (256, 64), (4096, 100), (5120, 17408), (17408, 64), (17408, 5120), (65536, 700)):
+        sizes = [L.rq_mx4_workspace_bytes(K, N, M) for M in tokens]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])) and sizes[0] > 0, (K, N)
+    for E, K, F, N, top in ((1, 32, 32, 1, 1), (8, 64, 32, 33, 2), (64, 5120, 1280, 5120, 8), (60, 512, 96, 100, 4), (1024, 64, 32, 16, 1)):
+        sizes = [L.rq_mx4_experts_workspace_bytes(E, K, F, N, M, top) for M in tokens]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:])) and sizes[0] > 0, (E, K, F, N, top)
+
+
 def test_refusals_without_a_gpu():
     L = rq.load_library()
     bad, unsupported, workspace = -3, -1, -2
