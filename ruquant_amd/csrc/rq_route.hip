@@ -51,19 +51,29 @@ constexpr int kNever = -2147483647 - 1;   // in front of every number: what cann
 
 // A wavefront per token, experts V lane .. V lane + V - 1 in a lane. The choice is `top` rounds of a maximum over the wavefront, of whole
 // numbers that have the order of the choices: the lowest lane and place that holds it is the lowest index. Bound by the vector ALU
-// from some thousand tokens on (600 instructions a token of 256 experts, 8 of them from 4 of 8 groups, 30 a round: 16384 tokens 20 us; their
-// 17.8 MB would take 3.6), by its latency below (a token of 64 experts 2.2 us). The sums of exponentials are in 64 bits, so that no order
+// from some thousand tokens on (520 instructions a token of 256 experts, 8 of them from 4 of 8 groups, of which 190 are the rounds and 100 the
+// sigmoid: 16384 tokens 16.4 us; their 17.8 MB would take 3.6), by its latency below (a token of 64 experts 2.2 us). The sums of exponentials are in 64 bits, so that no order
 // of addition changes a choice between two equal scores.
 template <int DT, int V>
-__global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs a, const bool vec) {
+__global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs a, const bool vec, const bool vec_bias) {
     using T = typename Element<DT>::type;
     const int     lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t m = (int64_t) blockIdx.x * (kRouteThreads / 64) + wave;
     if (m >= a.M) return;
     const T *x = reinterpret_cast<const T *>(a.logits) + m * a.ldl + lane * V;
     const int mine = min(max(a.E - lane * V, 0), V);   // experts of this lane
-    float s[V];
+    float s[V], bias[V];
     int   c[V];
+    // (loads of places past the last expert are of the last one: a branch for each would wait for one after the other)
+    if (vec_bias) {
+        typedef float B __attribute__((ext_vector_type(V > 1 ? V : 2)));
+        const B b = reinterpret_cast<const B *>(a.bias)[mine ? lane : 0];
+#pragma unroll
+        for (int j = 0; j < V; ++j) bias[j] = b[j];
+    } else if (a.bias) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) bias[j] = a.bias[min(lane * V + j, a.E - 1)];
+    }
     if (V > 1 && vec) {   // (whole lanes)
         if constexpr (DT == RQ_F32) {
             typedef float F __attribute__((ext_vector_type(V)));
@@ -82,7 +92,9 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = j < mine ? to_float(x[j]) : -INFINITY;
+        for (int j = 0; j < V; ++j) s[j] = to_float((x - lane * V)[min(lane * V + j, a.E - 1)]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = j < mine ? s[j] : -INFINITY;
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j] = s[j] != s[j] ? -INFINITY : s[j];
@@ -108,29 +120,39 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         float v = s[j];
-        if (a.bias && j < mine) v += a.bias[lane * V + j];
+        if (a.bias) v += bias[j];
         c[j] = j < mine ? ordered(v > kLowest ? v : kLowest) : kNever;   // (a NaN is not greater)
     }
     if (a.groups > 1) {
         // 2^share lanes a group find its two largest; the groups' sums are compared by all of their lanes
         __shared__ int all[kRouteThreads / 64][64 * V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) all[wave][lane * V + j] = c[j];
-        __builtin_amdgcn_wave_barrier();
-        const int size = a.E / a.groups, share = 31 - __clz(64 / a.groups), group = lane >> share, first = lane & ((1 << share) - 1);
-        int       one = kNever, two = kNever;
-        if (group < a.groups) {
-            for (int i = first; i < size; i += 1 << share) {
-                const int v = all[wave][group * size + i];
-                two = max(two, min(one, v));
-                one = max(one, v);
-            }
-        }
-        for (int o = 1; o < 1 << share; o <<= 1) {
-            const int p = __shfl_xor(one, o), q = __shfl_xor(two, o);
+        const int  size = a.E / a.groups, share = 31 - __clz(64 / a.groups), group = lane >> share, first = lane & ((1 << share) - 1);
+        const bool own = size == V << share;   // the lanes of a group hold its experts
+        int        one = kNever, two = kNever;
+        auto       take = [&](int v) __attribute__((always_inline)) {
+            two = max(two, min(one, v));
+            one = max(one, v);
+        };
+        auto join = [&](int p, int q) __attribute__((always_inline)) {   // (p >= q)
             two = max(min(one, p), max(two, q));
             one = max(one, p);
+        };
+        if (own) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) take(c[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) all[wave][lane * V + j] = c[j];
+            __builtin_amdgcn_wave_barrier();
+            if (group < a.groups) {
+                for (int i = first; i < size; i += 1 << share) take(all[wave][group * size + i]);
+            }
         }
+        if (share > 0) join(moved<0xB1, 0xF>(one, kNever), moved<0xB1, 0xF>(two, kNever));
+        if (share > 1) join(moved<0x4E, 0xF>(one, kNever), moved<0x4E, 0xF>(two, kNever));
+        if (share > 2) join(moved<0x141, 0xF>(one, kNever), moved<0x141, 0xF>(two, kNever));
+        if (share > 3) join(moved<0x140, 0xF>(one, kNever), moved<0x140, 0xF>(two, kNever));
+        if (share > 4) join(__shfl_xor(one, 16), __shfl_xor(two, 16));
         float worth = size > 1 ? unordered(one) + unordered(two) : unordered(one);
         worth = worth > kLowest ? worth : kLowest;
         int place = 0;   // groups that are worth more, or as much in front of it
@@ -140,37 +162,81 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
         }
         const unsigned long long kept = __ballot(group < a.groups && place < a.top_groups);
         const float              per = 1.0f / (float) size;
+        if (own) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+            for (int j = 0; j < V; ++j) c[j] = place < a.top_groups ? c[j] : kNever;
+        }
+#pragma unroll
+        for (int j = 0; j < V && !own; ++j) {
             const int of = (int) (((float) (lane * V + j) + 0.5f) * per);   // (exact: under 1024, and half a unit away from whole numbers)
             if (!((kept >> (min(of, a.groups - 1) << share)) & 1)) c[j] = kNever;
         }
     }
     float chosen = 0, total = 0;
     int   id = 0;
-    for (int i = 0; i < a.top; ++i) {
-        int most = c[0];
+    if constexpr (V > 1 && V <= 4) {
+        // Each lane's experts in falling order, so that a round looks at its first and takes it off: 19 instructions for 30. (Neighbours are
+        // compared, and change places where the second is larger: equal ones keep their order. V = 8 and 16 would sort as long as they save.)
+        int order = 0, place[V];
 #pragma unroll
-        for (int j = 1; j < V; ++j) most = max(most, c[j]);
-        const int best = wave_max(most);
-        // (the lane and the place are the wavefront's, so the scalar unit finds them)
-        unsigned long long has[V], any = 0;
+        for (int j = 0; j < V; ++j) place[j] = j;
 #pragma unroll
-        for (int j = 0; j < V; ++j) has[j] = __ballot(c[j] == best), any |= has[j];
-        const int from = __builtin_ctzll(any);
-        int       at = 0;
-        float     w = s[0];
+        for (int round = 0; round < V; ++round) {
 #pragma unroll
-        for (int j = V - 1; j > 0; --j) at = (has[j] >> from) & 1 ? j : at;
-        at = (has[0] >> from) & 1 ? 0 : at;
+            for (int j = round & 1; j + 1 < V; j += 2) {
+                const bool swap = c[j] < c[j + 1];
+                const int  most = max(c[j], c[j + 1]), least = min(c[j], c[j + 1]), p = place[j], q = place[j + 1];
+                c[j] = most, c[j + 1] = least;
+                place[j] = swap ? q : p, place[j + 1] = swap ? p : q;
+            }
+        }
 #pragma unroll
-        for (int j = 1; j < V; ++j) w = at == j ? s[j] : w;
-        const float picked = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from));
-        const int   e = from * V + at;
+        for (int j = 0; j < V; ++j) order |= place[j] << (8 * j);
+        for (int i = 0; i < a.top; ++i) {
+            const int  best = wave_max(c[0]);
+            const int  from = __builtin_ctzll(__ballot(c[0] == best));
+            const int  e = from * V + (__builtin_amdgcn_readlane(order, from) & 255);
+            const bool off = lane == from;
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] = lane == (at == j ? from : -1) ? kNever : c[j];
-        total += picked;
-        if (lane == i) chosen = picked, id = e;
+            for (int j = 0; j < V; ++j) {
+                const int here = c[j], next = j + 1 < V ? c[(j + 1) % V] : kNever;
+                c[j] = off ? next : here;
+            }
+            order = off ? order >> 8 : order;
+            id = lane == i ? e : id;
+        }
+        // the scores of the chosen, a lane each, and their sum in the order of choice
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float of = __shfl(s[j], id / V);
+            chosen = id % V == j ? of : chosen;
+        }
+        for (int i = 0; i < a.top; ++i) total += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(chosen), i));
+    } else {
+        for (int i = 0; i < a.top; ++i) {
+            int most = c[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) most = max(most, c[j]);
+            const int best = wave_max(most);
+            // (the lane and the place are the wavefront's, so the scalar unit finds them)
+            unsigned long long has[V], any = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) has[j] = __ballot(c[j] == best), any |= has[j];
+            const int from = __builtin_ctzll(any);
+            int       at = 0;
+            float     w = s[0];
+#pragma unroll
+            for (int j = V - 1; j > 0; --j) at = (has[j] >> from) & 1 ? j : at;
+            at = (has[0] >> from) & 1 ? 0 : at;
+#pragma unroll
+            for (int j = 1; j < V; ++j) w = at == j ? s[j] : w;
+            const float picked = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from));
+            const int   e = from * V + at;
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[j] = lane == (at == j ? from : -1) ? kNever : c[j];
+            total += picked;
+            if (lane == i) chosen = picked, id = e;
+        }
     }
     if (lane < a.top) {
         const float w = a.renormalize ? (total > 0 ? chosen / total : 0.0f) : chosen;
@@ -183,8 +249,9 @@ template <int DT, int V>
 void route_with(const RouteArgs &a, hipStream_t stream) {
     const int64_t bytes = (DT == RQ_F32 ? 4 : 2) * V, align = bytes < 16 ? bytes : 16;
     const bool    vec = a.E % V == 0 && (uintptr_t) a.logits % align == 0 && (a.M == 1 || a.ldl * (DT == RQ_F32 ? 4 : 2) % align == 0);
+    const bool    vec_bias = V > 1 && a.bias && a.E % V == 0 && (uintptr_t) a.bias % (V < 4 ? 4 * V : 16) == 0;
     const dim3    grid((unsigned) ((a.M + kRouteThreads / 64 - 1) / (kRouteThreads / 64)));
-    hipLaunchKernelGGL((rq_route_kernel<DT, V>), grid, dim3(kRouteThreads), 0, stream, a, vec);
+    hipLaunchKernelGGL((rq_route_kernel<DT, V>), grid, dim3(kRouteThreads), 0, stream, a, vec, vec_bias);
 }
 template <int DT>
 hipError_t route(const RouteArgs &a, hipStream_t stream) {

@@ -276,7 +276,8 @@ def test_product_with_nan_and_infinity(M):
 ROUTES = [  # M, E, top, groups, top_groups
     (1, 1, 1, 1, 1), (1, 64, 8, 1, 1), (5, 7, 7, 1, 1), (130, 64, 1, 1, 1), (33, 65, 6, 1, 1), (64, 128, 32, 1, 1), (17, 256, 8, 8, 4),
     (100, 160, 6, 8, 3), (50, 24, 3, 4, 2), (9, 10, 2, 5, 2), (40, 8, 4, 8, 4), (3, 1024, 16, 1, 1), (20, 1024, 8, 64, 7), (31, 63, 5, 3, 1),
-    (2, 300, 9, 1, 1), (12, 512, 10, 4, 4)]
+    (2, 300, 9, 1, 1), (12, 512, 10, 4, 4), (19, 256, 8, 2, 1), (40, 128, 6, 16, 5), (21, 128, 9, 4, 2), (12, 192, 5, 6, 2), (70, 256, 32, 32, 9),
+    (6, 512, 3, 2, 2), (300, 256, 12, 1, 1)]
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
@@ -339,6 +340,16 @@ def test_route_with_a_bias_of_infinities_and_nan():
         ids, w = rq.route(_gpu(x), top, scoring="sigmoid", bias=_gpu(bias), groups=groups, top_groups=top_groups)
         assert ids.cpu().tolist() == [want]
         assert np.allclose(w.cpu().numpy(), 1 / top, rtol=2e-7)
+
+
+@pytest.mark.parametrize("E,groups", [(64, 1), (128, 4), (256, 8), (512, 2), (1000, 1)])
+def test_route_reads_a_bias_at_any_address(E, groups):
+    x, room = torch.randn((33, E), device=DEV), torch.randn(E + 3, device=DEV)
+    for at in range(4):
+        bias = room[at:at + E]
+        for scoring in ("softmax", "sigmoid"):
+            for a, b in zip(rq.route(x, 5, scoring, bias, groups, groups), rq.route(x, 5, scoring, bias.clone(), groups, groups)):
+                assert torch.equal(a, b)
 
 
 def test_route_reads_rows_of_a_wider_matrix():
