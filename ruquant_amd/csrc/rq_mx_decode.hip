@@ -61,37 +61,19 @@ struct Tokens {
     }
 };
 
-// Eight elements of a token from k on (zeros past its end)
+// Eight elements of a token from 8 u on (zeros past its end)
 template <int DT>
-__device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, bool aligned, int K, int u, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0;
+__device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, bool aligned, int K, int u, Unit<DT> &v) {
+    v.clear();
     if (u * 8 >= K) return;
-    const typename Element<DT>::type *p = x + u * 8;
-    if (!aligned) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float(p[i]);
-    } else if constexpr (DT == RQ_F32) {
-        const v4f a = *reinterpret_cast<const v4f *>(p), b = *reinterpret_cast<const v4f *>(p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
-    } else {
-        const v4i a = *reinterpret_cast<const v4i *>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = to_float(__builtin_bit_cast(typename Element<DT>::type, (uint16_t) a[i]));
-            v[2 * i + 1] = to_float(__builtin_bit_cast(typename Element<DT>::type, (uint16_t) ((uint32_t) a[i] >> 16)));
-        }
-    }
+    if (aligned) v.template load<true>(x + u * 8);
+    else v.template load<false>(x + u * 8);
 }
 // ... rounded by the four lanes that hold their block
-__device__ __forceinline__ void store_unit(uint8_t *codes, uint8_t *scales, int u, const float (&v)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max_of_four(top);
-    const int X = block_scale(top);
-    *reinterpret_cast<uint32_t *>(codes + u * 4) = X == 255 ? 0u : pack8(v, scale_down(X));
+template <int DT>
+__device__ __forceinline__ void store_unit(uint8_t *codes, uint8_t *scales, int u, const Unit<DT> &v) {
+    const int X = block_scale(max_of_four(v.top()));
+    *reinterpret_cast<uint32_t *>(codes + u * 4) = v.pack(X);
     if ((u & 3) == 0) scales[u >> 2] = (uint8_t) X;
 }
 
@@ -105,7 +87,7 @@ __device__ __forceinline__ void stream(const Rows (&rows)[MAT][NR], const Lane &
     const Tokens tokens(lds, T, steps);
     const int    wave = threadIdx.x >> 6, u0 = threadIdx.x;
     const int    s0 = steps * wave / W, s1 = steps * (wave + 1) / W;
-    float        v[2][8];
+    Unit<DT> v[2];
     if constexpr (!ROWS) {   // (the first two units of the first token: all there is of a short one)
         if (u0 < units) load_unit<DT>(x, a.aligned, K, u0, v[0]);
         if (u0 + kThreads < units) load_unit<DT>(x, a.aligned, K, u0 + kThreads, v[1]);
@@ -244,7 +226,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void rq_mx_decode_gate_up_kernel(co
         }
         top = max_of_four(top);
         const int X = block_scale(top), b = blockIdx.x, blocks = gridDim.x;
-        reinterpret_cast<uint32_t *>(a.h_codes + (int64_t) slot * a.h_stride + b * 16)[threadIdx.x] = X == 255 ? 0u : pack8(h, scale_down(X));
+        reinterpret_cast<uint32_t *>(a.h_codes + (int64_t) slot * a.h_stride + b * 16)[threadIdx.x] = pack8(h, X);
         if (threadIdx.x == 0) {
             uint8_t *s = a.h_scales + (int64_t) slot * (a.h_stride >> 4);
             s[b] = (uint8_t) X;

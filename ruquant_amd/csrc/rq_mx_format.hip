@@ -23,26 +23,6 @@ Divider make_divider(uint32_t d) {
 }
 __device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &v) { return (uint32_t) (((uint64_t) n * v.mul) >> v.shift); }
 
-// eight consecutive elements as floats
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const typename Element<DT>::type *p, float (&v)[8]) {
-    if constexpr (!VEC) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float(p[i]);
-    } else if constexpr (DT == RQ_F32) {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-        const uint4    a = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = { a.x, a.y, a.z, a.w };
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = to_float(__builtin_bit_cast(typename Element<DT>::type, (uint16_t) (w[i] & 0xFFFF)));
-            v[2 * i + 1] = to_float(__builtin_bit_cast(typename Element<DT>::type, (uint16_t) (w[i] >> 16)));
-        }
-    }
-}
-
 // Eight elements a thread, so four lanes hold a block and its maximum crosses them in two steps. ACT: the workspace's form, rows
 // padded with zeros; otherwise rows of K / 2 and K / 32 bytes.
 template <int DT, bool VEC, bool ACT>
@@ -52,14 +32,11 @@ __global__ __launch_bounds__(kThreads) void rq_mx_quantize_kernel(const typename
     const uint32_t n = blockIdx.x * kThreads + threadIdx.x;
     if (n >= units) return;   // (whole blocks: units is a multiple of four)
     const uint32_t m = divide(n, per_row), u = n - m * per_row.d;
-    float          v[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
-    if (!ACT || (int64_t) u * 8 < K) load8<DT, VEC>(x + (int64_t) m * ldx + (int64_t) u * 8, v);
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max_of_four(top);
-    const int      X = block_scale(top);
-    const uint32_t c = X == 255 ? 0u : pack8(v, scale_down(X));
+    Unit<DT>       v;
+    v.clear();
+    if (!ACT || (int64_t) u * 8 < K) v.template load<VEC>(x + (int64_t) m * ldx + (int64_t) u * 8);
+    const int      X = block_scale(max_of_four(v.top()));
+    const uint32_t c = v.pack(X);
     if (!ACT || (int64_t) u * 4 < code_stride) *reinterpret_cast<uint32_t *>(codes + (int64_t) m * code_stride + (int64_t) u * 4) = c;
     if ((u & 3) == 0) {
         const uint32_t b = u >> 2;
@@ -82,22 +59,17 @@ __global__ __launch_bounds__(kThreads) void rq_mx_panel_quantize_kernel(const ty
     if (m < 0) return;   // (all eight threads of a row)
     uint8_t *codes = panels + ((int64_t) block * L.steps * 2 + part * 4) * 1024 + ((u >> 2) * 32 + row) * 16 + (u & 3) * 4;
     uint32_t word = 0;
-    float    v[4][8];
+    Unit<DT> v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int64_t k = (int64_t) part * 256 + j * 64 + u * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = 0;
-        if (k < L.K) load8<DT, VEC>(x + m * ldx + k, v[j]);
+        v[j].clear();
+        if (k < L.K) v[j].template load<VEC>(x + m * ldx + k);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
-        top = max_of_four(top);
-        const int X = block_scale(top);
-        if (part * 4 + j < 2 * L.steps) *reinterpret_cast<uint32_t *>(codes + j * 1024) = X == 255 ? 0u : pack8(v[j], scale_down(X));
+        const int X = block_scale(max_of_four(v[j].top()));
+        if (part * 4 + j < 2 * L.steps) *reinterpret_cast<uint32_t *>(codes + j * 1024) = v[j].pack(X);
         word |= (uint32_t) X << (8 * j);
     }
     if ((u & 3) == 0)
