@@ -221,6 +221,20 @@ def test_product_whose_tiles_are_shared(M, K, N, dtype):
         assert torch.equal(rq.mx_mul_mat(W, x, workspace=ws), y)
 
 
+def test_shared_tiles_of_calls_behind_one_another():
+    """calls on one workspace with nothing between them: no sum of the one in front shows"""
+    K, N = 16384, 512
+    codes, scales = _weights((N,), K, 3)
+    W = rq.MXWeight(_gpu(codes), _gpu(scales))
+    xs = [_activations(M, K, M, torch.float32)[0] for M in (40, 64, 40, 17, 33, 64)]
+    want = [rq.mx_mul_mat(W, x) for x in xs]
+    torch.cuda.synchronize()
+    ws = W.workspace(64)
+    for _ in range(10):
+        got = [rq.mx_mul_mat(W, x, workspace=ws) for x in xs]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_one_workspace_serves_every_number_of_tokens():
     K, N, most = 8992, 300, 700
     codes, scales = _weights((N,), K, 3)
