@@ -222,12 +222,6 @@ struct Tile {
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
-// Rows of the slots in 16 bits, for outputs in bf16: fp16 numbers of a unit that 32 outputs share, 2^(X - 141), X the exponent of the
-// largest finite one (16 .. 254), which lies under 2^15 of it. An output is off by at most 2^-11 of itself, 1 / 8 of what its last rounding
-// to bf16 costs (and by no more than 2^-40 of the largest, under 2^-29 of it); infinities and NaN stay what they are. The rows' traffic,
-// which is what their sum takes, is halved. Outputs in fp16 have as many bits as such rows, so theirs are in fp32.
-constexpr int kRows16 = 3;
-
 struct ProductArgs {
     WeightLayout   L;
     const uint8_t *w, *w2;          // prepared weights; kGateUp: w the gate, w2 the up projection
@@ -242,9 +236,8 @@ struct ProductArgs {
     int            most_tiles;      //   so many; those past the last one have no tokens
     const int     *row_of;          // kDown: position -> row of y
     int            out_dtype;
-    void          *y;               // kDense: the result; kDown: rows of the slots, fp32 or kRows16
+    void          *y;               // kDense: the result; kDown: rows of the slots, fp32
     int64_t        ldy;
-    uint8_t       *row_scales;      // kRows16: ldy / 32 a row
     uint8_t       *h;               // kGateUp: the down projection's activations, panels by position
     WeightLayout   HP;
 };
@@ -291,30 +284,6 @@ __device__ __forceinline__ void store_out(int dtype, void *y, int64_t base, int6
     }
     store_out(dtype, y, base, n, N, x);
     store_out(dtype, y, base, n + 4, N, z);
-}
-// Eight outputs n .. n + 7 of a row in 16 bits, of 32 that this lane and its three neighbours have (N is padded to 64).
-__device__ __forceinline__ void store_rows16(const ProductArgs &a, int64_t row, int64_t n, const float *v) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max_of_four(top);
-    if (top >= 0x7F800000u) {   // (the four alike) the largest finite one's
-        top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t u = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-            top = max(top, u < 0x7F800000u ? u : 0u);
-        }
-        top = max_of_four(top);
-    }
-    const int   X = max((int) (top >> 23), 16);
-    const float by = __uint_as_float((uint32_t) (268 - X) << 23);   // 2^(141 - X)
-    uint32_t    w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pair_bits<RQ_F16>(v[2 * i] * by, v[2 * i + 1] * by);
-    if (n >= a.ldy) return;   // (a tile past the padded rows)
-    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y) + row * a.ldy + n) = make_uint4(w[0], w[1], w[2], w[3]);
-    if ((n & 31) == 0) a.row_scales[row * (a.ldy >> 5) + (n >> 5)] = (uint8_t) X;
 }
 // Block b (32 rows) of h = silu(gate) * up for the token in column lane % 32, from both lanes that hold it, as activations of the down
 // projection in row p. Behind the last block that the rows of h have (their padding to 64), the step's remaining scales are set
@@ -411,10 +380,9 @@ inline int64_t most_tiles(int64_t slots, int64_t E, int tile_tokens) {
     const int64_t some = slots < E ? slots : E;
     return some + slots / tile_tokens;
 }
-// y[m] = sum_j weights[m][j] * rows[m * top + j], over the slots whose id is an expert's. row_scales: rows of kRows16 with ld outputs
-// each; null: fp32 rows of N
-hipError_t launch_combine(const void *rows, const uint8_t *row_scales, int64_t ld, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E,
-                          int out_dtype, void *y, int64_t ldy, hipStream_t stream);
+// y[m] = sum_j weights[m][j] * rows[m * top + j], over the slots whose id is an expert's; rows of N
+hipError_t launch_combine(const float *rows, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E, int out_dtype, void *y,
+                          int64_t ldy, hipStream_t stream);
 
 struct RouteArgs {
     int            dtype;

@@ -29,12 +29,11 @@ struct ExpertsPlan {
     bool    decode;               // slot by slot (rq_mx_decode.hip); otherwise sorted by expert and tiled
     int     tile_tokens;          // of both products
     int     form;                 // of the tiles of both
-    bool    rows16;
-    int64_t slots, positions, tiles, ld;   // (ld: of rows16)
+    int64_t slots, positions, tiles;
     WeightLayout XP, HP;
-    size_t  x, h, h_scales, rows, row_scales, token_of, slot_of, tile_table, used, total;   // offsets
+    size_t  x, h, h_scales, rows, token_of, slot_of, tile_table, used, total;   // offsets
 };
-ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top, int out_dtype) {
+ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top) {
     ExpertsPlan p = {};
     p.slots = M * top;
     size_t at = 0;
@@ -61,12 +60,9 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
     p.positions = most_positions(p.slots, E);
     p.XP = weight_layout(p.positions, K);
     p.HP = weight_layout(p.positions, F);
-    p.rows16 = out_dtype == RQ_BF16;
-    p.ld = up_to(N, 64);
     p.x = take(p.XP.expert_bytes);
     p.h = take(p.HP.expert_bytes);
-    p.rows = take(p.rows16 ? p.slots * p.ld * 2 : p.slots * N * 4);
-    p.row_scales = take(p.rows16 ? p.slots * p.ld / 32 : 0);
+    p.rows = take(p.slots * N * 4);   // (fp32: what a token's slots cancel is not lost)
     p.token_of = take(p.positions * 4);
     p.slot_of = take(p.positions * 4);
     p.tile_table = take(most_tiles(p.slots, E, tiled_tokens(kForm64)) * (int64_t) sizeof(Tile));   // (room for the smallest, so that it grows with M)
@@ -156,9 +152,7 @@ extern "C" int rq_route(int dtype, const void *logits, int64_t ldl, int64_t M, i
 
 extern "C" size_t rq_mx4_experts_workspace_bytes(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top) {
     if (!good_experts(E, K, F, N, M, top)) return 0;
-    // (room for either kind of rows)
-    const size_t a = experts_plan(E, K, F, N, M, top, RQ_F32).total, b = experts_plan(E, K, F, N, M, top, RQ_BF16).total;
-    return (a > b ? a : b) + 256;
+    return experts_plan(E, K, F, N, M, top).total + 256;
 }
 
 extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down, int64_t E, int64_t K, int64_t F, int64_t N,
@@ -171,7 +165,7 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
         !aligned(weights, 4) || (M > 1 && (ldx < K || ldy < N))) {
         return RQ_E_ARGUMENT;
     }
-    const ExpertsPlan p = experts_plan(E, K, F, N, M, top, out_dtype);
+    const ExpertsPlan p = experts_plan(E, K, F, N, M, top);
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < p.total) return RQ_E_WORKSPACE;
     const hipStream_t st = (hipStream_t) stream;
     uint8_t *ws = (uint8_t *) workspace;
@@ -230,13 +224,9 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     d.panels = a.h;
     d.P = p.HP;
     d.row_of = s.slot_of;
-    d.out_dtype = p.rows16 ? kRows16 : RQ_F32;
     d.y = ws + p.rows;
-    d.ldy = p.rows16 ? p.ld : N;
-    d.row_scales = ws + p.row_scales;
+    d.ldy = N;
     if (e == hipSuccess) e = launch_tiled(kDown, p.form, d, st);
-    if (e == hipSuccess) {
-        e = launch_combine(ws + p.rows, p.rows16 ? d.row_scales : nullptr, d.ldy, N, ids, weights, M, top, (int) E, out_dtype, y, ldy, st);
-    }
+    if (e == hipSuccess) e = launch_combine((const float *) (ws + p.rows), N, ids, weights, M, top, (int) E, out_dtype, y, ldy, st);
     return e;
 }

@@ -271,7 +271,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
         constexpr int kStride = 68;
         static_assert(G::kWaves * 32 * kStride * 4 <= G::kBytes, "a region per wavefront");
         float    *mine = reinterpret_cast<float *>(lds) + g.wave * 32 * kStride;
-        const int dtype = a.out_dtype;   // (kDown: RQ_F32 or kRows16)
+        const int dtype = MODE == kDown ? RQ_F32 : a.out_dtype;
         // (the rows of this wavefront's tokens, a token a lane)
         int64_t row_at[TB];
 #pragma unroll
@@ -319,10 +319,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
             for (int i = 0; i < 32 / kTokens; ++i) {
                 const int     at = i * kTokens + lane / kLanes;
                 const int64_t row = MODE == kDown ? __shfl((int) row_at[t], at) : tile.first + first + at;
-                if (first + at < tile.count) {
-                    if (MODE == kDown && dtype == kRows16) store_rows16(a, row, n0, mine + at * kStride + n);
-                    else store_out(dtype, a.y, row * a.ldy, n0, a.L.N, mine + at * kStride + n);
-                }
+                if (first + at < tile.count) store_out(dtype, a.y, row * a.ldy, n0, a.L.N, mine + at * kStride + n);
             }
         };
 #pragma unroll

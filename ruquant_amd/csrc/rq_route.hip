@@ -347,79 +347,50 @@ __global__ __launch_bounds__(kSortThreads) void rq_sort_kernel(const SortArgs a)
     }
 }
 
-// y[m] = sum_j weights[m][j] * rows[m top + j] in the order of j, fp32; the slots' rows are loaded four at a time, 16 bytes a thread and
-// slot: four outputs of fp32 rows, eight of 16-bit ones. Bound by memory: 2048 tokens x 8 rows of 5120 in 16 bits, 31 us for 194 MB,
-// half of them from the memory-side cache that the down projection has just filled.
-template <int DT, bool ROWS16, bool VEC>
-__global__ __launch_bounds__(256) void rq_combine_kernel(const void *rows, const uint8_t *row_scales, int64_t ld, int64_t N, const int32_t *ids,
-                                                         const float *weights, int top, int E, typename Element<DT>::type *y, int64_t ldy) {
-    constexpr int kEach = ROWS16 ? 8 : 4;
-    const int64_t m = blockIdx.x, n = ((int64_t) blockIdx.y * 256 + threadIdx.x) * kEach;
+// y[m] = sum_j weights[m][j] * rows[m top + j] in the order of j, fp32; the slots' rows are loaded four at a time, four outputs a
+// thread. Bound by memory.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void rq_combine_kernel(const float *rows, int64_t N, const int32_t *ids, const float *weights, int top, int E,
+                                                         typename Element<DT>::type *y, int64_t ldy) {
+    const int64_t m = blockIdx.x, n = ((int64_t) blockIdx.y * 256 + threadIdx.x) * 4;
     if (n >= N) return;
-    float sum[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) sum[i] = 0;
+    v4f sum = { 0, 0, 0, 0 };
     for (int j0 = 0; j0 < top; j0 += 4) {
-        v4i   v[4];
+        v4f   v[4];
         float w[4];
-        int   X[4];
         bool  there[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int64_t slot = m * top + j0 + k;
             const int     e = j0 + k < top ? ids[slot] : -1;
             there[k] = e >= 0 && e < E;
-            v[k] = v4i{ 0, 0, 0, 0 };
-            w[k] = 0, X[k] = 0;
+            v[k] = v4f{ 0, 0, 0, 0 };
+            w[k] = 0;
             if (there[k]) {
                 w[k] = weights[slot];
-                if constexpr (ROWS16) {
-                    v[k] = *reinterpret_cast<const v4i *>(reinterpret_cast<const uint16_t *>(rows) + slot * ld + n);
-                    X[k] = row_scales[slot * (ld >> 5) + (n >> 5)];
-                } else if constexpr (VEC) {
-                    v[k] = *reinterpret_cast<const v4i *>(reinterpret_cast<const float *>(rows) + slot * ld + n);
+                const float *row = rows + slot * N + n;
+                if constexpr (VEC) {
+                    v[k] = *reinterpret_cast<const v4f *>(row);
                 } else {
                     for (int i = 0; i < 4; ++i)
-                        if (n + i < N) v[k][i] = reinterpret_cast<const int *>(rows)[slot * ld + n + i];
+                        if (n + i < N) v[k][i] = row[i];
                 }
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (!there[k]) continue;
-            if constexpr (ROWS16) {
-                // (2^(X - 141) is a normal number from X = 16 on in two factors only: 2^(X - 127) and 2^-14)
-                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-                const float unit = __uint_as_float((uint32_t) X[k] << 23);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int two = v[k][i];   // (of an element of a vector itself, the compiler casts element 0)
-                    const h2  h = __builtin_bit_cast(h2, two);
-                    sum[2 * i] += w[k] * ((float) h[0] * 6.103515625e-05f * unit);
-                    sum[2 * i + 1] += w[k] * ((float) h[1] * 6.103515625e-05f * unit);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += w[k] * __int_as_float(v[k][i]);
-            }
-        }
+        for (int k = 0; k < 4; ++k)
+            if (there[k]) sum += w[k] * v[k];
     }
-#pragma unroll
-    for (int i = 0; i < kEach; i += 4) store_out(DT, y, m * ldy, n + i, N, v4f{ sum[i], sum[i + 1], sum[i + 2], sum[i + 3] });
+    store_out(DT, y, m * ldy, n, N, sum);
 }
 
 template <int DT>
-hipError_t combine(const void *rows, const uint8_t *row_scales, int64_t ld, int64_t N, const int32_t *ids, const float *weights, int64_t M,
-                   int top, int E, void *y, int64_t ldy, hipStream_t stream) {
-    auto *out = reinterpret_cast<typename Element<DT>::type *>(y);
-    if (row_scales) {
-        const dim3 grid((unsigned) M, (unsigned) ((N + 2047) / 2048));
-        hipLaunchKernelGGL((rq_combine_kernel<DT, true, true>), grid, dim3(256), 0, stream, rows, row_scales, ld, N, ids, weights, top, E, out, ldy);
-    } else {
-        const dim3 grid((unsigned) M, (unsigned) ((N + 1023) / 1024));
-        if (ld % 4 == 0) hipLaunchKernelGGL((rq_combine_kernel<DT, false, true>), grid, dim3(256), 0, stream, rows, row_scales, ld, N, ids, weights, top, E, out, ldy);
-        else hipLaunchKernelGGL((rq_combine_kernel<DT, false, false>), grid, dim3(256), 0, stream, rows, row_scales, ld, N, ids, weights, top, E, out, ldy);
-    }
+hipError_t combine(const float *rows, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E, void *y, int64_t ldy,
+                   hipStream_t stream) {
+    auto      *out = reinterpret_cast<typename Element<DT>::type *>(y);
+    const dim3 grid((unsigned) M, (unsigned) ((N + 1023) / 1024));
+    if (N % 4 == 0) hipLaunchKernelGGL((rq_combine_kernel<DT, true>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E, out, ldy);
+    else hipLaunchKernelGGL((rq_combine_kernel<DT, false>), grid, dim3(256), 0, stream, rows, N, ids, weights, top, E, out, ldy);
     return hipGetLastError();
 }
 
@@ -440,11 +411,11 @@ hipError_t launch_sort(const SortArgs &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-hipError_t launch_combine(const void *rows, const uint8_t *row_scales, int64_t ld, int64_t N, const int32_t *ids, const float *weights, int64_t M,
-                          int top, int E, int out_dtype, void *y, int64_t ldy, hipStream_t stream) {
-    if (out_dtype == RQ_F32) return combine<RQ_F32>(rows, row_scales, ld, N, ids, weights, M, top, E, y, ldy, stream);
-    if (out_dtype == RQ_F16) return combine<RQ_F16>(rows, row_scales, ld, N, ids, weights, M, top, E, y, ldy, stream);
-    return combine<RQ_BF16>(rows, row_scales, ld, N, ids, weights, M, top, E, y, ldy, stream);
+hipError_t launch_combine(const float *rows, int64_t N, const int32_t *ids, const float *weights, int64_t M, int top, int E, int out_dtype, void *y,
+                          int64_t ldy, hipStream_t stream) {
+    if (out_dtype == RQ_F32) return combine<RQ_F32>(rows, N, ids, weights, M, top, E, y, ldy, stream);
+    if (out_dtype == RQ_F16) return combine<RQ_F16>(rows, N, ids, weights, M, top, E, y, ldy, stream);
+    return combine<RQ_BF16>(rows, N, ids, weights, M, top, E, y, ldy, stream);
 }
 
 }  // namespace mx
