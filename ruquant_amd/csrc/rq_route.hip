@@ -97,7 +97,11 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
         for (int j = 0; j < V; ++j) s[j] = j < mine ? s[j] : -INFINITY;
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = s[j] != s[j] ? -INFINITY : s[j];
+    for (int j = 0; j < V; ++j) {
+        if (!a.bias) bias[j] = 0;
+        bias[j] = s[j] != s[j] ? s[j] : bias[j];   // (what the choice goes by is NaN then, and the score 0)
+        s[j] = s[j] != s[j] ? -INFINITY : s[j];
+    }
     if (a.scoring == 0) {
         int most = kNever;
 #pragma unroll
@@ -119,8 +123,7 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
     // what the choice goes by: numbers from the lowest finite one up
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float v = s[j];
-        if (a.bias) v += bias[j];
+        const float v = s[j] + bias[j];
         c[j] = j < mine ? ordered(v > kLowest ? v : kLowest) : kNever;   // (a NaN is not greater)
     }
     if (a.groups > 1) {
@@ -153,8 +156,8 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
         if (share > 2) join(moved<0x141, 0xF>(one, kNever), moved<0x141, 0xF>(two, kNever));
         if (share > 3) join(moved<0x140, 0xF>(one, kNever), moved<0x140, 0xF>(two, kNever));
         if (share > 4) join(__shfl_xor(one, 16), __shfl_xor(two, 16));
-        float worth = size > 1 ? unordered(one) + unordered(two) : unordered(one);
-        worth = worth > kLowest ? worth : kLowest;
+        // (from half the lowest number up each, so that one number in front of nothing is more than two of those)
+        const float worth = size > 1 ? fmaxf(unordered(one), 0.5f * kLowest) + fmaxf(unordered(two), 0.5f * kLowest) : unordered(one);
         int place = 0;   // groups that are worth more, or as much in front of it
         for (int g = 0; g < a.groups; ++g) {
             const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(worth), g << share));
