@@ -57,7 +57,7 @@ int rq_mx4_mul_mat(const void *prepared_dev, int64_t K, int64_t N, int in_dtype,
  * is held in 64 bits) or sigmoid(logits) (scoring 1); the choice goes by c = s + bias (bias may be null). With groups > 1 the
  * experts are `groups` runs of E / groups; only those of the top_groups groups whose two largest c have the largest sums can be
  * chosen. ids[m][j]: the experts with the largest c, in falling order, ties to the lowest index; weights[m][j] = s of the chosen
- * ones (without bias), divided by their sum if renormalize (0 where that is 0), times scale. A NaN logit scores 0 whatever its bias, and
+ * ones (without bias), divided by their sum (in 64 bits) if renormalize (0 where that is 0), times scale. A NaN logit scores 0 whatever its bias, and
  * is chosen behind every number, as an expert is whose bias is NaN or minus infinity; a group that holds a number is in front of one that
  * holds only such experts. */
 int rq_route(int dtype, const void *logits_dev, int64_t ldl, int64_t M, int64_t E, int scoring, const float *bias_dev, int groups,

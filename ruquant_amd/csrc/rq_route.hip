@@ -175,8 +175,9 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
             if (!((kept >> (min(of, a.groups - 1) << share)) & 1)) c[j] = kNever;
         }
     }
-    float chosen = 0, total = 0;
-    int   id = 0;
+    float  chosen = 0;
+    double total = 0;   // (so that small scores beside a large one are not lost one after the other)
+    int    id = 0;
     if constexpr (V > 1 && V <= 4) {
         // Each lane's experts in falling order, so that a round looks at its first and takes it off: 19 instructions for 30. (Neighbours are
         // compared, and change places where the second is larger: equal ones keep their order. V = 8 and 16 would sort as long as they save.)
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
             const float of = __shfl(s[j], id / V);
             chosen = id % V == j ? of : chosen;
         }
-        for (int i = 0; i < a.top; ++i) total += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(chosen), i));
+        for (int i = 0; i < a.top; ++i) total += (double) __int_as_float(__builtin_amdgcn_readlane(__float_as_int(chosen), i));
     } else {
         for (int i = 0; i < a.top; ++i) {
             int most = c[0];
@@ -237,12 +238,12 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
             const int   e = from * V + at;
 #pragma unroll
             for (int j = 0; j < V; ++j) c[j] = lane == (at == j ? from : -1) ? kNever : c[j];
-            total += picked;
+            total += (double) picked;
             if (lane == i) chosen = picked, id = e;
         }
     }
     if (lane < a.top) {
-        const float w = a.renormalize ? (total > 0 ? chosen / total : 0.0f) : chosen;
+        const float sum = (float) total, w = a.renormalize ? (sum > 0 ? chosen / sum : 0.0f) : chosen;
         a.ids[m * a.top + lane] = id;
         a.weights[m * a.top + lane] = w * a.scale;
     }

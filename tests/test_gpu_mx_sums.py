@@ -56,3 +56,18 @@ def test_output_is_rounded_once(M, E, top, K, F, N):
     for dtype in (torch.bfloat16, torch.float16):
         out = rq.expert_ffn(gate, up, down, x, ids, w, out=torch.empty((M, N), dtype=dtype, device=DEV))
         assert torch.equal(out, y.to(dtype))
+
+
+@pytest.mark.parametrize("E", [40, 128, 256, 300, 1024])
+def test_weights_are_shares_of_the_whole_sum(E):
+    """One score of 1 and 31 of 2^-24.5, each of which an fp32 sum that holds the first would drop. The sum is exact to 2^-24, and so are
+    the first score (1 exactly) and the quotient; exp's error is one of 2^-19 in 31 scores that are 2^-19.6 of the sum."""
+    logits = torch.full((3, E), -30.0, device=DEV)
+    at = torch.arange(0, 32, device=DEV) * (E // 32)
+    logits[:, at] = -17.0
+    logits[:, at[7]] = 40.0
+    ids, w = rq.route(logits, 32, scoring="sigmoid")
+    small = 1 / (1 + np.exp(17.0))
+    assert (ids[:, 0] == at[7]).all()
+    assert np.abs(w[:, 0].double().cpu().numpy() - 1 / (1 + 31 * small)).max() <= 4 * 2.0 ** -24
+    assert np.allclose(w[:, 1:].double().cpu().numpy(), small, rtol=2.0 ** -18)
