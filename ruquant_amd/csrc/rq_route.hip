@@ -250,12 +250,20 @@ __global__ __launch_bounds__(kRouteThreads) void rq_route_kernel(const RouteArgs
 }
 
 template <int DT, int V>
-void route_with(const RouteArgs &a, hipStream_t stream) {
+void route_with(RouteArgs a, hipStream_t stream) {
     const int64_t bytes = (DT == RQ_F32 ? 4 : 2) * V, align = bytes < 16 ? bytes : 16;
     const bool    vec = a.E % V == 0 && (uintptr_t) a.logits % align == 0 && (a.M == 1 || a.ldl * (DT == RQ_F32 ? 4 : 2) % align == 0);
     const bool    vec_bias = V > 1 && a.bias && a.E % V == 0 && (uintptr_t) a.bias % (V < 4 ? 4 * V : 16) == 0;
-    const dim3    grid((unsigned) ((a.M + kRouteThreads / 64 - 1) / (kRouteThreads / 64)));
-    hipLaunchKernelGGL((rq_route_kernel<DT, V>), grid, dim3(kRouteThreads), 0, stream, a, vec, vec_bias);
+    // (a launch has under 2^32 threads, and a token is 64 of them; the rows in front of a launch are a multiple of 16 bytes for any stride)
+    constexpr int64_t kMost = 1 << 25;
+    for (int64_t left = a.M; left > 0; left -= kMost) {
+        a.M = left < kMost ? left : kMost;
+        const dim3 grid((unsigned) ((a.M + kRouteThreads / 64 - 1) / (kRouteThreads / 64)));
+        hipLaunchKernelGGL((rq_route_kernel<DT, V>), grid, dim3(kRouteThreads), 0, stream, a, vec, vec_bias);
+        a.logits = reinterpret_cast<const typename Element<DT>::type *>(a.logits) + a.M * a.ldl;
+        a.ids += a.M * a.top;
+        a.weights += a.M * a.top;
+    }
 }
 template <int DT>
 hipError_t route(const RouteArgs &a, hipStream_t stream) {
