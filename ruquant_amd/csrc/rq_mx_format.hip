@@ -45,13 +45,16 @@ __global__ __launch_bounds__(kThreads) void rq_mx_quantize_kernel(const typename
 }
 
 // The panel form: a workgroup has 32 rows x 256 elements, eight threads a row and run of 64, so that a wavefront reads eight rows'
-// lines and writes two lines of codes; a thread's four scales are one word.
+// lines and writes two lines of codes; a thread's four scales are one word. The grid is the parts of a row, then the row blocks: the threads of a
+// long call are more than one dimension of a grid may have.
+constexpr int kPanelBlocks = 32768;
 template <int DT, bool VEC>
 __global__ __launch_bounds__(kThreads) void rq_mx_panel_quantize_kernel(const typename Element<DT>::type *x, int64_t ldx, WeightLayout L,
                                                                         const int *row_of, const int *rows, uint8_t *panels, int *zero, int zeros) {
-    for (int i = blockIdx.x * kThreads + threadIdx.x; i < zeros; i += gridDim.x * kThreads) zero[i] = 0;
+    if (blockIdx.y == 0 && blockIdx.z == 0)
+        for (int i = blockIdx.x * kThreads + threadIdx.x; i < zeros; i += gridDim.x * kThreads) zero[i] = 0;
     const int     parts = 2 * L.chunks;
-    const int     block = blockIdx.x / parts, part = blockIdx.x - block * parts;
+    const int     block = blockIdx.z * kPanelBlocks + blockIdx.y, part = blockIdx.x;
     const int     row = threadIdx.x >> 3, u = threadIdx.x & 7;
     const int64_t r = (int64_t) block * 32 + row;
     if ((int64_t) block * 32 >= (rows ? *rows : L.N)) return;
@@ -174,7 +177,8 @@ hipError_t panel_quantize(const void *x_, int64_t ldx, const WeightLayout &L, co
     using T = typename Element<DT>::type;
     const T   *x = reinterpret_cast<const T *>(x_);
     const bool vec = (uintptr_t) x % 16 == 0 && ldx * (int64_t) sizeof(T) % 16 == 0;
-    const dim3 grid((unsigned) ((L.N + 31) / 32 * 2 * L.chunks));
+    const int64_t blocks = (L.N + 31) / 32;
+    const dim3    grid((unsigned) (2 * L.chunks), (unsigned) (blocks < kPanelBlocks ? blocks : kPanelBlocks), (unsigned) ((blocks + kPanelBlocks - 1) / kPanelBlocks));
     if (vec) hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, true>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels, zero, zeros);
     else hipLaunchKernelGGL((rq_mx_panel_quantize_kernel<DT, false>), grid, dim3(kThreads), 0, stream, x, ldx, L, row_of, rows, panels, zero, zeros);
     return hipGetLastError();

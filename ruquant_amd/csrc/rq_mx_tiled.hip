@@ -190,14 +190,16 @@ struct Tiled {
 // wavefront: 512 outputs of 17408 inputs, 64 tokens, 4 parts 13.7 us, 16 parts 17.2, 2048 outputs, 8 parts 29.4; so 13.6, 16.1, 16.4.
 // Unshared 22.0 and 22.5.)
 template <int MODE, int RB, int TB, int WC, int R, bool SPLIT>
-__global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB <= 4 ? 3 : 2) void rq_mx_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles) {
+__global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB <= 4 ? 3 : 2) void rq_mx_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles, const int across) {
     using G = Tiled<MODE, RB, TB, WC, R>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     // Workgroups go to the XCDs in turn. Each XCD takes a run of the tiles in an order in which the token tiles run fastest, so that
     // those that share rows of the weight share an L2.
     const int total = row_tiles * token_tiles * (SPLIT ? a.splits : 1);
-    const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
-    const int place_of = xcd * each + min(xcd, more) + (int) (blockIdx.x >> 3);
+    const int index = (int) blockIdx.y * across + (int) blockIdx.x;   // (across: a multiple of 8 where there is more than one row of them)
+    if (index >= total) return;
+    const int xcd = index & 7, each = total >> 3, more = total & 7;
+    const int place_of = xcd * each + min(xcd, more) + (index >> 3);
     const int v = SPLIT ? place_of / a.splits : place_of, part = SPLIT ? place_of - v * a.splits : 0;
     const int row_tile = v / token_tiles, token_tile = v - row_tile * token_tiles;
     Tile tile = { 0, 0, 0, 0 };
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     // (a wavefront's number mod 4 is its SIMD: the two that a tile with half of its tokens leaves idle, or the four, are of all of them; with
     // four wavefronts the workgroups take turns)
     g.wr = g.wave & 1;
-    g.wc = WC == 2 ? ((g.wave >> 1) ^ (int) (blockIdx.x >> 3)) & 1 : g.wave >> 1;
+    g.wc = WC == 2 ? ((g.wave >> 1) ^ (index >> 3)) & 1 : g.wave >> 1;
     g.lane16 = g.lane * 16;
     const int step0 = SPLIT ? part * a.split_steps : 0;   // (a multiple of two: the scales' parts)
     g.steps = SPLIT ? min(a.split_steps, a.L.steps - step0) : a.L.steps;
@@ -343,18 +345,21 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     }
 }
 
+constexpr int64_t kAcross = 1 << 20;   // workgroups in one dimension of a grid, which may have under 2^32 threads
+
 template <int MODE, int RB, int TB, int WC, int R, bool SPLIT = false>
 hipError_t launch(const ProductArgs &a, hipStream_t stream) {
     using G = Tiled<MODE, RB, TB, WC, R>;
     const int row_tiles = MODE == kDense ? a.row_tiles : (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
     const int token_tiles = MODE == kDense ? (int) ((a.M + G::kTileTokens - 1) / G::kTileTokens) : a.most_tiles;
     const int64_t groups = (int64_t) row_tiles * token_tiles * (SPLIT ? a.splits : 1);
-    if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    if (groups > 0x7FFFFFFF - kAcross) return hipErrorInvalidConfiguration;
+    const unsigned across = (unsigned) (groups < kAcross ? groups : kAcross);
     static std::atomic<uint64_t> allowed{ 0 };   // devices on which the kernel may have its LDS
     const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R, SPLIT>), G::kBytes, allowed);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE, RB, TB, WC, R, SPLIT>), dim3((unsigned) groups), dim3(G::kThreads), G::kBytes, stream, a,
-                       row_tiles, token_tiles);
+    hipLaunchKernelGGL((rq_mx_tiled_kernel<MODE, RB, TB, WC, R, SPLIT>), dim3(across, (unsigned) ((groups + across - 1) / across)),
+                       dim3(G::kThreads), G::kBytes, stream, a, row_tiles, token_tiles, (int) across);
     return hipGetLastError();
 }
 
