@@ -29,13 +29,13 @@ extern "C" {
 #define RQ_ROUTE_MAX_E   1024       /* most experts of a routing call */
 #define RQ_ROUTE_MAX_TOP 32         /* most experts per token */
 
-/* x (M rows of K elements, row stride ldx elements) -> codes and scales. A block's X is the exponent of its largest magnitude
+/* x (M rows of K elements, row stride ldx elements, any alignment of its type) -> codes (4-byte aligned) and scales. A block's X is the exponent of its largest magnitude
  * less 2 (at least 0), so that the largest element lies in [4, 8) units; elements are rounded to the nearest, ties to the even
  * code, and saturate at 6. A block with an infinity or a NaN gets the scale 255 and zero codes. */
 int rq_mx4_quantize(int dtype, const void *x_dev, int64_t ldx, int64_t M, int64_t K, void *codes_dev, void *scales_dev,
                     rq_stream_t stream);
 
-/* codes and scales -> out (M rows of K elements, row stride ldo), rounded once to dtype. */
+/* codes (4-byte aligned) and scales -> out (M rows of K elements, row stride ldo elements, any alignment of its type), rounded once to dtype. */
 int rq_mx4_dequantize(int dtype, const void *codes_dev, const void *scales_dev, int64_t M, int64_t K, void *out_dev, int64_t ldo,
                       rq_stream_t stream);
 

@@ -231,6 +231,7 @@ using namespace rq::mx;
 
 namespace {
 bool known_dtype(int dtype) { return dtype == RQ_F32 || dtype == RQ_F16 || dtype == RQ_BF16; }
+bool element_aligned(const void *p, int dtype) { return (uintptr_t) p % (dtype == RQ_F32 ? 4 : 2) == 0; }
 // rows of K elements whose blocks are counted in 64 bits, but a row's own units in 32
 bool good_row(int64_t K) { return K > 0 && K % RQ_MX4_BLOCK == 0 && K <= (1ll << 30); }
 }  // namespace
@@ -238,7 +239,7 @@ bool good_row(int64_t K) { return K > 0 && K % RQ_MX4_BLOCK == 0 && K <= (1ll <<
 extern "C" int rq_mx4_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, void *codes, void *scales, rq_stream_t stream) {
     if (!known_dtype(dtype) || !good_row(K) || M < 0) return RQ_E_UNSUPPORTED;
     if (M == 0) return 0;
-    if (!x || !codes || !scales || (uintptr_t) codes % 4 || (M > 1 && ldx < K)) return RQ_E_ARGUMENT;
+    if (!x || !element_aligned(x, dtype) || !codes || !scales || (uintptr_t) codes % 4 || (M > 1 && ldx < K)) return RQ_E_ARGUMENT;
     uint8_t *c = (uint8_t *) codes, *s = (uint8_t *) scales;
     const hipStream_t st = (hipStream_t) stream;
     if (dtype == RQ_F32) return quantize<RQ_F32, false>(x, ldx, M, K, c, s, K / 2, K / 32, K / 8, st);
@@ -250,7 +251,7 @@ extern "C" int rq_mx4_dequantize(int dtype, const void *codes, const void *scale
                                  rq_stream_t stream) {
     if (!known_dtype(dtype) || !good_row(K) || M < 0) return RQ_E_UNSUPPORTED;
     if (M == 0) return 0;
-    if (!out || !codes || !scales || (uintptr_t) codes % 4 || (M > 1 && ldo < K)) return RQ_E_ARGUMENT;
+    if (!out || !element_aligned(out, dtype) || !codes || !scales || (uintptr_t) codes % 4 || (M > 1 && ldo < K)) return RQ_E_ARGUMENT;
     const uint8_t *c = (const uint8_t *) codes, *s = (const uint8_t *) scales;
     const hipStream_t st = (hipStream_t) stream;
     if (dtype == RQ_F32) return dequantize<RQ_F32>(c, s, M, K, out, ldo, st);
