@@ -46,7 +46,7 @@ int rq_mx4_prepare(const void *codes_dev, const void *scales_dev, int64_t E, int
                    size_t prepared_bytes, rq_stream_t stream);
 
 /* y[m][n] = sum_k x^[m][k] w[n][k], x^ the activations after rq_mx4_quantize's rounding, sums in fp32, rounded once to out_dtype.
- * x: M rows, stride ldx elements, any alignment of its type; y: row stride ldy elements. workspace: 256-byte aligned,
+ * x: M rows, stride ldx elements, any alignment of its type; y: row stride ldy elements, no memory of x. workspace: 256-byte aligned,
  * rq_mx4_workspace_bytes, need not be initialised, not shared by calls that can overlap; where that is 256 (a few tokens, which
  * the product quantises as it reads them) it is not looked at and may be null. It grows with M: the most tokens' serves all. */
 size_t rq_mx4_workspace_bytes(int64_t K, int64_t N, int64_t M);
@@ -66,7 +66,7 @@ int rq_route(int dtype, const void *logits_dev, int64_t ldl, int64_t M, int64_t 
 /* The experts' gated feed-forward: y[m] = sum_j weights[m][j] D_e h^, h = silu(G_e x^) * (U_e x^), e = ids[m][j], ^ the rounding of
  * rq_mx4_quantize, sums in fp32. gate, up: E prepared weights of F rows and K inputs; down: E of N rows and F inputs. ids and
  * weights: M x top, contiguous; an id outside 0 .. E - 1 adds nothing (its weight is not looked at).
- * The workspace's bytes serve every out_dtype and grow with M. */
+ * y shares no memory with the inputs. The workspace's bytes serve every out_dtype and grow with M. */
 size_t rq_mx4_experts_workspace_bytes(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top);
 int rq_mx4_experts(const void *gate_dev, const void *up_dev, const void *down_dev, int64_t E, int64_t K, int64_t F, int64_t N,
                    int in_dtype, const void *x_dev, int64_t ldx, int64_t M, const int32_t *ids_dev, const float *weights_dev,

@@ -127,8 +127,15 @@ def _output(out, M, N, what):
                   % (what, M, N, tuple(out.shape), out.stride()))
 
 
+def _workspace_bytes(workspace):
+    if not workspace.is_contiguous():
+        raise RqError("a workspace is one run of memory, got strides %s" % (workspace.stride(),))
+    return workspace.numel() * workspace.element_size()
+
+
 def mx_mul_mat(weight, x, out=None, workspace=None):
-    """y[M, N] = x^[M, K] . W^T, x^ = x rounded as by mx_quantize, sums in fp32, rounded once to out's type (x's by default)."""
+    """y[M, N] = x^[M, K] . W^T, x^ = x rounded as by mx_quantize, sums in fp32, rounded once to out's type (x's by default).
+    `out` shares no memory with x."""
     M, K, ldx = _rows(x, "mx_mul_mat")
     N = weight.N
     if weight.E != 1 or K != weight.K:
@@ -149,7 +156,7 @@ def mx_mul_mat(weight, x, out=None, workspace=None):
             workspace = x.new_empty((n,), dtype=torch.uint8)
             at = workspace.data_ptr()
     else:
-        n, at = workspace.numel() * workspace.element_size(), workspace.data_ptr()
+        n, at = _workspace_bytes(workspace), workspace.data_ptr()
         _elsewhere(index, workspace=workspace)
     if weight._index != index or out.get_device() != index:
         _elsewhere(index, weight=weight, out=out)
@@ -196,7 +203,7 @@ def expert_ffn(gate, up, down, x, ids, weights, out=None, workspace=None):
     values are rounded as by mx_quantize, sums are fp32, y is rounded once to out's type (x's by default).
 
     gate, up: MXWeight [E, F, K]; down: MXWeight [E, N, F]; ids [M, top] int32 and weights [M, top] fp32 as route gives them. An id
-    outside 0 .. E - 1 adds nothing (an expert that another device holds, a token that is padding)."""
+    outside 0 .. E - 1 adds nothing (an expert that another device holds, a token that is padding). `out` shares no memory with the inputs."""
     M, K, ldx = _rows(x, "expert_ffn")
     E, F, N = gate.E, gate.N, down.N
     if (up.E, up.N, up.K, down.E, down.K, gate.K) != (E, F, K, E, F, K):
@@ -220,7 +227,7 @@ def expert_ffn(gate, up, down, x, ids, weights, out=None, workspace=None):
         n = L.rq_mx4_experts_workspace_bytes(E, K, F, N, M, top)
         workspace = x.new_empty((n,), dtype=torch.uint8)
     else:
-        n = workspace.numel() * workspace.element_size()
+        n = _workspace_bytes(workspace)
     _elsewhere(index, gate=gate, up=up, down=down, ids=ids, weights=weights, out=out, workspace=workspace)
     rc = _on_device_of(x, L.rq_mx4_experts, gate._ptr, up._ptr, down._ptr, E, K, F, N, dt, x.data_ptr(), ldx, M, ids.data_ptr(),
                        weights.data_ptr(), top, odt, out.data_ptr(), ldy, workspace.data_ptr(), n)
