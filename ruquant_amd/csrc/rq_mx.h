@@ -359,7 +359,9 @@ struct ProductPlan {
 ProductPlan plan_product(int64_t M, int64_t N, int64_t K);
 int64_t     product_sums_bytes(int64_t M, int64_t N, int64_t K);   // for sums and counters of up to M tokens
 hipError_t launch_tiled_product(const ProductPlan &plan, const ProductArgs &a, hipStream_t stream);
+int tiled_rows(int form);   // of a tile
 int tiled_tokens(int form);
+int tiled_resident(int form);
 int64_t tiled_row_tiles(int mode, int form, int64_t N);
 
 // Sorts the slots by expert, every expert's from a multiple of 32 positions on, and cuts them into tiles of tile_tokens positions.

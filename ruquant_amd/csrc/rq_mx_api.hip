@@ -1,4 +1,7 @@
 // Entry points of the MXFP4 product, the routing and the experts' feed-forward: argument checks, workspaces, order of launches.
+#include <string.h>
+
+#include "../../include/rq_mx4_plan.h"
 #include "rq_mx.h"
 
 using namespace rq::mx;
@@ -229,4 +232,30 @@ extern "C" int rq_mx4_experts(const void *gate, const void *up, const void *down
     if (e == hipSuccess) e = launch_tiled(kDown, p.form, d, st);
     if (e == hipSuccess) e = launch_combine((const float *) (ws + p.rows), N, ids, weights, M, top, (int) E, out_dtype, y, ldy, st);
     return e;
+}
+
+extern "C" int rq_mx4_product_plan(int64_t K, int64_t N, int64_t M, int64_t plan[8]) {
+    if (!plan) return RQ_E_ARGUMENT;
+    if (rq_mx4_workspace_bytes(K, N, M) == 0 || M < 1) return RQ_E_UNSUPPORTED;
+    memset(plan, 0, 8 * sizeof(plan[0]));
+    plan[0] = alone(M, K, N) ? RQ_MX4_ALONE : few_tokens(M, K, N) ? RQ_MX4_ROWS : RQ_MX4_TILES;
+    if (plan[0] != RQ_MX4_TILES) return 0;
+    const ProductPlan p = plan_product(M, N, K);
+    plan[1] = tiled_rows(p.form);
+    plan[2] = tiled_tokens(p.form);
+    plan[3] = p.main_tiles;
+    if (p.rest >= 0) plan[4] = tiled_rows(p.rest), plan[5] = tiled_tokens(p.rest);
+    plan[6] = p.splits;
+    plan[7] = tiled_resident(p.form);
+    return 0;
+}
+
+extern "C" int rq_mx4_experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top, int64_t plan[3]) {
+    if (!plan) return RQ_E_ARGUMENT;
+    if (!good_experts(E, K, F, N, M, top) || M < 1) return RQ_E_UNSUPPORTED;
+    const ExpertsPlan p = experts_plan(E, K, F, N, M, top);
+    plan[0] = p.decode ? RQ_MX4_ALONE : RQ_MX4_TILES;
+    plan[1] = p.decode ? 0 : tiled_rows(p.form);
+    plan[2] = p.decode ? 0 : p.tile_tokens;
+    return 0;
 }

@@ -396,7 +396,9 @@ constexpr Form kForms[kTiledForms] = { { 64, 64, 2, .098, .155, 2.0 },   { 128, 
 
 }  // namespace
 
+int tiled_rows(int form) { return kForms[form].rows; }
 int tiled_tokens(int form) { return kForms[form].tokens; }
+int tiled_resident(int form) { return kForms[form].resident; }
 int64_t tiled_row_tiles(int mode, int form, int64_t N) {
     const int rows = mode == kGateUp ? kForms[form].rows / 2 : kForms[form].rows;
     return (N + rows - 1) / rows;

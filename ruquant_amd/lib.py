@@ -97,6 +97,9 @@ PROTOTYPES.update({
     "rq_mx4_experts_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _int]),
     "rq_mx4_experts": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _int, _ptr, _i64, _i64, _ptr, _ptr, _int, _int, _ptr, _i64,
                               _ptr, _size, _ptr]),
+    # include/rq_mx4_plan.h
+    "rq_mx4_product_plan": (_int, [_i64, _i64, _i64, _ptr]),
+    "rq_mx4_experts_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _int, _ptr]),
 })
 
 for _name in ("rq_w4a4_mul_mat", "rq_w4a4_mul_mat_fused"):
