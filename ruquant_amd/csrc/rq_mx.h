@@ -322,7 +322,7 @@ __device__ __forceinline__ void store_h(const ProductArgs &a, const v16f &gate, 
     }
 }
 // Few tokens (rq_mx_decode.hip): up to four that every workgroup quantises for itself, or up to 16 in row form (a_codes set). The
-// experts of up to four tokens in two launches; their h is rows of h_stride bytes of codes by slot, and of h_stride / 16 scales.
+// experts of few tokens in two launches; their h is rows of h_stride bytes of codes by slot, and of h_stride / 16 scales.
 struct DecodeArgs {
     WeightLayout   L;
     const uint8_t *w, *w2;

@@ -18,8 +18,22 @@ int64_t pad256(int64_t n) { return up_to(n, 256); }
 
 constexpr int64_t kMaxTokens = 1 << 22;   // rows of a call; slots of an experts' call
 
-// Most tokens whose experts' weights are streamed slot by slot, without sorting.
-constexpr int64_t kExpertsDecodeTokens = 4;
+// Whether the experts' weights are streamed slot by slot (rq_mx_decode.hip) or the slots are sorted and go in tiles: the first reads a weight again
+// for every slot that has it, the second has three launches more. Prices in us by the bytes of an expert's three weights and how many experts the
+// tokens can be expected to hit, from 14 sizes of K = 1024 to 5120, F = 256 to 4096, 8 to 256 experts, 1 to 32 a token, 1 to 24 tokens: the one that they
+// choose is at worst 2 % slower than the other, and 4 % over nine more sizes (K = 768 to 6144, F = 192 to 17408, 4 to 512 experts). (us, slot by slot -> tiles, K x F, experts: 5120 x 1280: 8 of 64 1 token 24.3 -> 36.4, 6 tokens
+// 83 -> 91, 8 105 -> 104, 12 152 -> 126; 8 of 8 2 tokens 31 -> 37, 4 48 -> 37; 32 of 64 4 tokens 200 -> 145; 2048 x 512: 8 of 256 16 tokens 46 -> 61, 8 of 8
+// 8 tokens 19 -> 25, 16 31 -> 25; 4096 x 4096, 2 of 8: 4 tokens 43 -> 47, 8 68 -> 52; 1024 x 256, 4 of 32: 24 tokens 17 -> 23.)
+constexpr int64_t kExpertsDecodeTokens = 24;   // (as far as was measured)
+bool experts_decode(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, int top) {
+    if (M > kExpertsDecodeTokens || K > 65536) return false;   // (K: a token in LDS)
+    const double mb = (double) F * (2 * K + N) * 17 / 32 * 1e-6, share = top < E ? (double) top / (double) E : 1.0;
+    double       missed = 1;
+    for (int64_t m = 0; m < M; ++m) missed *= 1 - share;
+    const double hit = (double) E * (1 - missed), again = (double) (M * top) - hit;
+    const double first = mb / 5.6 > .06 ? mb / 5.6 : .06, more = mb / 10 > .06 ? mb / 10 : .06;   // of a slot: its weight from memory, and from a cache
+    return 8 + hit * first + again * more + (double) (M * K) / 17000 <= 20 + hit * mb / 5;
+}
 // Products whose weights go from memory into registers (rq_mx_decode.hip): up to 16 tokens, fewer where the sizes make each more costly than
 // the tiles' start. (us, here -> in tiles, at the fewest tokens that go to those: K = 17408: N = 64 9 tokens 11.6 -> 11.0, N = 5120 4 tokens
 // 17.8 -> 16.6, N = 17408 2 tokens 29.2 -> 28.6; K = 8992, N = 5120 8 tokens 12.5 -> 12.7; K = 5120: N = 5120 14 tokens 10.5 -> 10.7, N = 9000
@@ -45,7 +59,7 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
         at += (size_t) pad256(bytes);
         return here;
     };
-    p.decode = M <= kExpertsDecodeTokens && K <= 65536;
+    p.decode = experts_decode(E, K, F, N, M, top);
     if (p.decode) {
         p.h = take(p.slots * (up_to(F, 256) / 2));
         p.h_scales = take(p.slots * (up_to(F, 256) / 32));

@@ -1,9 +1,9 @@
-// MXFP4 products for up to four tokens, and one token's experts: few launches, every workgroup quantises the tokens for itself.
+// MXFP4 products for up to 16 tokens, and the experts of few tokens: few launches, and weights from memory into registers.
 //
 // A call of this size is the stream of its weights and what stands in front of it and behind it, so a product is one launch: a
 // workgroup fetches the tokens first and its first weights behind them, quantises the tokens into LDS while the weights are on
-// their way, and its wavefronts split the inputs. One token's experts are two launches: gate and up of every chosen expert, then
-// the down projections of all of them with their weighted sum. 16x16x128 MFMAs: workgroups of 16 rows spread a small weight over
+// their way, and its wavefronts split the inputs. (From some size on a launch in front quantises them: decode_takes.) The experts are two
+// launches, too: gate and up of every slot, then the down projections of a token's slots with their weighted sum. 16x16x128 MFMAs: workgroups of 16 rows spread a small weight over
 // twice as many compute units as the 32 rows of the other form would.
 //
 // Bound by the weights' stream where they are large, by the chain of a load, the rounding, the products and the join of the inputs' parts

@@ -141,3 +141,11 @@ def test_rows_that_are_longer_than_a_products():
     for m in range(2):
         want = ref.quantize(x[m:m + 1].double().numpy())
         assert (scales[m].cpu().numpy() == want[1][0]).all() and (back[m].double().numpy() == ref.values(*want)[0]).all()
+
+
+@pytest.mark.parametrize("E,K,F,N,top", [(40, 288, 352, 100, 3), (256, 544, 96, 65, 8), (3, 416, 160, 300, 1)])
+@pytest.mark.parametrize("M", [5, 13, 24])
+def test_experts_of_some_tokens_slot_by_slot(M, E, K, F, N, top):
+    assert plans.experts(E, K, F, N, M, top)[0] == plans.ALONE
+    ids = np.random.default_rng(M).integers(-1, E, size=(M, top)).astype(np.int32)
+    _check_experts(E, K, F, N, M, top, ids, M)
