@@ -196,8 +196,10 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     // Workgroups go to the XCDs in turn. Each XCD takes a run of the tiles in an order in which the token tiles run fastest, so that
     // those that share rows of the weight share an L2.
     const int total = row_tiles * token_tiles * (SPLIT ? a.splits : 1);
-    const int index = (int) blockIdx.y * across + (int) blockIdx.x;   // (across: a multiple of 8 where there is more than one row of them)
-    if (index >= total) return;
+    // (A plain product's grid is one row: in the tiles that large ones take, outputs that made it too wide fit no memory, and the test costs 0.25 us. across: a
+    // multiple of 8 where there is more than one row.)
+    const int index = MODE == kDense ? (int) blockIdx.x : (int) blockIdx.y * across + (int) blockIdx.x;
+    if (MODE != kDense && index >= total) return;
     const int xcd = index & 7, each = total >> 3, more = total & 7;
     const int place_of = xcd * each + min(xcd, more) + (index >> 3);
     const int v = SPLIT ? place_of / a.splits : place_of, part = SPLIT ? place_of - v * a.splits : 0;
@@ -353,8 +355,8 @@ hipError_t launch(const ProductArgs &a, hipStream_t stream) {
     const int row_tiles = MODE == kDense ? a.row_tiles : (int) ((a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows);
     const int token_tiles = MODE == kDense ? (int) ((a.M + G::kTileTokens - 1) / G::kTileTokens) : a.most_tiles;
     const int64_t groups = (int64_t) row_tiles * token_tiles * (SPLIT ? a.splits : 1);
-    if (groups > 0x7FFFFFFF - kAcross) return hipErrorInvalidConfiguration;
-    const unsigned across = (unsigned) (groups < kAcross ? groups : kAcross);
+    if (groups > (MODE == kDense ? 0xFFFFFFFFll / G::kThreads : 0x7FFFFFFFll - kAcross)) return hipErrorInvalidConfiguration;
+    const unsigned across = (unsigned) (MODE == kDense || groups < kAcross ? groups : kAcross);
     static std::atomic<uint64_t> allowed{ 0 };   // devices on which the kernel may have its LDS
     const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_mx_tiled_kernel<MODE, RB, TB, WC, R, SPLIT>), G::kBytes, allowed);
     if (e != hipSuccess) return e;
