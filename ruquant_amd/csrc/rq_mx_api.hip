@@ -67,9 +67,9 @@ ExpertsPlan experts_plan(int64_t E, int64_t K, int64_t F, int64_t N, int64_t M, 
         return p;
     }
     // Tiles of 64 tokens up to 96 slots an expert; of 128 above, 256 rows of weights each where those are enough to keep the chip busy.
-    // (us for the whole call, 64 -> 128 tokens x 128 rows -> 128 x 256, by experts x slots an expert: 5120 x 1280 64 x 62: 210 -> 213 -> 226,
-    // 60 x 136: 295 -> 285 -> 258, 64 x 256: 479 -> 444 -> 403, 8 x 125: 50 -> 55 -> 64, 8 x 512: 134 -> 107 -> 120; 2048 x 512 60 x 136: 88 ->
-    // 83 -> 86, 64 x 256: 140 -> 128 -> 134)
+    // (us for the whole call, 64 -> 128 tokens x 128 rows -> 128 x 256, by experts x slots an expert: 5120 x 1280 64 x 62: 213 -> 216 -> 230,
+    // 64 x 125: 292 -> 295 -> 275, 64 x 256: 511 -> 491 -> 444, 8 x 125: 54 -> 59 -> 65, 8 x 512: 128 -> 107 -> 111; 2048 x 512 60 x 136: 84 ->
+    // 88 -> 80, 64 x 256: 146 -> 134 -> 131; 4096 x 4096 8 x 250: 130 -> 113 -> 126, 8 x 1000: 413 -> 340 -> 327. At worst 11 % behind the fastest.)
     const int64_t token_tiles = p.slots / 128 + ((p.slots < E ? p.slots : E) + 1) / 2;
     p.form = p.slots <= 96 * E ? kForm64 : tiled_row_tiles(kGateUp, kForm256, F) * token_tiles >= 768 ? kForm256 : kForm128;
     p.tile_tokens = tiled_tokens(p.form);

@@ -8,7 +8,8 @@
 //
 // Bound by the weights' stream where they are large, by the chain of a load, the rounding, the products and the join of the inputs' parts
 // where they are not: one token x 5120: 5120 outputs (14 MB) 6.3 us, 17408 outputs (47 MB) 11.5 us, 4.1 TB/s; three tokens x 17408 x 5120
-// 12.9 us behind a launch of 2.8 that rounds them. One token's 8 experts of 1280 x 5120: 14.7 + 9.0 us, 56 and 28 MB, 3.8 and 3.1 TB/s.
+// 12.9 us behind a launch of 2.8 that rounds them. One token's 8 experts of 1280 x 5120: 14.0 + 9.5 us, 56 and 28 MB, 4.0 and 2.9 TB/s;
+// with 8 of 64, 2, 3 and 4 tokens 38, 49 and 62 us.
 #include "rq_mx.h"
 
 namespace rq {

@@ -7,8 +7,8 @@
 // MFMAs: LDS delivers a fragment in 16 clocks (64 bytes each), in which the four SIMDs do one and a half MFMAs, so 4 x 2 blocks (12 reads in
 // 192 clocks, 16 MFMAs in 170) are bound by LDS and MFMA nearly alike, and registers end there (128 accumulators and two steps' fragments
 // of 256).
-// 2048 tokens x 17408 x 5120: 88 us for the 512 tiles of 256 x 256 that are two rounds of the chip, 3.9 PFLOP/s, the MFMAs busy for 48 % of the
-// cycles (a plain bf16 library product of 8192^3 here: 1.16), and 13.5 us for the rows behind them. 64 tokens x 17408 x 5120 is 12.2 us
+// 2048 tokens x 17408 x 5120: 85 us for the 512 tiles of 256 x 256 that are two rounds of the chip, 4.0 PFLOP/s, the MFMAs busy for 48 % of the
+// cycles (a plain bf16 library product of 8192^3 here: 1.16), and 12 us for the rows behind them. 64 tokens x 17408 x 5120 is 12.2 us
 // behind the quantiser's 3.2, 47 MB of weights at 3.9 TB/s.
 // Tried and dropped: 16x16x128 MFMAs (4.4 to 5.5 PFLOP/s in registers against 7.0 to 7.8); the weights' fragments from L1 in place of
 // LDS; deeper rings for the large forms.

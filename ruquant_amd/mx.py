@@ -5,8 +5,8 @@ MXFP4 (microscaled 4-bit floating point): 32 consecutive elements of a row share
 NaN. A tensor [.., K] is codes [.., K / 2] and scales [.., K / 32], both uint8.
 
 As in the rest of the package torch owns device memory and the stream, and every computation happens inside librq_w4a4.so, on the
-current stream of the inputs' device. With `out` and `workspace` given the calls allocate nothing, and all of them can be captured
-in a graph.
+current stream of the inputs' device. With `out` and `workspace` given the product and the experts allocate nothing; the other calls
+make their outputs. All of them can be captured in a graph.
 """
 import torch
 
