@@ -14,3 +14,6 @@ from .w4a4 import (  # noqa: F401
 from .mx import (  # noqa: F401
     MXWeight, mx_quantize, mx_dequantize, mx_mul_mat, route, expert_ffn, expert_workspace_bytes,
 )
+from .i8 import (  # noqa: F401
+    I8Weight, HalfWeight, i8_quantize, i8_dequantize, i8_mul_mat, sort_slots, grouped_mul_mat, grouped_workspace_bytes,
+)

@@ -1,0 +1,162 @@
+// Shared definitions of the int8 products and of the products grouped by expert: layouts, matrix instructions, launch arguments.
+#pragma once
+
+#include "../../include/rq_i8.h"
+#include "rq_mx.h"
+
+namespace rq {
+namespace prod {
+
+using mx::allow_lds;
+using mx::Element;
+using mx::from_float;
+using mx::store_out;
+using mx::to_float;
+using mx::up_to;
+using mx::v16f;
+using mx::v4f;
+using mx::v4i;
+typedef int    v16i __attribute__((ext_vector_type(16)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+inline int type_bytes(int type) { return type == RQ_F32 ? 4 : type == RQ_I8 ? 1 : 2; }
+
+// ---------------------------------------------------------------------------------------------------
+// All three types are fed to the matrix cores in 16 bytes a lane: a 32x32x32 (int8) or 32x32x16 (16 bits) MFMA takes from lane l of
+// either operand row l % 32 and bytes 16 (l / 32) .. + 15 of a run of 32 bytes of the row. Lane l holds of the 32 x 32 result column l % 32
+// and rows 8 (i / 4) + 4 (l / 32) + i % 4, i = 0 .. 15. The 16x16 forms take row l % 16 and bytes 16 (l / 16) of a run of 64; lane l holds column
+// l % 16 and rows 4 (l / 16) + i. (Which element of a run a byte stands for is the same for both operands, so it does not matter.)
+//
+// Prepared weight, per expert: N / 32 row blocks x steps of 64 bytes x 2 runs x 64 lanes x 16 bytes (rows and bytes padded with zeros), so a
+// wavefront reads a fragment as 1 KiB of consecutive bytes; behind them, of int8, a scale for each row of the blocks.
+// Activations stay rows, `pitch` bytes apart and on multiples of 16: what gathers them costs nothing then.
+// ---------------------------------------------------------------------------------------------------
+struct Panels {
+    int64_t N, row_bytes;                // rows; bytes of a row that count
+    int     row_blocks, steps;
+    int64_t code_bytes, expert_bytes;    // of one expert
+};
+inline Panels panels(int type, int64_t N, int64_t K) {
+    Panels L;
+    L.N = N;
+    L.row_bytes = K * type_bytes(type);
+    L.row_blocks = (int) (up_to(N, 32) / 32);
+    L.steps = (int) (up_to(L.row_bytes, 64) / 64);
+    L.code_bytes = (int64_t) L.row_blocks * L.steps * 2048;
+    L.expert_bytes = L.code_bytes + (type == RQ_I8 ? up_to((int64_t) L.row_blocks * 128, 256) : 0);
+    return L;
+}
+
+template <int WT> struct Matrix;
+template <> struct Matrix<RQ_I8> {
+    using Acc = v16i;
+    using Acc4 = v4i;
+    static __device__ __forceinline__ Acc mfma(const v4i &a, const v4i &b, const Acc &c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc4 mfma16(const v4i &a, const v4i &b, const Acc4 &c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+};
+template <> struct Matrix<RQ_BF16> {
+    using Acc = v16f;
+    using Acc4 = v4f;
+    static __device__ __forceinline__ Acc mfma(const v4i &a, const v4i &b, const Acc &c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Acc4 mfma16(const v4i &a, const v4i &b, const Acc4 &c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    }
+};
+template <> struct Matrix<RQ_F16> {
+    using Acc = v16f;
+    using Acc4 = v4f;
+    static __device__ __forceinline__ Acc mfma(const v4i &a, const v4i &b, const Acc &c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Acc4 mfma16(const v4i &a, const v4i &b, const Acc4 &c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+};
+
+struct ProductArgs {
+    Panels         L;
+    const uint8_t *w;              // prepared
+    const uint8_t *x;              // rows of x, on multiples of 16 bytes
+    int64_t        pitch, x_bytes; // of a row: distance, and how many there are to read (a multiple of 16; zeros behind them)
+    const float   *x_scales;       // of int8 rows
+    int64_t        M;              // rows of x
+    int64_t        P;              // positions
+    const int32_t *offsets;        // null: one group of all positions
+    int            E;
+    const int32_t *rows, *out_rows;
+    int            out_dtype;
+    void          *y;
+    int64_t        ldy, y_rows;
+};
+
+// The rows that position p reads and writes; -1: none.
+__device__ __forceinline__ int64_t row_read(const ProductArgs &a, int64_t p) {
+    if (!a.rows) return p < a.M ? p : -1;
+    const int64_t r = a.rows[p];
+    return r >= 0 && r < a.M ? r : -1;
+}
+__device__ __forceinline__ int64_t row_written(const ProductArgs &a, int64_t p) {
+    if (!a.out_rows) return p < a.y_rows ? p : -1;
+    const int64_t r = a.out_rows[p];
+    return r >= 0 && r < a.y_rows ? r : -1;
+}
+// Group e's first position and how many it has.
+__device__ __forceinline__ void group(const ProductArgs &a, int e, int &first, int &count) {
+    const int P = (int) a.P;
+    first = min(max(a.offsets[e], 0), P);
+    count = max(min(a.offsets[e + 1], P) - first, 0);
+}
+// Of the groups, which one has the unit `want` (a uniform number) if group e has units(its count) of them, and the place in it; all lanes
+// of a wavefront take part. Returns false (group and place left) if there are fewer. total: all units.
+template <typename F>
+__device__ __forceinline__ bool find_group(const ProductArgs &a, int want, F units, int &e_, int &first_, int &count_, int &place_, int &total_) {
+    const int lane = threadIdx.x & 63;
+    int       before = 0;
+    bool      found = false;
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+        int first = 0, count = 0;
+        if (e0 + lane < a.E) group(a, e0 + lane, first, count);
+        const int mine = units(count);
+        int       sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(sum, o);
+            if (lane >= o) sum += u;
+        }
+        const int      from = before + sum - mine;
+        const uint64_t here = __ballot(want >= from && want < from + mine);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            e_ = e0 + l;
+            first_ = __builtin_amdgcn_readlane(first, l);
+            count_ = __builtin_amdgcn_readlane(count, l);
+            place_ = want - __builtin_amdgcn_readlane(from, l);
+            found = true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    total_ = before;
+    return found;
+}
+
+// ---- launches ---------------------------------------------------------------------------------------
+// x -> codes in rows of `pitch` bytes, the places behind K zeros up to `padded` of them, and scales
+hipError_t launch_i8_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded,
+                              float *scales, hipStream_t stream);
+// rows of row_bytes bytes (distance ld_bytes) -> rows of `pitch` bytes, zeros behind them
+hipError_t launch_pack(const void *x, int64_t ld_bytes, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch, hipStream_t stream);
+
+// few rows a group: weights from memory into registers
+hipError_t launch_stream(int weight_type, const ProductArgs &a, hipStream_t stream);
+
+// more: both operands through LDS, in tiles of several forms
+constexpr int kForms = 4;   // 64 x 64, 128 x 64, 128 x 128, 256 x 256 rows x positions
+hipError_t launch_tiled(int weight_type, int form, const ProductArgs &a, hipStream_t stream);
+int        tiled_rows(int form);
+int        tiled_tokens(int form);
+
+}  // namespace prod
+}  // namespace rq

@@ -100,6 +100,18 @@ PROTOTYPES.update({
     # include/rq_mx4_plan.h
     "rq_mx4_product_plan": (_int, [_i64, _i64, _i64, _ptr]),
     "rq_mx4_experts_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _int, _ptr]),
+    # include/rq_i8.h
+    "rq_i8_quantize": (_int, [_int, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr]),
+    "rq_i8_dequantize": (_int, [_int, _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr]),
+    "rq_weight_prepared_bytes": (_size, [_int, _i64, _i64, _i64]),
+    "rq_weight_prepare": (_int, [_int, _ptr, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr]),
+    "rq_i8_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "rq_i8_mul_mat": (_int, [_ptr, _i64, _i64, _int, _ptr, _i64, _ptr, _i64, _int, _ptr, _i64, _ptr, _size, _ptr]),
+    "rq_sort_workspace_bytes": (_size, [_i64, _int, _i64]),
+    "rq_sort_slots": (_int, [_ptr, _i64, _int, _i64, _ptr, _ptr, _ptr, _ptr, _size, _ptr]),
+    "rq_grouped_workspace_bytes": (_size, [_int, _i64, _i64, _i64, _i64, _i64]),
+    "rq_grouped_mul_mat": (_int, [_int, _ptr, _i64, _i64, _i64, _int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _int, _ptr, _i64,
+                                  _i64, _ptr, _size, _ptr]),
 })
 
 for _name in ("rq_w4a4_mul_mat", "rq_w4a4_mul_mat_fused"):
