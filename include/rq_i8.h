@@ -5,8 +5,9 @@
  * it, allocate nothing, synchronize nothing and can be captured in a graph. Return values: 0 = success; > 0 = a hipError_t;
  * < 0 = one of the RQ_E_* codes of rq_w4a4.h; nothing is launched then. These operators have no counterpart in the reference.
  *
- * int8 rows: a row of K numbers is K codes and one fp32 scale s; a code c stands for c s. Rounding a row x: s = max |x| / 127, at least
- * 2^-126, in fp32; r = 1 / s in fp32; code = the whole number nearest to x r (the exact product), ties to even, so -127 .. 127.
+ * int8 rows: a row of K numbers is K codes and one fp32 scale s; a code c stands for c s. Rounding a row x: s = max |x| times the
+ * fp32 number nearest to 1 / 127, in fp32, at least 2^-126; r = 1 / s in fp32; code = the whole number nearest to x r (the exact product), ties to
+ * even, so -127 .. 127.
  * A row that holds an infinity or a NaN has a NaN scale and zero codes. Tensors hold codes row by row and scales by row.
  */
 #ifndef RQ_I8_H

@@ -1,7 +1,6 @@
 // int8 quantiser and dequantiser, the rewriting of weights, and rows brought to multiples of 16 bytes.
 //
-// A code is the nearest whole number of x r: fma(x, r, 1.5 x 2^23) rounds the exact product once, to the nearest whole number, ties to
-// even, and leaves it in the low bits; |x r| is at most 127 (1 + 2^-22). All of these are bound by memory.
+// All of these are bound by memory.
 #include "rq_prod.h"
 
 namespace rq {
@@ -36,25 +35,13 @@ __device__ __forceinline__ uint32_t top_bits(const float (&v)[8], uint32_t top) 
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
     return top;
 }
-// the codes of eight elements, those in `keep`
-__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float r, uint32_t keep) {
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(v[4 * h + i], r, 12582912.0f));
-        const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000C0Cu);
-        w[h] = (lo | hi) & keep;
-    }
-    return make_uint2(w[0], w[1]);
-}
-
 // A row a workgroup of G threads, or 256 / G rows where G < 256. VEC: rows of x on multiples of 16 bytes, K a multiple of 8. PITCH: codes go to rows of `pitch`
 // bytes, on multiples of eight, with zeros up to `padded`; else to rows of K bytes in a row.
 template <int DT, bool VEC, int G>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void rq_i8_quantize_kernel(const typename Element<DT>::type *x, int64_t ldx, int64_t M, int64_t K,
-                                                                           uint8_t *codes, int64_t pitch, int64_t padded, float *scales) {
+                                                                           uint8_t *codes, int64_t pitch, int64_t padded, float *scales, int *zero, int zeros) {
+    if (zeros && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < zeros; i += (int) blockDim.x) zero[i] = 0;
     constexpr int kRows = G < 256 ? 256 / G : 1;
     const int     t = threadIdx.x % G, lane = threadIdx.x & 63;
     const int64_t m = (int64_t) blockIdx.x * kRows + threadIdx.x / G;
@@ -77,8 +64,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rq_i8_quantize_kernel(const
             top = top_bits(w, top);
         }
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) top = max(top, (uint32_t) __shfl_xor((int) top, o));
+    top = wave_max(top);
     if constexpr (G > 64) {
         __shared__ uint32_t tops[G / 64];
         if (lane == 0) tops[threadIdx.x >> 6] = top;
@@ -87,16 +73,11 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rq_i8_quantize_kernel(const
         for (int i = 0; i < G / 64; ++i) top = max(top, tops[i]);
     }
     if (!there) return;
-    const float largest = __uint_as_float(top);
-    float       s = largest / 127.0f;
-    s = s > 0x1p-126f ? s : 0x1p-126f;
-    const float r = 1.0f / s;
-    const bool finite = top < 0x7F800000u;
-    if (!finite) s = __uint_as_float(0x7FC00000u);
-    if (t == 0) scales[m] = s;
+    const RowScale q(top);
+    if (t == 0) scales[m] = q.s;
     uint8_t *to = codes + m * pitch;
     auto     put = [&](int64_t k, const float(&w)[8]) __attribute__((always_inline)) {
-        const uint2 c = codes_of(w, r, finite ? ~0u : 0u);
+        const uint2 c = codes_of(w, q.r, q.keep);
         if (VEC || k + 8 <= padded) {
             // (rows of K bytes are on multiples of eight where VEC is set, and padded rows always)
             *reinterpret_cast<uint2 *>(to + k) = c;
@@ -180,7 +161,9 @@ __global__ __launch_bounds__(256) void rq_weight_prepare_kernel(const uint8_t *w
 }
 
 // 16 bytes a thread
-__global__ __launch_bounds__(256) void rq_pack_kernel(const uint8_t *x, int64_t ld, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch) {
+__global__ __launch_bounds__(256) void rq_pack_kernel(const uint8_t *x, int64_t ld, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch, int *zero, int zeros) {
+    if (zeros && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < zeros; i += 256) zero[i] = 0;
     const int64_t per_row = pitch / 16, n = (int64_t) blockIdx.x * 256 + threadIdx.x;
     const int64_t m = n / per_row, b = (n - m * per_row) * 16;
     if (m >= M) return;
@@ -196,14 +179,14 @@ constexpr int64_t kGrid = 1ll << 23;   // workgroups of a launch (of up to 512 t
 
 template <int DT, bool VEC, int G>
 hipError_t quantize_rows(const void *x_, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded, float *scales,
-                         hipStream_t stream) {
+                         int *zero, int zeros, hipStream_t stream) {
     constexpr int kRows = G < 256 ? 256 / G : 1;
     constexpr int64_t kMost = kGrid / 2 * kRows;
     const auto   *x = reinterpret_cast<const typename Element<DT>::type *>(x_);
     for (int64_t m = 0; m < M; m += kMost) {
         const int64_t rows = M - m < kMost ? M - m : kMost;
         hipLaunchKernelGGL((rq_i8_quantize_kernel<DT, VEC, G>), dim3((unsigned) ((rows + kRows - 1) / kRows)), dim3(G < 256 ? 256 : G), 0, stream,
-                           x + m * ldx, ldx, rows, K, codes + m * pitch, pitch, padded, scales + m);
+                           x + m * ldx, ldx, rows, K, codes + m * pitch, pitch, padded, scales + m, zero, m ? 0 : zeros);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -211,15 +194,15 @@ hipError_t quantize_rows(const void *x_, int64_t ldx, int64_t M, int64_t K, uint
 }
 template <int DT>
 hipError_t quantize(const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded, float *scales,
-                    hipStream_t stream) {
+                    int *zero, int zeros, hipStream_t stream) {
     const int  size = DT == RQ_F32 ? 4 : 2;
     const bool vec = (uintptr_t) x % 16 == 0 && (M == 1 || ldx * size % 16 == 0) && K % 8 == 0 && (uintptr_t) codes % 8 == 0;
-    if (K <= 2048) return vec ? quantize_rows<DT, true, 64>(x, ldx, M, K, codes, pitch, padded, scales, stream)
-                              : quantize_rows<DT, false, 64>(x, ldx, M, K, codes, pitch, padded, scales, stream);
-    if (K <= 8192) return vec ? quantize_rows<DT, true, 256>(x, ldx, M, K, codes, pitch, padded, scales, stream)
-                              : quantize_rows<DT, false, 256>(x, ldx, M, K, codes, pitch, padded, scales, stream);
-    return vec ? quantize_rows<DT, true, 512>(x, ldx, M, K, codes, pitch, padded, scales, stream)
-               : quantize_rows<DT, false, 512>(x, ldx, M, K, codes, pitch, padded, scales, stream);
+    if (K <= 2048) return vec ? quantize_rows<DT, true, 64>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
+                              : quantize_rows<DT, false, 64>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    if (K <= 8192) return vec ? quantize_rows<DT, true, 256>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
+                              : quantize_rows<DT, false, 256>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    return vec ? quantize_rows<DT, true, 512>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
+               : quantize_rows<DT, false, 512>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
 }
 
 template <int DT>
@@ -243,18 +226,18 @@ hipError_t dequantize(const void *codes_, const float *scales, int64_t M, int64_
 }  // namespace
 
 hipError_t launch_i8_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded,
-                              float *scales, hipStream_t stream) {
-    if (dtype == RQ_F32) return quantize<RQ_F32>(x, ldx, M, K, codes, pitch, padded, scales, stream);
-    if (dtype == RQ_F16) return quantize<RQ_F16>(x, ldx, M, K, codes, pitch, padded, scales, stream);
-    return quantize<RQ_BF16>(x, ldx, M, K, codes, pitch, padded, scales, stream);
+                              float *scales, int *zero, int zeros, hipStream_t stream) {
+    if (dtype == RQ_F32) return quantize<RQ_F32>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    if (dtype == RQ_F16) return quantize<RQ_F16>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    return quantize<RQ_BF16>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
 }
 
-hipError_t launch_pack(const void *x, int64_t ld_bytes, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch, hipStream_t stream) {
+hipError_t launch_pack(const void *x, int64_t ld_bytes, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch, int *zero, int zeros, hipStream_t stream) {
     const int64_t per_row = pitch / 16, most = kGrid * 256 / per_row;   // (pitch up to 2^18)
-    for (int64_t m = 0; m < M; m += most) {
+    for (int64_t m = 0; m < M || m == 0; m += most) {
         const int64_t rows = M - m < most ? M - m : most;
-        hipLaunchKernelGGL(rq_pack_kernel, dim3((unsigned) ((rows * per_row + 255) / 256)), dim3(256), 0, stream,
-                           (const uint8_t *) x + m * ld_bytes, ld_bytes, rows, row_bytes, to + m * pitch, pitch);
+        hipLaunchKernelGGL(rq_pack_kernel, dim3((unsigned) ((rows * per_row + 255) / 256 + (rows == 0))), dim3(256), 0, stream,
+                           (const uint8_t *) x + m * ld_bytes, ld_bytes, rows, row_bytes, to + m * pitch, pitch, zero, m ? 0 : zeros);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -276,7 +259,7 @@ extern "C" int rq_i8_quantize(int dtype, const void *x, int64_t ldx, int64_t M, 
     if (!float_dtype(dtype) || K < 1 || K > kMostK || M < 0) return RQ_E_UNSUPPORTED;
     if (M == 0) return 0;
     if (!x || !aligned_to(x, type_bytes(dtype)) || !codes || !scales || !aligned_to(scales, 4) || (M > 1 && ldx < K)) return RQ_E_ARGUMENT;
-    return launch_i8_quantize(dtype, x, ldx, M, K, (uint8_t *) codes, K, 0, scales, (hipStream_t) stream);
+    return launch_i8_quantize(dtype, x, ldx, M, K, (uint8_t *) codes, K, 0, scales, nullptr, 0, (hipStream_t) stream);
 }
 
 extern "C" int rq_i8_dequantize(int dtype, const void *codes, const float *scales, int64_t M, int64_t K, void *out, int64_t ldo,

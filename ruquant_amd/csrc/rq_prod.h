@@ -81,6 +81,9 @@ struct ProductArgs {
     const uint8_t *w;              // prepared
     const uint8_t *x;              // rows of x, on multiples of 16 bytes
     int64_t        pitch, x_bytes; // of a row: distance, and how many there are to read (a multiple of 16; zeros behind them)
+    int64_t        K;              // launch_stream where it rounds: x is the call's own, `pitch` its row stride in elements, rows of K;
+    bool           aligned;        //   whether they are on multiples of 16 bytes, and K of eight;
+    int            chunk;          //   up to so many rows at a time (16 where it does not round)
     const float   *x_scales;       // of int8 rows
     int64_t        M;              // rows of x
     int64_t        P;              // positions
@@ -90,6 +93,10 @@ struct ProductArgs {
     int            out_dtype;
     void          *y;
     int64_t        ldy, y_rows;
+    int            first_block, row_tiles;   // tiles: the row blocks of this launch start here, and how many tiles they make (0: all)
+    int            splits, split_steps;      //   workgroups that share a tile, and the steps of 64 bytes of each (even)
+    uint32_t      *sums;                     //   splits > 1: what they leave
+    int           *arrived;                  //   and how many have, by wavefront's outputs: zero before the launch
 };
 
 // The rows that position p reads and writes; -1: none.
@@ -142,21 +149,59 @@ __device__ __forceinline__ bool find_group(const ProductArgs &a, int want, F uni
     return found;
 }
 
-// ---- launches ---------------------------------------------------------------------------------------
-// x -> codes in rows of `pitch` bytes, the places behind K zeros up to `padded` of them, and scales
-hipError_t launch_i8_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded,
-                              float *scales, hipStream_t stream);
-// rows of row_bytes bytes (distance ld_bytes) -> rows of `pitch` bytes, zeros behind them
-hipError_t launch_pack(const void *x, int64_t ld_bytes, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch, hipStream_t stream);
+// ---- rounding of a row to int8 ------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t) __shfl_xor((int) v, o));
+    return v;
+}
+// From the bits of a row's largest magnitude: its scale, what the elements are multiplied by, and the codes' bits that count (none where the row holds
+// an infinity or a NaN).
+struct RowScale {
+    float    s, r;
+    uint32_t keep;
+    __device__ __forceinline__ RowScale(uint32_t top) {
+        s = __uint_as_float(top) * (1.0f / 127.0f);
+        s = s > 0x1p-126f ? s : 0x1p-126f;
+        r = 1.0f / s;
+        keep = top < 0x7F800000u ? ~0u : 0u;
+        if (!keep) s = __uint_as_float(0x7FC00000u);
+    }
+};
+// The codes of eight elements. A code is the nearest whole number of x r: fma(x, r, 1.5 x 2^23) rounds the exact product once, to the nearest whole
+// number, ties to even, and leaves it in the low bits; |x r| is at most 127 (1 + 2^-22).
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float r, uint32_t keep) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(v[4 * h + i], r, 12582912.0f));
+        const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000C0Cu);
+        w[h] = (lo | hi) & keep;
+    }
+    return make_uint2(w[0], w[1]);
+}
 
-// few rows a group: weights from memory into registers
-hipError_t launch_stream(int weight_type, const ProductArgs &a, hipStream_t stream);
+// ---- launches ---------------------------------------------------------------------------------------
+// x -> codes in rows of `pitch` bytes, the places behind K zeros up to `padded` of them, and scales. Sets zero[0 .. zeros - 1] to 0.
+hipError_t launch_i8_quantize(int dtype, const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded,
+                              float *scales, int *zero, int zeros, hipStream_t stream);
+// rows of row_bytes bytes (distance ld_bytes) -> rows of `pitch` bytes, zeros behind them. Sets zero[0 .. zeros - 1] to 0, also where M is 0.
+hipError_t launch_pack(const void *x, int64_t ld_bytes, int64_t M, int64_t row_bytes, uint8_t *to, int64_t pitch, int *zero, int zeros, hipStream_t stream);
+
+// Few rows a group: weights from memory into registers. x_type: the type of the rows of x where it rounds them, else RQ_I8.
+hipError_t launch_stream(int weight_type, int x_type, const ProductArgs &a, hipStream_t stream);
+// How many rows at a time launch_stream rounds itself, of P in E groups (0: one); 0 where a launch in front is faster, or they do not fit.
+int stream_rounds(int64_t P, int64_t K, int64_t N, int64_t E);
 
 // more: both operands through LDS, in tiles of several forms
-constexpr int kForms = 4;   // 64 x 64, 128 x 64, 128 x 128, 256 x 256 rows x positions
+constexpr int kForms = 5;   // 64 x 64, 128 x 64, 128 x 128 (two a compute unit), 128 x 128 (one), 256 x 256 rows x positions
 hipError_t launch_tiled(int weight_type, int form, const ProductArgs &a, hipStream_t stream);
 int        tiled_rows(int form);
 int        tiled_tokens(int form);
+// tiles of T positions: of P in one group (E = 0), or at most, of P in E groups
+inline int64_t most_token_tiles(int T, int64_t P, int64_t E) { return E == 0 ? (P + T - 1) / T : P / T + (P < E ? P : E); }
 
 }  // namespace prod
 }  // namespace rq

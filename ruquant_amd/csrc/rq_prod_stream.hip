@@ -1,8 +1,9 @@
 // Products of few rows a group (int8, or grouped by expert): weights from memory into registers.
 //
-// A call of this size is the stream of its weights. A workgroup has 32 rows of one weight (or 16, where those are too few for the chip) and
-// up to 16 rows of x at a time; its wavefronts split the row's bytes, each with DEPTH steps of 64 bytes on their way, and join their sums in LDS in
-// their order.
+// A call of this size is the stream of its weights. A workgroup has 32 rows of one weight (or 16) and up to 16 rows of x at a time; its wavefronts
+// split the row's bytes, each with DEPTH steps of 64 bytes on their way, and join their sums in LDS in their order. Rows of x that are still to be
+// rounded are rounded by every workgroup for itself, into LDS, while its first weights are on their way: a launch in front costs more from some hundred
+// workgroups down to few rows.
 #include "rq_prod.h"
 
 namespace rq {
@@ -11,11 +12,39 @@ namespace {
 
 __device__ __attribute__((aligned(16))) const uint8_t kZeros[16] = { 0 };
 
-// WT: the weight's type; W wavefronts; NR runs of 16 rows of the weight; GROUPED: blockIdx.y is a group that has rows.
-template <int WT, int W, int NR, int DEPTH, bool GROUPED>
+// Eight elements of a row from k on, zeros behind its end.
+template <int DT>
+__device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, bool aligned, int K, int k, float (&v)[8]) {
+    using T = typename Element<DT>::type;
+    if (aligned) {   // (on 16 bytes, and K a multiple of eight)
+        if constexpr (DT == RQ_F32) {
+            const float4 a = reinterpret_cast<const float4 *>(x + k)[0], b = reinterpret_cast<const float4 *>(x + k)[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4    u = *reinterpret_cast<const uint4 *>(x + k);
+            const uint32_t w[4] = { u.x, u.y, u.z, u.w };
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = to_float(__builtin_bit_cast(T, (uint16_t) w[i]));
+                v[2 * i + 1] = to_float(__builtin_bit_cast(T, (uint16_t) (w[i] >> 16)));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_float(x[k + i]) : 0.0f;
+    }
+}
+
+// WT: the weight's type; DT: RQ_F32, RQ_F16, RQ_BF16: rows of x of that type, to be rounded to int8; RQ_I8: rows as the products take them. W wavefronts; NR
+// runs of 16 rows of the weight; GROUPED: blockIdx.y is a group that has rows.
+template <int WT, int DT, int W, int NR, int DEPTH, bool GROUPED>
 __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) {
     using Acc4 = typename Matrix<WT>::Acc4;
-    __shared__ Acc4 part[W][NR][16][4];   // [wavefront][run of rows][row of x][block of four rows]
+    constexpr bool kRound = DT != RQ_I8;
+    constexpr int  kKept = 3, kThreads = 64 * W;   // units of a row that a thread keeps while its maximum is found
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ uint32_t tops[2][W];
+    __shared__ float    scale_of[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
     int       e = 0, first = 0, count = (int) a.P;
     if constexpr (GROUPED) {
@@ -33,48 +62,122 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
         from[r] = weight + (int64_t) (unit >> 1) * steps * 2048 + (unit & 1) * 256 + (quarter >> 1) * 1024 + (quarter & 1) * 512 + col * 16;
     }
     const float *t_scales = reinterpret_cast<const float *>(weight + a.L.code_bytes);
-    for (int t0 = 0; t0 < count; t0 += 16) {
-        const int      T = min(16, count - t0);
-        const int64_t  row = row_read(a, first + t0 + min(col, T - 1));   // (columns past the rows repeat the last one)
-        const uint8_t *x = a.x + (row < 0 ? 0 : row) * a.pitch + quarter * 16;
-        v4i            A[DEPTH][NR], B[DEPTH];
-        Acc4           acc[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) acc[r] = Acc4{ 0, 0, 0, 0 };
+    const int    pitch = steps * 64 + 16;   // (of rows in LDS: the same bytes of 16 rows in 16 places of the banks)
+    for (int t0 = 0; t0 < count; t0 += a.chunk) {
+        const int T = min(a.chunk, count - t0);
+        v4i       A[DEPTH][NR], B[kRound ? 1 : DEPTH];
+        Acc4      acc[NR];
+        const uint8_t *x = lds + min(col, T - 1) * pitch + quarter * 16;   // (columns past the rows repeat the last one)
+        if constexpr (!kRound) {
+            const int64_t row = row_read(a, first + t0 + min(col, T - 1));
+            x = a.x + (row < 0 ? 0 : row) * a.pitch + quarter * 16;
+        }
         auto load = [&](int i, int s) __attribute__((always_inline)) {
 #pragma unroll
             for (int r = 0; r < NR; ++r) A[i][r] = *reinterpret_cast<const v4i *>(from[r] + (int64_t) s * 2048);
-            B[i] = *reinterpret_cast<const v4i *>(s * 64 + quarter * 16 < a.x_bytes ? x + s * 64 : kZeros);
+            if constexpr (!kRound) B[i] = *reinterpret_cast<const v4i *>(s * 64 + quarter * 16 < a.x_bytes ? x + s * 64 : kZeros);
         };
+        if constexpr (kRound) {
+            using X = typename Element<DT>::type;
+            const int K = (int) a.K, units = steps * 8;
+            float     v[kKept][8];
+            auto      row_at = [&](int t) __attribute__((always_inline)) { return row_read(a, first + t0 + t); };
+            auto      begin = [&](int64_t row) __attribute__((always_inline)) {
+                const X *p = reinterpret_cast<const X *>(a.x) + (row < 0 ? 0 : row) * a.pitch;
 #pragma unroll
-        for (int i = 0; i < DEPTH; ++i)
-            if (s0 + i < s1) load(i, s0 + i);
+                for (int i = 0; i < kKept; ++i) {
+                    const int k = ((int) threadIdx.x + i * kThreads) * 8;
+                    if (k < K) load_unit<DT>(p, a.aligned, K, k, v[i]);
+                }
+                return p;
+            };
+            int64_t  row = row_at(0);
+            const X *p = begin(row);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < DEPTH; ++i)
+                if (s0 + i < s1) load(i, s0 + i);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t0) __syncthreads();   // (the sums of the rows before, in the rows' place, are not read any more)
+            for (int t = 0; t < T; ++t) {
+                if (t) row = row_at(t), p = begin(row);
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < kKept; ++i) {
+                    const int k = ((int) threadIdx.x + i * kThreads) * 8;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (k < K) top = max(top, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+                }
+                for (int u = threadIdx.x + kKept * kThreads; u * 8 < K; u += kThreads) {
+                    float w[8];
+                    load_unit<DT>(p, a.aligned, K, u * 8, w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(w[j]) & 0x7FFFFFFFu);
+                }
+                top = wave_max(top);
+                if (lane == 0) tops[t & 1][wave] = top;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < W; ++i) top = max(top, tops[t & 1][i]);
+                const RowScale q(top);
+                if (threadIdx.x == 0) scale_of[t] = row < 0 ? 0.0f : q.s;
+                const uint32_t keep = row < 0 ? 0u : q.keep;
+                uint8_t       *to = lds + t * pitch;
+#pragma unroll
+                for (int i = 0; i < kKept; ++i) {
+                    const int u = threadIdx.x + i * kThreads;
+                    if (u * 8 < K) *reinterpret_cast<uint2 *>(to + u * 8) = codes_of(v[i], q.r, keep);
+                }
+                for (int u = threadIdx.x + kKept * kThreads; u < units; u += kThreads) {
+                    float w[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
+                    if (u * 8 < K) load_unit<DT>(p, a.aligned, K, u * 8, w);
+                    *reinterpret_cast<uint2 *>(to + u * 8) = codes_of(w, q.r, keep);
+                }
+#pragma unroll
+                for (int i = 0; i < kKept; ++i) {   // (the places behind the row)
+                    const int u = threadIdx.x + i * kThreads;
+                    if (u * 8 >= K && u < units) *reinterpret_cast<uint2 *>(to + u * 8) = make_uint2(0, 0);
+                }
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int i = 0; i < DEPTH; ++i)
+                if (s0 + i < s1) load(i, s0 + i);
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[r] = Acc4{ 0, 0, 0, 0 };
         for (int s = s0; s < s1; s += DEPTH) {
 #pragma unroll
             for (int i = 0; i < DEPTH; ++i) {
                 if (s + i < s1) {
+                    const v4i b = kRound ? *reinterpret_cast<const v4i *>(x + (s + i) * 64) : B[kRound ? 0 : i];
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) acc[r] = Matrix<WT>::mfma16(A[i][r], B[i], acc[r]);
+                    for (int r = 0; r < NR; ++r) acc[r] = Matrix<WT>::mfma16(A[i][r], b, acc[r]);
                     if (s + i + DEPTH < s1) load(i, s + i + DEPTH);
                 }
             }
         }
-        if (t0) __syncthreads();   // (the sums of the rows before are not read any more)
+        // [wavefront][run of rows][row of x][block of four rows], in the place of the rows
+        Acc4 *part = reinterpret_cast<Acc4 *>(lds);
+        if (kRound || t0) __syncthreads();   // (neither they nor the sums before are read any more)
 #pragma unroll
         for (int r = 0; r < NR; ++r)
-            if (col < T) part[wave][r][col][quarter] = acc[r];
+            if (col < T) part[((wave * NR + r) * T + col) * 4 + quarter] = acc[r];
         __syncthreads();
-        for (int c = threadIdx.x; c < NR * T * 4; c += 64 * W) {
+        const int cells = NR * T * 4;
+        for (int c = threadIdx.x; c < cells; c += kThreads) {
             const int r = c / (T * 4), t = (c >> 2) % T, block = c & 3;
-            Acc4      sum = part[0][r][t][block];
+            Acc4      sum = part[c];
 #pragma unroll
-            for (int w = 1; w < W; ++w) sum += part[w][r][t][block];
-            const int64_t p = first + t0 + t, n = (int64_t) (unit0 + r) * 16 + block * 4, out = row_written(a, p), in = row_read(a, p);
+            for (int w = 1; w < W; ++w) sum += part[w * cells + c];
+            const int64_t place = first + t0 + t, n = (int64_t) (unit0 + r) * 16 + block * 4, out = row_written(a, place), in = row_read(a, place);
             if (out < 0 || n >= a.L.N) continue;
             v4f v;
             if constexpr (WT == RQ_I8) {
                 const v4f   tn = *reinterpret_cast<const v4f *>(t_scales + n);
-                const float sm = in < 0 ? 0.0f : a.x_scales[in];
+                const float sm = kRound ? scale_of[t] : in < 0 ? 0.0f : a.x_scales[in];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = (float) sum[i] * tn[i] * sm;
             } else {
@@ -86,28 +189,46 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
     }
 }
 
-template <int WT, bool GROUPED>
+constexpr int kMostLds = 65536;
+int           lds_bytes(int W, int NR, bool round, const ProductArgs &a) {
+    const int T = (int) (a.P < a.chunk ? a.P : a.chunk), sums = W * NR * T * 64, rows = round ? T * (a.L.steps * 64 + 16) : 0;
+    return sums > rows ? sums : rows;
+}
+
+template <int WT, int DT, bool GROUPED>
 hipError_t stream(const ProductArgs &a, hipStream_t s) {
     const int64_t  units = (a.L.N + 15) / 16;
     const unsigned groups = GROUPED ? (unsigned) (a.P < a.E ? a.P : a.E) : 1;
-    if (units * groups > 1024) {
-        hipLaunchKernelGGL((rq_stream_kernel<WT, 8, 2, 4, GROUPED>), dim3((unsigned) ((units + 1) / 2), groups), dim3(512), 0, s, a);
+    constexpr bool kRound = DT != RQ_I8;
+    if (units * groups > 768) {
+        hipLaunchKernelGGL((rq_stream_kernel<WT, DT, 4, 2, 4, GROUPED>), dim3((unsigned) ((units + 1) / 2), groups), dim3(256), lds_bytes(4, 2, kRound, a), s, a);
     } else {
-        hipLaunchKernelGGL((rq_stream_kernel<WT, 8, 1, 8, GROUPED>), dim3((unsigned) units, groups), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((rq_stream_kernel<WT, DT, 8, 2, 6, GROUPED>), dim3((unsigned) ((units + 1) / 2), groups), dim3(512), lds_bytes(8, 2, kRound, a), s, a);
     }
     return hipGetLastError();
 }
 template <bool GROUPED>
-hipError_t stream(int weight_type, const ProductArgs &a, hipStream_t s) {
-    if (weight_type == RQ_I8) return stream<RQ_I8, GROUPED>(a, s);
-    if (weight_type == RQ_F16) return stream<RQ_F16, GROUPED>(a, s);
-    return stream<RQ_BF16, GROUPED>(a, s);
+hipError_t stream(int weight_type, int x_type, const ProductArgs &a, hipStream_t s) {
+    if (weight_type == RQ_F16) return stream<RQ_F16, RQ_I8, GROUPED>(a, s);
+    if (weight_type == RQ_BF16) return stream<RQ_BF16, RQ_I8, GROUPED>(a, s);
+    if (x_type == RQ_F32) return stream<RQ_I8, RQ_F32, GROUPED>(a, s);
+    if (x_type == RQ_F16) return stream<RQ_I8, RQ_F16, GROUPED>(a, s);
+    if (x_type == RQ_BF16) return stream<RQ_I8, RQ_BF16, GROUPED>(a, s);
+    return stream<RQ_I8, RQ_I8, GROUPED>(a, s);
 }
 
 }  // namespace
 
-hipError_t launch_stream(int weight_type, const ProductArgs &a, hipStream_t s) {
-    return a.offsets ? stream<true>(weight_type, a, s) : stream<false>(weight_type, a, s);
+int stream_rounds(int64_t P, int64_t K, int64_t N, int64_t E) {
+    // (us, rounded by every workgroup -> by a launch in front: K = 5120: N = 17408 1 row 21.0 -> 23.8, 2 rows 23.1 -> 24.2, 4 26.1 -> 24.6; N = 5120 1 8.0 -> 9.9,
+    // 2 9.0 -> 10.1, 4 11.0 -> 10.4; N = 1024 1 6.7 -> 9.0, 4 9.6 -> 9.4; K = 17408, N = 5120 1 22.6 -> 25.7; 8 groups of 1 row, N = 1280 17.5 -> 20.6, 16 27.7 -> 26.7)
+    const int64_t most = kMostLds / (up_to(K, 64) + 16), T = most < 16 ? most : 16;
+    if (T == 0 || P > (E ? 8 : 2)) return 0;
+    return P * K * ((N + 31) / 32) <= 6000000 ? (int) (T < P ? T : P) : 0;
+}
+
+hipError_t launch_stream(int weight_type, int x_type, const ProductArgs &a, hipStream_t s) {
+    return a.offsets ? stream<true>(weight_type, x_type, a, s) : stream<false>(weight_type, x_type, a, s);
 }
 
 }  // namespace prod

@@ -1,9 +1,9 @@
 // Products of many rows (int8, or grouped by expert): tiles of rows of the weight x rows of x, both operands through LDS.
 //
-// Loads go from memory to LDS without passing registers, a ring of R steps of 64 bytes of both operands ahead. The weight lies in memory as
+// Loads go from memory to LDS without passing registers, rings of steps of 64 bytes ahead. The weight lies in memory as
 // the matrix instructions take it. Rows of x lie as they are, wherever the call's indices say, so that nothing copies them together:
-// a load takes 64 bytes of each of 16 rows, and which 16 of those 64 bytes go to which place of the row in LDS turns with the row, so
-// that the reads of a fragment, the same bytes of 32 rows, meet different banks.
+// a load takes 128 bytes, two steps, of each of 8 rows, and which 16 of those bytes go to which place of the row in LDS turns with the row,
+// so that the reads of a fragment, the same bytes of 32 rows, meet different banks.
 #include <type_traits>
 
 #include "rq_prod.h"
@@ -36,120 +36,171 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
                      (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (b >> 32)) << 32));
 }
 
-// Wavefront (wr, wc) of 2 x WC has RB blocks of 32 rows x TB of 32 positions. R: slots of the ring of steps in LDS.
-template <int WT, int RB, int TB, int WC, int R>
+// Wavefront (wr, wc) of WR x WC has RB blocks of 32 rows x TB of 32 positions. In LDS S slots of pairs of steps of x and RA slots of steps of the weight.
+template <int WT, int RB, int TB, int WR, int WC, int S, int RA>
 struct Tiled {
     using Acc = typename Matrix<WT>::Acc;
-    static constexpr int kWaves = 2 * WC, kThreads = 64 * kWaves;
-    static constexpr int kABlocks = 2 * RB, kBBlocks = WC * TB;
-    static constexpr int kSlot = (kABlocks + kBBlocks) * 2048;   // one step of both operands
-    static constexpr int kRing = R * kSlot, kStride = 68, kOut = kWaves * 32 * kStride * 4;   // (of the outputs on their way out)
+    static constexpr int kWaves = WR * WC, kThreads = 64 * kWaves;
+    static constexpr int kABlocks = WR * RB, kBBlocks = WC * TB;
+    static constexpr int kSlotA = kABlocks * 2048, kSlotB = kBBlocks * 4096;   // a step of the weight, a pair of steps of x
+    static constexpr int kRingA = RA * kSlotA, kRing = kRingA + S * kSlotB, kStride = 68, kOut = kWaves * 32 * kStride * 4;   // (of the outputs on their way out)
     static constexpr int kBytes = kRing > kOut ? kRing : kOut;
-    static constexpr int kARuns = 2 * kABlocks / kWaves, kBRuns = 2 * kBBlocks / kWaves, kRuns = kARuns + kBRuns;   // 1 KiB each, of a wavefront per step
-    static_assert(2 * kABlocks % kWaves == 0 && 2 * kBBlocks % kWaves == 0, "split of the loads");
-    static_assert(R >= 3 && kBytes <= 163840, "ring");
-    static constexpr int kTileRows = 64 * RB, kTileTokens = 32 * WC * TB;
+    static constexpr int kARuns = 2 * kABlocks / kWaves, kBRuns = 4 * kBBlocks / kWaves;   // 1 KiB each, of a wavefront per step and per pair of steps
+    static_assert(2 * kABlocks % kWaves == 0 && 4 * kBBlocks % kWaves == 0, "split of the loads");
+    static_assert(RA >= 3 && S >= 2 && kBytes <= 163840, "rings");
+    static constexpr int kTileRows = 32 * WR * RB, kTileTokens = 32 * WC * TB;
 
     const uint8_t *a_src[kARuns];   // wave-uniform
     const uint8_t *b_src[kBRuns];   // the lane's
-    bool           b_last;          // whether the lane's 16 bytes of the last step are of the row
+    bool           b_last[2];       // whether the lane's 16 bytes of the last pair of steps are of the row, for its even and odd runs
     uint32_t       lds0, lane16;
     int            wave, wr, wc, lane, steps;
     const uint8_t *a_lds;           // this lane's place in slot 0
-    const uint8_t *b_lds[2];        // of either run of a step
+    const uint8_t *b_lds[4];        // of the runs of a pair of steps
     Acc            acc[RB][TB];
-    v4i            A[RB][2];
 
+    __device__ __forceinline__ void fetch_a(int t, int slot, int i) {
+        load_run(a_src[i] + (int64_t) t * 2048, lane16, lds0 + slot * kSlotA + (wave * kARuns + i) * 1024);
+    }
+    // pair q of steps
     template <bool LAST>
-    __device__ __forceinline__ void fetch_run(int t, int slot, int i) {
-        const uint32_t to = lds0 + slot * kSlot;
-        if (i < kARuns) {
-            load_run(a_src[i] + (int64_t) t * 2048, lane16, to + (wave * kARuns + i) * 1024);
-        } else {
-            const uint8_t *from = b_src[i - kARuns] + (int64_t) t * 64;
-            if (LAST && t == steps - 1 && !b_last) from = kZeros;
-            load_run(from, to + (2 * kABlocks + wave * kBRuns + i - kARuns) * 1024);
-        }
+    __device__ __forceinline__ void fetch_b(int q, int slot, int i) {
+        const uint8_t *from = b_src[i] + (int64_t) q * 128;
+        if (LAST && q == (steps - 1) >> 1 && !b_last[(wave * kBRuns + i) & 1]) from = kZeros;
+        load_run(from, lds0 + kRingA + slot * kSlotB + (wave * kBRuns + i) * 1024);
     }
-    __device__ __forceinline__ void read_a(int slot, int i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) A[i][h] = *reinterpret_cast<const v4i *>(a_lds + slot * kSlot + (2 * i + h) * 1024);
+    __device__ __forceinline__ v4i read_a(int slot, int i, int h) const { return *reinterpret_cast<const v4i *>(a_lds + slot * kSlotA + (2 * i + h) * 1024); }
+    template <int J>
+    __device__ __forceinline__ v4i read_b(int slot, int i, int h) const {
+        return *reinterpret_cast<const v4i *>(b_lds[2 * J + h] + slot * kSlotB + i * 4096);
     }
-    __device__ __forceinline__ void read_b(v4i (&B)[TB][2], int slot, int i) const {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) B[i][h] = *reinterpret_cast<const v4i *>(b_lds[h] + slot * kSlot + i * 2048);
-    }
-
-    // Step t: its products from A and B, behind each row block's the read of its fragments of step t + 1, between them the reads of
-    // step t + 1's rows of x into N and the fetch of step t + R - 1 into the slot of step t - 1. Who has passed this step's barrier has issued
-    // the products of step t - 1, which waited for that slot's reads. MORE: all of those steps exist, and the one fetched is not the last.
-    template <bool ACTIVE, bool MORE>
-    __device__ __forceinline__ void step(int t, int slot, const v4i (&B)[TB][2], v4i (&N)[TB][2]) {
-        const int  next = slot + 1 == R ? 0 : slot + 1, last = slot == 0 ? R - 1 : slot - 1;
-        const bool get = MORE || t + R - 1 < steps;
-        // step t + 1 has arrived; those behind it need not have
-        if (MORE || t + R - 2 < steps) wait_loads<(R - 3) * kRuns>();
-        else wait_loads<0>();
-        barrier();
-        if (!MORE && get) {
-#pragma unroll
-            for (int i = 0; i < kRuns; ++i) fetch_run<true>(t + R - 1, last, i);
-        }
-#pragma unroll
-        for (int r = 0; r < RB; ++r) {
-            if constexpr (ACTIVE) {
-#pragma unroll
-                for (int b = 0; b < TB; ++b) acc[r][b] = Matrix<WT>::mfma(A[r][0], B[b][0], acc[r][b]);
-                // (past the last step: what the ring holds, for nobody)
-#pragma unroll
-                for (int i = r * TB / RB; i < (r + 1) * TB / RB; ++i) read_b(N, next, i);
-            }
-            if (MORE) {
-#pragma unroll
-                for (int i = r * kRuns / RB; i < (r + 1) * kRuns / RB; ++i) fetch_run<false>(t + R - 1, last, i);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (ACTIVE) {
-#pragma unroll
-                for (int b = 0; b < TB; ++b) acc[r][b] = Matrix<WT>::mfma(A[r][1], B[b][1], acc[r][b]);
-                read_a(next, r);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-
-    // ACTIVE: this wavefront has positions; otherwise it moves its share and keeps the barriers
-    template <bool ACTIVE>
-    __device__ __forceinline__ void loop() {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
             for (int t = 0; t < TB; ++t) acc[r][t] = Acc{ 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0 };
+    }
+
+    // Step t fetches the pair of steps that begins at t + 2 S - 2, if t is even, and behind it the weight's of t + RA - 1, each into the slot that step t - 1
+    // was the last to use: who has passed step t's barrier has issued the products of step t - 1, which waited for its reads. In front of its barrier step t
+    // waits for what step t + 1 needs, whose fragments it reads: `behind` counts what was fetched since, by the parity J of t, and need not be there.
+    static constexpr bool kBoth = RB * TB <= 4;   // fragments of both operands are held twice
+    static constexpr int even_steps(int J, int back) {   // of the `back` steps in front of t
+        int n = 0;
+        for (int k = 1; k <= back; ++k) n += (J + k) % 2 == 0;
+        return n;
+    }
+    static constexpr int behind(int J) {
+        const int a = RA - 3;                                // steps whose fetches all stand behind the weight's of t + 1
+        const int b = 2 * S - 4;                             // J == 1: ... behind the pair of t + 1, the weight's beside it too
+        const int by_a = a * kARuns + even_steps(J, a) * kBRuns, by_b = (b + 1) * kARuns + even_steps(J, b) * kBRuns;
+        return J == 0 || by_a < by_b ? by_a : by_b;
+    }
+    // (a fetch past the last step is not made, and the count would be wrong)
+    template <int J, bool MORE>
+    __device__ __forceinline__ void wait_for_next(int t) const {
+        if (MORE || (t + RA - 2 < steps && t + 2 * S - 3 < steps)) wait_loads<behind(J)>();
+        else wait_loads<0>();
+    }
+    // i-th fetch of step t: x's first
+    __device__ __forceinline__ void fetch_new(int i, int pairs, int t, int slot_a, int slot_b) {
+        if (i < pairs) fetch_b<false>((t >> 1) + S - 1, slot_b, i);
+        else fetch_a(t + RA - 1, slot_a, i - pairs);
+    }
+    // Where a wavefront has few blocks the reads stand in front, so that the rest of the step's products hide them; where it has eight, registers do not
+    // hold both steps' A (NA is A), and a row block's is read behind its products. MORE: all of those steps exist, and the pair fetched is not the last.
+    template <bool ACTIVE, int J, bool MORE>
+    __device__ __forceinline__ void step(int t, int sa, int sb, v4i (&A)[RB][2], const v4i (&B)[TB][2], v4i (&NA)[RB][2], v4i (&NB)[TB][2]) {
+        const int next_a = sa + 1 == RA ? 0 : sa + 1, last_a = sa == 0 ? RA - 1 : sa - 1;
+        const int next_b = J == 0 ? sb : sb + 1 == S ? 0 : sb + 1, last_b = sb == 0 ? S - 1 : sb - 1;
+        wait_for_next<J, MORE>(t);
+        barrier();
+        if (!MORE) {
+            if (J == 0 && t + 2 * S - 2 < steps)
 #pragma unroll
-        for (int t = 0; t < R - 1; ++t) {
-            if (t < steps) {
+                for (int i = 0; i < kBRuns; ++i) fetch_b<true>((t >> 1) + S - 1, last_b, i);
+            if (t + RA - 1 < steps)
 #pragma unroll
-                for (int i = 0; i < kRuns; ++i) fetch_run<true>(t, t, i);
+                for (int i = 0; i < kARuns; ++i) fetch_a(t + RA - 1, last_a, i);
+        }
+        // One read or fetch behind each product, as far as there are products: a wavefront issues in order, and a run of fetches would leave the matrix
+        // core idle while they queue.
+        constexpr int kX = MORE && J == 0 ? kBRuns : 0, kNew = kX + (MORE ? kARuns : 0);
+        if constexpr (!ACTIVE) {
+#pragma unroll
+            for (int i = 0; i < kNew; ++i) fetch_new(i, kX, t, last_a, last_b);
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            // of this row block's share: A's fragments of the row block in front (of all, where A is held twice), B's, fetches
+            // (past the last step the fragments are what the rings hold, for nobody)
+            const int a0 = kBoth ? 2 * RB * r / RB : r == 0 ? 0 : 2 * (r - 1), a1 = kBoth ? 2 * RB * (r + 1) / RB : 2 * r;
+            const int b0 = 2 * TB * r / RB, b1 = 2 * TB * (r + 1) / RB, f0 = kNew * r / RB, f1 = kNew * (r + 1) / RB;
+            const int ops = a1 - a0 + b1 - b0 + f1 - f0;
+#pragma unroll
+            for (int m = 0; m < 2 * TB; ++m) {
+                const int h = m / TB, b = m % TB;
+                acc[r][b] = Matrix<WT>::mfma(A[r][h], B[b][h], acc[r][b]);
+#pragma unroll
+                for (int k = ops * m / (2 * TB); k < ops * (m + 1) / (2 * TB); ++k) {
+                    if (k < b1 - b0) {
+                        const int i = b0 + k;
+                        NB[i >> 1][i & 1] = read_b<1 - J>(next_b, i >> 1, i & 1);
+                    } else if (k < b1 - b0 + a1 - a0) {
+                        const int i = a0 + k - (b1 - b0);
+                        NA[i >> 1][i & 1] = read_a(next_a, i >> 1, i & 1);
+                    } else {
+                        fetch_new(f0 + k - (b1 - b0) - (a1 - a0), kX, t, last_a, last_b);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (steps >= R - 1) wait_loads<(R - 2) * kRuns>();
-        else wait_loads<0>();
+        if constexpr (!kBoth) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) NA[RB - 1][h] = read_a(next_a, RB - 1, h);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // ACTIVE: this wavefront has positions; otherwise it moves its share and keeps the barriers
+    template <bool ACTIVE>
+    __device__ __forceinline__ void loop() {
+        clear();
+        constexpr int kAhead = RA > 2 * S - 1 ? RA : 2 * S;
+#pragma unroll
+        for (int t = -kAhead; t < 0; ++t) {   // (as the steps in front of the first would)
+            if (t % 2 == 0 && t / 2 + S - 1 >= 0 && t + 2 * S - 2 < steps)
+#pragma unroll
+                for (int i = 0; i < kBRuns; ++i) fetch_b<true>(t / 2 + S - 1, t / 2 + S - 1, i);
+            if (t + RA - 1 >= 0 && t + RA - 1 < steps)
+#pragma unroll
+                for (int i = 0; i < kARuns; ++i) fetch_a(t + RA - 1, t + RA - 1, i);
+        }
+        wait_for_next<1, false>(-1);
         barrier();
-        v4i B[TB][2], N[TB][2];
+        v4i A[RB][2], NA[kBoth ? RB : 1][2], B[TB][2], NB[TB][2];
+        auto &A2 = [&]() -> v4i(&)[RB][2] {
+            if constexpr (kBoth) return NA;
+            else return A;
+        }();
 #pragma unroll
-        for (int i = 0; i < RB; ++i) read_a(0, i);
+        for (int i = 0; i < 2 * RB; ++i) A[i >> 1][i & 1] = read_a(0, i >> 1, i & 1);
 #pragma unroll
-        for (int i = 0; i < TB; ++i) read_b(B, 0, i);
-        int  t = 0, slot = 0;
-        auto next = [&]() __attribute__((always_inline)) { ++t, slot = slot + 1 == R ? 0 : slot + 1; };
-        while (t + R + 1 < steps) {   // (both steps fetch one in front of the last)
-            step<ACTIVE, true>(t, slot, B, N), next();
-            step<ACTIVE, true>(t, slot, N, B), next();
+        for (int i = 0; i < 2 * TB; ++i) B[i >> 1][i & 1] = read_b<0>(0, i >> 1, i & 1);
+        int  t = 0, sa = 0, sb = 0;
+        auto next = [&](bool pair) __attribute__((always_inline)) {
+            ++t, sa = sa + 1 == RA ? 0 : sa + 1;
+            if (pair) sb = sb + 1 == S ? 0 : sb + 1;
+        };
+        while (t + RA < steps && t + 2 * S - 2 < ((steps - 1) & ~1)) {
+            step<ACTIVE, 0, true>(t, sa, sb, A, B, A2, NB), next(false);
+            step<ACTIVE, 1, true>(t, sa, sb, A2, NB, A, B), next(true);
         }
         while (true) {
-            step<ACTIVE, false>(t, slot, B, N), next();
+            step<ACTIVE, 0, false>(t, sa, sb, A, B, A2, NB), next(false);
             if (t >= steps) break;
-            step<ACTIVE, false>(t, slot, N, B), next();
+            step<ACTIVE, 1, false>(t, sa, sb, A2, NB, A, B), next(true);
             if (t >= steps) break;
         }
         wait_loads<0>();   // (none of this wavefront's loads lands in LDS behind this)
@@ -162,75 +213,85 @@ __device__ __forceinline__ int place_of(int index, int total) {
     return xcd * each + min(xcd, more) + (index >> 3);
 }
 
-template <int WT, int RB, int TB, int WC, int R, bool GROUPED>
-__global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB <= 4 ? 3 : 1) void rq_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles,
+// SPLIT: a.splits workgroups share a tile's bytes, a.split_steps steps each. Each wavefront leaves its sums, as they lie in its registers, in the
+// workspace and counts itself in; the last of those that hold the same outputs adds them up, in the order of the bytes, so that the bits do
+// not depend on who is last. The sums go past the XCDs' caches (atomic stores and loads of the device's scope) and are waited for before the count, so
+// who sees the last count sees all sums.
+template <int WT, int RB, int TB, int WR, int WC, int S, int RA, bool GROUPED, bool SPLIT>
+__global__ __launch_bounds__(64 * WR * WC, 2) void rq_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles,
                                                                                                  const int across) {
-    using G = Tiled<WT, RB, TB, WC, R>;
+    using G = Tiled<WT, RB, TB, WR, WC, S, RA>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int index = (int) blockIdx.y * across + (int) blockIdx.x;
-    int       e = 0, first, count, row_tile;
+    const int splits = SPLIT ? a.splits : 1;
+    int       e = 0, first, count, row_tile, v;   // v: which tile of all, then which part of it
     if constexpr (GROUPED) {
-        // The tiles of the groups in a row, rows of the weight fastest: an XCD then reads the weights of its groups, and few others do.
+        // The groups one behind the other; in a group, for each run of rows of its weight the tiles of its positions, which start together on one XCD
+        // and read the weight together.
         constexpr int T = G::kTileTokens;
-        auto tiles = [](int n) { return (n + T - 1) / T; };
+        auto units = [&](int n) { return (n + T - 1) / T * row_tiles * splits; };
         int  gfirst, gcount, place, total;
-        find_group(a, -1, tiles, e, gfirst, gcount, place, total);
-        if (index >= total * row_tiles) return;
-        const int v = place_of(index, total * row_tiles), tile = v / row_tiles;
-        row_tile = v - tile * row_tiles;
-        if (!find_group(a, tile, tiles, e, gfirst, gcount, place, total)) return;
-        first = gfirst + place * T;
-        count = min(T, gcount - place * T);
-    } else {
-        const int total = row_tiles * token_tiles;
+        find_group(a, -1, units, e, gfirst, gcount, place, total);
         if (index >= total) return;
-        const int v = place_of(index, total);
-        row_tile = v / token_tiles;
-        first = (v - row_tile * token_tiles) * G::kTileTokens;
+        v = place_of(index, total);
+        if (!find_group(a, v, units, e, gfirst, gcount, place, total)) return;
+        place /= splits;
+        const int tiles = (gcount + T - 1) / T, tile = place % tiles;
+        row_tile = place / tiles;
+        first = gfirst + tile * T;
+        count = min(T, gcount - tile * T);
+    } else {
+        const int total = row_tiles * token_tiles * splits;
+        if (index >= total) return;
+        v = place_of(index, total);
+        row_tile = v / splits / token_tiles;
+        first = (v / splits - row_tile * token_tiles) * G::kTileTokens;
         count = (int) (a.P - first < G::kTileTokens ? a.P - first : G::kTileTokens);
     }
+    const int part = SPLIT ? v % splits : 0;
+    v /= splits;
     G g;
     g.lane = threadIdx.x & 63;
     g.wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    g.wr = g.wave & 1;
+    g.wr = g.wave % WR;
     // (with four wavefronts the workgroups take turns in which SIMDs a tile with half of its positions leaves idle)
-    g.wc = WC == 2 ? ((g.wave >> 1) ^ (index >> 3)) & 1 : g.wave >> 1;
+    g.wc = WR == 2 && WC == 2 ? ((g.wave >> 1) ^ (index >> 3)) & 1 : g.wave / WR;
     g.lane16 = g.lane * 16;
-    g.steps = a.L.steps;
+    const int step0 = SPLIT ? part * a.split_steps : 0;   // (even: the pairs of steps)
+    g.steps = SPLIT ? min(a.split_steps, a.L.steps - step0) : a.L.steps;
     g.lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void *) lds;
     g.a_lds = lds + g.wr * RB * 2048 + g.lane * 16;
-    // Row j of 16 keeps its bytes 16 c .. + 15 at place c ^ (j / 4) of its 64: 16 rows' same bytes lie in 16 places of the banks' 256 bytes.
+    // A row keeps its bytes 16 c .. + 15 at place c ^ (row / 2 % 8) of its 128: 16 rows' same bytes lie in 16 places of the banks' 256 bytes.
     {
-        const int row = g.lane & 31, turn = (row >> 2) & 3, half = g.lane >> 5;
-        const uint8_t *b = lds + (2 * G::kABlocks + g.wc * TB * 2) * 1024 + row * 64;
-        g.b_lds[0] = b + (half ^ turn) * 16;
-        g.b_lds[1] = b + ((2 + half) ^ turn) * 16;
+        const int      row = g.lane & 31, turn = (row >> 1) & 7, half = g.lane >> 5;
+        const uint8_t *b = lds + G::kRingA + g.wc * TB * 4096 + row * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g.b_lds[i] = b + ((2 * i + half) ^ turn) * 16;
     }
-    const int      block0 = row_tile * G::kABlocks;
+    const int      block0 = a.first_block + row_tile * G::kABlocks;
     const uint8_t *w = a.w + (int64_t) e * a.L.expert_bytes;
 #pragma unroll
     for (int i = 0; i < G::kARuns; ++i) {   // (blocks past the weight's repeat its last one)
         const int run = g.wave * G::kARuns + i, block = min(block0 + (run >> 1), a.L.row_blocks - 1);
-        g.a_src[i] = uniform(w + (int64_t) block * a.L.steps * 2048 + (run & 1) * 1024);
+        g.a_src[i] = uniform(w + ((int64_t) block * a.L.steps + step0) * 2048 + (run & 1) * 1024);
     }
-    const int chunk = (g.lane & 3) ^ ((g.lane >> 4) & 3);
-    g.b_last = (int64_t) (a.L.steps - 1) * 64 + chunk * 16 < a.x_bytes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) g.b_last[i] = (int64_t) ((step0 + g.steps - 1) >> 1) * 128 + ((g.lane & 7) ^ (i * 4 + (g.lane >> 4))) * 16 < a.x_bytes;
 #pragma unroll
     for (int i = 0; i < G::kBRuns; ++i) {   // (positions past the last repeat it)
-        const int     at = min((g.wave * G::kBRuns + i) * 16 + (g.lane >> 2), count - 1);
+        const int     run = g.wave * G::kBRuns + i, at = min(run * 8 + (g.lane >> 3), count - 1);
         const int64_t row = row_read(a, first + at);
-        g.b_src[i] = a.x + (row < 0 ? 0 : row) * a.pitch + chunk * 16;
+        g.b_src[i] = a.x + (row < 0 ? 0 : row) * a.pitch + (int64_t) step0 * 64 + ((g.lane & 7) ^ ((run & 1) * 4 + (g.lane >> 4))) * 16;
     }
     if (g.wc * TB * 32 < count) g.template loop<true>();
     else g.template loop<false>();
 
-    // 32 positions x 64 rows at a time through LDS (a region of the wavefront's own), so that a position's outputs leave as whole lines.
+    // 32 positions x 64 rows at a time through LDS (a region of the wavefront's own), in the output's type, so that a position's outputs
+    // leave as whole lines and LDS moves no more than they are.
     const int    lane = g.lane, wr = g.wr, wc = g.wc;
-    float       *mine = reinterpret_cast<float *>(lds) + g.wave * 32 * G::kStride;
-    const int    dtype = a.out_dtype;
     const float *t_scales = reinterpret_cast<const float *>(w + a.L.code_bytes);
     int          out_at[TB];   // (a position a lane; y's rows are fewer than 2^31)
-    float        s_m[TB];      // of int8; and 0 for a row that is not there
+    float        s_m[TB];      // of int8
     bool         in_there[TB];
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
@@ -246,73 +307,131 @@ __global__ __launch_bounds__(128 * WC, WC == 4 ? 2 : RB * TB <= 2 ? 2 : RB * TB 
     }
     barrier();   // (the ring is not read any more)
     if (wc * TB * 32 >= count) return;
-    // LANES of a position write 16 bytes each
-    auto store = [&](auto lanes, int t, int r) __attribute__((always_inline)) {
-        constexpr int kLanes = decltype(lanes)::value, kTokens = 64 / kLanes;
-        const int     n = lane % kLanes * (dtype == RQ_F32 ? 4 : 8);
-        const int64_t n0 = (int64_t) (block0 + wr * RB + r) * 32 + n;
+    if constexpr (SPLIT) {
+        constexpr int kPairs = RB * TB * 8;   // 512 bytes each
+        const int     outputs = v * G::kWaves + WR * wc + wr;   // (of the tile's: which wavefront has them differs by workgroup)
+        auto         *sums = reinterpret_cast<uint64_t *>(a.sums) + (int64_t) outputs * splits * kPairs * 64 + lane;
+        auto          bits = [](auto x) __attribute__((always_inline)) { return __builtin_bit_cast(uint32_t, x); };
 #pragma unroll
-        for (int i = 0; i < 32 / kTokens; ++i) {
-            const int     at = i * kTokens + lane / kLanes;
-            const int64_t row = __shfl(out_at[t], at);
-            if (row >= 0) store_out(dtype, a.y, row * a.ldy, n0, a.L.N, mine + at * G::kStride + n);
+        for (int i = 0; i < kPairs; ++i) {
+            const auto    &c = g.acc[i / 8 / TB][i / 8 % TB];
+            const uint64_t x = (uint64_t) bits(c[i % 8 * 2 + 1]) << 32 | bits(c[i % 8 * 2]);
+            __hip_atomic_store(sums + (part * kPairs + i) * 64, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-    };
+        wait_loads<0>();   // (stores count alike: all of them are where every XCD sees them)
+        int before = 0;
+        if (lane == 0) before = __hip_atomic_fetch_add(a.arrived + outputs, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__builtin_amdgcn_readfirstlane(before) != splits - 1) return;
+        asm volatile("" : : : "memory");
+        for (int p = 0; p < splits; ++p) {
+            constexpr int kBatch = kPairs < 16 ? kPairs : 16;   // (more, and the registers do not hold them)
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
+            for (int i0 = 0; i0 < kPairs; i0 += kBatch) {
+                uint64_t x[kBatch];
 #pragma unroll
-        for (int r = 0; r < RB; r += 2) {
-            constexpr int kTwo = RB > 1 ? 2 : 1;   // row blocks at a time
-            static_assert(RB % kTwo == 0, "row blocks in pairs");
+                for (int i = 0; i < kBatch; ++i)
+                    x[i] = __hip_atomic_load(sums + (p * kPairs + i0 + i) * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-            for (int q = 0; q < 4 * kTwo; ++q) {
-                const auto &c = g.acc[r + q / 4][t];
-                v4f         v;
-                if constexpr (WT == RQ_I8) {
-                    const int block = min(block0 + wr * RB + r + q / 4, a.L.row_blocks - 1);
-                    const v4f tn = *reinterpret_cast<const v4f *>(t_scales + block * 32 + q % 4 * 8 + (lane >> 5) * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = (float) c[q % 4 * 4 + i] * tn[i] * s_m[t];
-                } else {
-                    v = v4f{ c[q % 4 * 4], c[q % 4 * 4 + 1], c[q % 4 * 4 + 2], c[q % 4 * 4 + 3] };
+                for (int i = 0; i < kBatch; ++i) {
+                    const int k = i0 + i;
+                    auto     &c = g.acc[k / 8 / TB][k / 8 % TB];
+                    using E = std::remove_reference_t<decltype(c[0] + c[0])>;
+                    const E lo = __builtin_bit_cast(E, (uint32_t) x[i]), hi = __builtin_bit_cast(E, (uint32_t) (x[i] >> 32));
+                    c[k % 8 * 2] = p ? c[k % 8 * 2] + lo : lo;
+                    c[k % 8 * 2 + 1] = p ? c[k % 8 * 2 + 1] + hi : hi;
                 }
-                if (!in_there[t]) v = v4f{ 0, 0, 0, 0 };
-                *reinterpret_cast<v4f *>(mine + (lane & 31) * G::kStride + q * 8 + (lane >> 5) * 4) = v;
             }
-            __builtin_amdgcn_wave_barrier();
-            if (dtype == RQ_F32) store(std::integral_constant<int, 8 * kTwo>{}, t, r);
-            else store(std::integral_constant<int, 4 * kTwo>{}, t, r);
-            __builtin_amdgcn_wave_barrier();
         }
     }
+    auto write = [&](auto out) __attribute__((always_inline)) {
+        constexpr int OT = decltype(out)::value;
+        using T = typename Element<OT>::type;
+        constexpr int kTwo = RB > 1 ? 2 : 1;                                  // row blocks at a time
+        constexpr int kEach = 16 / (int) sizeof(T), kLanes = 32 * kTwo / kEach;   // a lane writes 16 bytes, so many lanes a position
+        constexpr int kPlaces = 64 / kLanes, kPitch = 64 + kEach;             // (of elements: 16 bytes behind a position's 64)
+        static_assert(RB % kTwo == 0, "row blocks in pairs");
+        T *mine = reinterpret_cast<T *>(lds + g.wave * 32 * G::kStride * 4);
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+#pragma unroll
+            for (int r = 0; r < RB; r += kTwo) {
+#pragma unroll
+                for (int q = 0; q < 4 * kTwo; ++q) {
+                    const auto &c = g.acc[r + q / 4][t];
+                    v4f         v;
+                    if constexpr (WT == RQ_I8) {
+                        const int block = min(block0 + wr * RB + r + q / 4, a.L.row_blocks - 1);
+                        const v4f tn = *reinterpret_cast<const v4f *>(t_scales + block * 32 + q % 4 * 8 + (lane >> 5) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = (float) c[q % 4 * 4 + i] * tn[i] * s_m[t];
+                    } else {
+                        v = v4f{ c[q % 4 * 4], c[q % 4 * 4 + 1], c[q % 4 * 4 + 2], c[q % 4 * 4 + 3] };
+                    }
+                    if (!in_there[t]) v = v4f{ 0, 0, 0, 0 };
+                    T *to = mine + (lane & 31) * kPitch + q * 8 + (lane >> 5) * 4;
+                    if constexpr (OT == RQ_F32) *reinterpret_cast<v4f *>(to) = v;
+                    else *reinterpret_cast<uint2 *>(to) = make_uint2(mx::pair_bits<OT>(v[0], v[1]), mx::pair_bits<OT>(v[2], v[3]));
+                }
+                __builtin_amdgcn_wave_barrier();
+                const int     n = lane % kLanes * kEach;
+                const int64_t n0 = (int64_t) (block0 + wr * RB + r) * 32 + n;
+                T            *y = reinterpret_cast<T *>(a.y);
+#pragma unroll
+                for (int i = 0; i < 32 / kPlaces; ++i) {
+                    const int     at = i * kPlaces + lane / kLanes;
+                    const int64_t row = __shfl(out_at[t], at);
+                    const T      *from = mine + at * kPitch + n;
+                    if (row < 0 || n0 >= a.L.N) continue;
+                    T *to = y + row * a.ldy + n0;
+                    if (n0 + kEach <= a.L.N && ((uintptr_t) to & 15) == 0) {
+                        *reinterpret_cast<v4i *>(to) = *reinterpret_cast<const v4i *>(from);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kEach; ++k)
+                            if (n0 + k < a.L.N) to[k] = from[k];
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+    };
+    if (a.out_dtype == RQ_F32) write(std::integral_constant<int, RQ_F32>{});
+    else if (a.out_dtype == RQ_F16) write(std::integral_constant<int, RQ_F16>{});
+    else write(std::integral_constant<int, RQ_BF16>{});
 }
 
 constexpr int64_t kAcross = 1 << 20;   // workgroups in one dimension of a grid, which may have under 2^32 threads
 
-template <int WT, int RB, int TB, int WC, int R, bool GROUPED>
+template <int WT, int RB, int TB, int WR, int WC, int S, int RA, bool GROUPED, bool SPLIT = false>
 hipError_t launch(const ProductArgs &a, hipStream_t stream) {
-    using G = Tiled<WT, RB, TB, WC, R>;
-    const int64_t row_tiles = (a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows;
-    int64_t       token_tiles = (a.P + G::kTileTokens - 1) / G::kTileTokens;
-    if (GROUPED) token_tiles = a.P / G::kTileTokens + (a.P < a.E ? a.P : a.E);   // (at most: every group's last tile is not full)
-    const int64_t groups = row_tiles * token_tiles;
+    using G = Tiled<WT, RB, TB, WR, WC, S, RA>;
+    const int64_t row_tiles = a.row_tiles ? a.row_tiles : (a.L.row_blocks * 32 + G::kTileRows - 1) / G::kTileRows;
+    const int64_t token_tiles = most_token_tiles(G::kTileTokens, a.P, GROUPED ? a.E : 0), groups = row_tiles * token_tiles * (SPLIT ? a.splits : 1);
     if (groups > 0x7FFFFFFFll - kAcross) return hipErrorInvalidConfiguration;
     const unsigned across = (unsigned) (groups < kAcross ? groups : kAcross);
     static std::atomic<uint64_t> allowed{ 0 };   // devices on which the kernel may have its LDS
-    const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_tiled_kernel<WT, RB, TB, WC, R, GROUPED>), G::kBytes, allowed);
+    const hipError_t e = allow_lds(reinterpret_cast<const void *>(rq_tiled_kernel<WT, RB, TB, WR, WC, S, RA, GROUPED, SPLIT>), G::kBytes, allowed);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((rq_tiled_kernel<WT, RB, TB, WC, R, GROUPED>), dim3(across, (unsigned) ((groups + across - 1) / across)),
+    hipLaunchKernelGGL((rq_tiled_kernel<WT, RB, TB, WR, WC, S, RA, GROUPED, SPLIT>), dim3(across, (unsigned) ((groups + across - 1) / across)),
                        dim3(G::kThreads), G::kBytes, stream, a, (int) row_tiles, (int) token_tiles, (int) across);
     return hipGetLastError();
 }
 
 template <int WT, bool GROUPED>
 hipError_t launch_form(int form, const ProductArgs &a, hipStream_t stream) {
+    if (a.splits > 1) {
+        switch (form) {
+            case 0: return launch<WT, 1, 1, 2, 2, 4, 9, GROUPED, true>(a, stream);
+            case 1: return launch<WT, 2, 1, 2, 2, 3, 7, GROUPED, true>(a, stream);
+            default: return launch<WT, 2, 2, 2, 2, 3, 5, GROUPED, true>(a, stream);
+        }
+    }
     switch (form) {
-        case 0: return launch<WT, 1, 1, 2, 8, GROUPED>(a, stream);
-        case 1: return launch<WT, 2, 1, 2, 6, GROUPED>(a, stream);
-        case 2: return launch<WT, 2, 2, 2, 4, GROUPED>(a, stream);
-        default: return launch<WT, 4, 2, 4, 4, GROUPED>(a, stream);
+        case 0: return launch<WT, 1, 1, 2, 2, 4, 9, GROUPED>(a, stream);
+        case 1: return launch<WT, 2, 1, 2, 2, 3, 7, GROUPED>(a, stream);
+        case 2: return launch<WT, 2, 2, 2, 2, 3, 4, GROUPED>(a, stream);
+        case 3: return launch<WT, 2, 2, 2, 2, 3, 5, GROUPED>(a, stream);
+        default: return launch<WT, 4, 2, 2, 4, 3, 4, GROUPED>(a, stream);
     }
 }
 template <bool GROUPED>
@@ -322,7 +441,7 @@ hipError_t launch_type(int weight_type, int form, const ProductArgs &a, hipStrea
     return launch_form<RQ_BF16, GROUPED>(form, a, stream);
 }
 
-constexpr int kRowsOf[kForms] = { 64, 128, 128, 256 }, kTokensOf[kForms] = { 64, 64, 128, 256 };
+constexpr int kRowsOf[kForms] = { 64, 128, 128, 128, 256 }, kTokensOf[kForms] = { 64, 64, 128, 128, 256 };
 
 }  // namespace
 

@@ -2,8 +2,8 @@
 C ABI of include/rq_i8.h.
 
 An int8 row of K numbers is K codes and one fp32 scale; a code c stands for c times the scale. Rounding a row: the scale is its largest
-magnitude / 127 (at least 2 ** -126), the codes are the whole numbers nearest to x times the scale's fp32 reciprocal, ties to even. A row
-that holds an infinity or a NaN becomes NaN.
+magnitude times 1 / 127, in fp32 (at least 2 ** -126), the codes are the whole numbers nearest to x times the scale's fp32 reciprocal, ties to
+even. A row that holds an infinity or a NaN becomes NaN.
 
 As in the rest of the package torch owns device memory and the stream, and every computation happens inside librq_w4a4.so, on the
 current stream of the inputs' device. With `out` and `workspace` given the products allocate nothing; the other calls make their

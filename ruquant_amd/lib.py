@@ -112,6 +112,9 @@ PROTOTYPES.update({
     "rq_grouped_workspace_bytes": (_size, [_int, _i64, _i64, _i64, _i64, _i64]),
     "rq_grouped_mul_mat": (_int, [_int, _ptr, _i64, _i64, _i64, _int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _int, _ptr, _i64,
                                   _i64, _ptr, _size, _ptr]),
+    # include/rq_i8_plan.h
+    "rq_i8_product_plan": (_int, [_i64, _i64, _int, _i64, _ptr]),
+    "rq_grouped_plan": (_int, [_int, _i64, _i64, _i64, _int, _i64, _i64, _ptr]),
 })
 
 for _name in ("rq_w4a4_mul_mat", "rq_w4a4_mul_mat_fused"):

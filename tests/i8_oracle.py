@@ -6,7 +6,7 @@ def quantize(x):
     """x [M, K] float64 (values of a float type) -> codes int8 [M, K], scales fp32 [M]"""
     finite = np.isfinite(x).all(axis=1)
     v = np.where(finite[:, None], x, 0.0)
-    scales = np.maximum((np.abs(v).max(axis=1) / 127).astype(np.float32), np.float32(2.0 ** -126))
+    scales = np.maximum(np.abs(v).max(axis=1).astype(np.float32) * np.float32(1 / 127), np.float32(2.0 ** -126))
     r = (1.0 / scales.astype(np.float64)).astype(np.float32)
     codes = np.rint(v * r.astype(np.float64)[:, None]).astype(np.int8)   # (the product of two 24-bit numbers is exact)
     return codes, np.where(finite, scales, np.float32(np.nan))
