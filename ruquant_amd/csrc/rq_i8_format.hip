@@ -7,93 +7,120 @@ namespace rq {
 namespace prod {
 namespace {
 
-constexpr int kUnits = 4;   // of eight elements that a thread keeps between its row's maximum and the codes
-
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, int64_t K, int64_t k, float (&v)[8]) {
+// Eight elements of a row as they lie, zeros behind its end; 16-bit ones in pairs. VEC: on 16 bytes, and rows of a multiple of eight.
+template <int DT> struct Eight {
     using T = typename Element<DT>::type;
-    if constexpr (VEC) {
-        if constexpr (DT == RQ_F32) {
-            const float4 a = reinterpret_cast<const float4 *>(x + k)[0], b = reinterpret_cast<const float4 *>(x + k)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4    u = *reinterpret_cast<const uint4 *>(x + k);
-            const uint32_t w[4] = { u.x, u.y, u.z, u.w };
+    static constexpr bool kWide = DT == RQ_F32;
+    uint32_t w[kWide ? 8 : 4];
+    template <bool VEC> __device__ __forceinline__ void load(const T *x, int64_t K, int64_t k) {
+        if constexpr (VEC) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = to_float(__builtin_bit_cast(T, (uint16_t) w[i]));
-                v[2 * i + 1] = to_float(__builtin_bit_cast(T, (uint16_t) (w[i] >> 16)));
+            for (int i = 0; i < (kWide ? 2 : 1); ++i) {
+                const uint4 u = reinterpret_cast<const uint4 *>(x + k)[i];
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
             }
+        } else if (k + 8 <= K) {
+            load_bytes(w, x + k);
+        } else if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = k + i < K ? __float_as_uint(x[k + i]) : 0u;
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(x) + k;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (k + 2 * i < K ? h[2 * i] : 0u) | (k + 2 * i + 1 < K ? (uint32_t) h[2 * i + 1] << 16 : 0u);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_float(x[k + i]) : 0.0f;
     }
-}
-__device__ __forceinline__ uint32_t top_bits(const float (&v)[8], uint32_t top) {
+    // the larger of `top`, the bits of a magnitude in this type, and those of the elements
+    __device__ __forceinline__ uint32_t top(uint32_t t) const {
+        if constexpr (kWide) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    return top;
-}
-// A row a workgroup of G threads, or 256 / G rows where G < 256. VEC: rows of x on multiples of 16 bytes, K a multiple of 8. PITCH: codes go to rows of `pitch`
-// bytes, on multiples of eight, with zeros up to `padded`; else to rows of K bytes in a row.
-template <int DT, bool VEC, int G>
+            for (int i = 0; i < 8; ++i) t = max(t, w[i] & 0x7FFFFFFFu);
+            return t;
+        } else {
+            typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+            u2 m = __builtin_bit_cast(u2, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u2, w[i] & 0x7FFF7FFFu));
+            const uint32_t both = __builtin_bit_cast(uint32_t, m);
+            return max(t, max(both & 0xFFFF, both >> 16));
+        }
+    }
+    static __device__ __forceinline__ uint32_t as_float_bits(uint32_t t) {
+        if constexpr (kWide) return t;
+        else return __float_as_uint(to_float(__builtin_bit_cast(T, (uint16_t) t)));
+    }
+    __device__ __forceinline__ uint2 codes(const RowScale &q) const {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (kWide) v[i] = __uint_as_float(w[i]);
+            else v[i] = to_float(__builtin_bit_cast(T, (uint16_t) (i & 1 ? w[i >> 1] >> 16 : w[i >> 1])));
+        }
+        return codes_of(v, q.r, q.keep);
+    }
+};
+
+// A row by G threads, U units of eight elements of it held by each between its maximum and the codes; what is longer is read twice. VEC: rows of x on multiples of
+// 16 bytes, K a multiple of 8. Codes go to rows of `pitch` bytes: on multiples of eight with zeros up to `padded`, or (padded 0) of K bytes in a row.
+template <int DT, bool VEC, int G, int U>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void rq_i8_quantize_kernel(const typename Element<DT>::type *x, int64_t ldx, int64_t M, int64_t K,
                                                                            uint8_t *codes, int64_t pitch, int64_t padded, float *scales, int *zero, int zeros) {
     if (zeros && blockIdx.x == 0)
         for (int i = threadIdx.x; i < zeros; i += (int) blockDim.x) zero[i] = 0;
-    constexpr int kRows = G < 256 ? 256 / G : 1;
+    constexpr int kRows = G < 256 ? 256 / G : 1, kWaves = G / 64;
     const int     t = threadIdx.x % G, lane = threadIdx.x & 63;
     const int64_t m = (int64_t) blockIdx.x * kRows + threadIdx.x / G;
     const bool    there = m < M;
     const auto   *row = x + (there ? m : 0) * ldx;
-    float         v[kUnits][8];
+    Eight<DT>     v[U];
     uint32_t      top = 0;
     if (there) {
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int64_t k = (int64_t) (u * G + t) * 8;
-            if (k < K) {
-                load_unit<DT, VEC>(row, K, k, v[u]);
-                top = top_bits(v[u], top);
-            }
+            if (k < K) v[u].template load<VEC>(row, K, k);
         }
-        for (int64_t k = (int64_t) (kUnits * G + t) * 8; k < K; k += G * 8) {
-            float w[8];
-            load_unit<DT, VEC>(row, K, k, w);
-            top = top_bits(w, top);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if ((int64_t) (u * G + t) * 8 < K) top = v[u].top(top);
+        for (int64_t k = (int64_t) (U * G + t) * 8; k < K; k += G * 8) {
+            Eight<DT> w;
+            w.template load<VEC>(row, K, k);
+            top = w.top(top);
         }
     }
     top = wave_max(top);
-    if constexpr (G > 64) {
-        __shared__ uint32_t tops[G / 64];
+    if constexpr (kWaves > 1) {
+        __shared__ uint32_t tops[G < 256 ? 4 : kWaves];
         if (lane == 0) tops[threadIdx.x >> 6] = top;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < G / 64; ++i) top = max(top, tops[i]);
+        for (int i = 0; i < kWaves; ++i) top = max(top, tops[threadIdx.x / G * kWaves + i]);
     }
     if (!there) return;
-    const RowScale q(top);
+    const RowScale q(Eight<DT>::as_float_bits(top));
     if (t == 0) scales[m] = q.s;
     uint8_t *to = codes + m * pitch;
-    auto     put = [&](int64_t k, const float(&w)[8]) __attribute__((always_inline)) {
-        const uint2 c = codes_of(w, q.r, q.keep);
+    auto     put = [&](int64_t k, const Eight<DT> &w) __attribute__((always_inline)) {
+        const uint2 c = w.codes(q);
         if (VEC || k + 8 <= padded) {
             // (rows of K bytes are on multiples of eight where VEC is set, and padded rows always)
             *reinterpret_cast<uint2 *>(to + k) = c;
+        } else if (k + 8 <= K) {
+            store_bytes(to + k, c);
         } else {
             for (int i = 0; i < 8; ++i)
                 if (k + i < K) to[k + i] = (uint8_t) ((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
         }
     };
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
+    for (int u = 0; u < U; ++u) {
         const int64_t k = (int64_t) (u * G + t) * 8;
         if (k < K) put(k, v[u]);
     }
-    for (int64_t k = (int64_t) (kUnits * G + t) * 8; k < K; k += G * 8) {
-        float w[8];
-        load_unit<DT, VEC>(row, K, k, w);
+    for (int64_t k = (int64_t) (U * G + t) * 8; k < K; k += G * 8) {
+        Eight<DT> w;
+        w.template load<VEC>(row, K, k);
         put(k, w);
     }
     for (int64_t k = (K + 7) / 8 * 8 + t * 8; k < padded; k += G * 8) *reinterpret_cast<uint2 *>(to + k) = make_uint2(0, 0);
@@ -109,21 +136,25 @@ __global__ __launch_bounds__(256) void rq_i8_dequantize_kernel(const int8_t *cod
     const float   s = scales[m];
     const int8_t *from = codes + m * K + k;
     auto         *to = out + m * ldo + k;
-    float         v[8];
-    if constexpr (VEC) {
-        const uint2 c = *reinterpret_cast<const uint2 *>(from);
+    if (!VEC && k + 8 > K) {
+        for (int i = 0; k + i < K; ++i) to[i] = from_float<DT>((float) from[i] * s);
+        return;
+    }
+    uint32_t c[2], w[DT == RQ_F32 ? 8 : 4];
+    float    v[8];
+    load_bytes(c, from);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float) (int8_t) ((i < 4 ? c.x : c.y) >> (8 * (i & 3))) * s;
-        if constexpr (DT == RQ_F32) {
-            reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(to) = make_uint4(mx::pair_bits<DT>(v[0], v[1]), mx::pair_bits<DT>(v[2], v[3]),
-                                                        mx::pair_bits<DT>(v[4], v[5]), mx::pair_bits<DT>(v[6], v[7]));
-        }
+    for (int i = 0; i < 8; ++i) v[i] = (float) (int8_t) (c[i >> 2] >> (8 * (i & 3))) * s;
+#pragma unroll
+    for (int i = 0; i < (DT == RQ_F32 ? 8 : 4); ++i) {
+        if constexpr (DT == RQ_F32) w[i] = __float_as_uint(v[i]);
+        else w[i] = mx::pair_bits<DT>(v[2 * i], v[2 * i + 1]);
+    }
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (DT == RQ_F32 ? 2 : 1); ++i) reinterpret_cast<uint4 *>(to)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     } else {
-        for (int i = 0; i < 8; ++i)
-            if (k + i < K) to[i] = from_float<DT>((float) from[i] * s);
+        __builtin_memcpy(to, w, sizeof(w));
     }
 }
 
@@ -150,10 +181,10 @@ __global__ __launch_bounds__(256) void rq_weight_prepare_kernel(const uint8_t *w
             if constexpr (VEC) {
                 const uint4 u = *reinterpret_cast<const uint4 *>(p);
                 v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+            } else if (b + 16 <= L.row_bytes) {
+                load_bytes(v, p);
             } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (b + j < L.row_bytes) v[j >> 2] |= (uint32_t) p[j] << (8 * (j & 3));
+                for (int j = 0; b + j < L.row_bytes; ++j) v[j >> 2] |= (uint32_t) p[j] << (8 * (j & 3));
             }
         }
         reinterpret_cast<uint4 *>(to)[i] = make_uint4(v[0], v[1], v[2], v[3]);
@@ -169,15 +200,17 @@ __global__ __launch_bounds__(256) void rq_pack_kernel(const uint8_t *x, int64_t 
     if (m >= M) return;
     const uint8_t *p = x + m * ld + b;
     uint32_t       v[4] = { 0, 0, 0, 0 };
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (b + j < row_bytes) v[j >> 2] |= (uint32_t) p[j] << (8 * (j & 3));
+    if (b + 16 <= row_bytes) {
+        load_bytes(v, p);
+    } else {
+        for (int j = 0; b + j < row_bytes; ++j) v[j >> 2] |= (uint32_t) p[j] << (8 * (j & 3));
+    }
     *reinterpret_cast<uint4 *>(to + m * pitch + b) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 constexpr int64_t kGrid = 1ll << 23;   // workgroups of a launch (of up to 512 threads, of which a grid has under 2^32)
 
-template <int DT, bool VEC, int G>
+template <int DT, bool VEC, int G, int U>
 hipError_t quantize_rows(const void *x_, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded, float *scales,
                          int *zero, int zeros, hipStream_t stream) {
     constexpr int kRows = G < 256 ? 256 / G : 1;
@@ -185,24 +218,27 @@ hipError_t quantize_rows(const void *x_, int64_t ldx, int64_t M, int64_t K, uint
     const auto   *x = reinterpret_cast<const typename Element<DT>::type *>(x_);
     for (int64_t m = 0; m < M; m += kMost) {
         const int64_t rows = M - m < kMost ? M - m : kMost;
-        hipLaunchKernelGGL((rq_i8_quantize_kernel<DT, VEC, G>), dim3((unsigned) ((rows + kRows - 1) / kRows)), dim3(G < 256 ? 256 : G), 0, stream,
+        hipLaunchKernelGGL((rq_i8_quantize_kernel<DT, VEC, G, U>), dim3((unsigned) ((rows + kRows - 1) / kRows)), dim3(G < 256 ? 256 : G), 0, stream,
                            x + m * ldx, ldx, rows, K, codes + m * pitch, pitch, padded, scales + m, zero, m ? 0 : zeros);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
+template <int DT, bool VEC>
+hipError_t quantize(const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded, float *scales,
+                    int *zero, int zeros, hipStream_t stream) {
+    if (K <= 2048) return quantize_rows<DT, VEC, 64, 4>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    if (K <= 8192) return quantize_rows<DT, VEC, 256, 4>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    return quantize_rows<DT, VEC, 512, 4>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+}
 template <int DT>
 hipError_t quantize(const void *x, int64_t ldx, int64_t M, int64_t K, uint8_t *codes, int64_t pitch, int64_t padded, float *scales,
                     int *zero, int zeros, hipStream_t stream) {
     const int  size = DT == RQ_F32 ? 4 : 2;
     const bool vec = (uintptr_t) x % 16 == 0 && (M == 1 || ldx * size % 16 == 0) && K % 8 == 0 && (uintptr_t) codes % 8 == 0;
-    if (K <= 2048) return vec ? quantize_rows<DT, true, 64>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
-                              : quantize_rows<DT, false, 64>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
-    if (K <= 8192) return vec ? quantize_rows<DT, true, 256>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
-                              : quantize_rows<DT, false, 256>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
-    return vec ? quantize_rows<DT, true, 512>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
-               : quantize_rows<DT, false, 512>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
+    return vec ? quantize<DT, true>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream)
+               : quantize<DT, false>(x, ldx, M, K, codes, pitch, padded, scales, zero, zeros, stream);
 }
 
 template <int DT>

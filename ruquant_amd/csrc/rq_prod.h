@@ -79,8 +79,8 @@ template <> struct Matrix<RQ_F16> {
 struct ProductArgs {
     Panels         L;
     const uint8_t *w;              // prepared
-    const uint8_t *x;              // rows of x, on multiples of 16 bytes
-    int64_t        pitch, x_bytes; // of a row: distance, and how many there are to read (a multiple of 16; zeros behind them)
+    const uint8_t *x;              // rows of x; for the tiles on multiples of 16 bytes
+    int64_t        pitch, x_bytes; // of a row: distance, and how many there are to read (for the tiles a multiple of 16), with zeros behind them
     int64_t        K;              // launch_stream where it rounds: x is the call's own, `pitch` its row stride in elements, rows of K;
     bool           aligned;        //   whether they are on multiples of 16 bytes, and K of eight;
     int            chunk;          //   up to so many rows at a time (16 where it does not round)
@@ -148,6 +148,11 @@ __device__ __forceinline__ bool find_group(const ProductArgs &a, int want, F uni
     total_ = before;
     return found;
 }
+
+// ---- loads and stores at any address (the card takes them, in pieces where they cross lines) ------------------
+template <int N>
+__device__ __forceinline__ void load_bytes(uint32_t (&w)[N], const void *p) { __builtin_memcpy(w, p, N * 4); }
+__device__ __forceinline__ void store_bytes(void *p, const uint2 &v) { __builtin_memcpy(p, &v, 8); }
 
 // ---- rounding of a row to int8 ------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {

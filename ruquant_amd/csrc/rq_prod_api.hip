@@ -23,7 +23,7 @@ size_t  act_bytes(int weight_type, int64_t K, int64_t M) { return pad256(M * pac
 
 // Sets a's rows of x; launches what brings them there, and zeros to a.arrived.
 hipError_t take_rows(ProductArgs &a, int weight_type, int64_t K, int in_dtype, const void *x, int64_t ldx, const float *x_scales, int64_t M,
-                     int counters, uint8_t *workspace, hipStream_t stream) {
+                     bool few, int counters, uint8_t *workspace, hipStream_t stream) {
     a.M = M, a.chunk = 16;
     const int64_t row_bytes = K * type_bytes(weight_type), pitch = packed_pitch(weight_type, K), padded = packed_bytes(weight_type, K);
     if (weight_type == RQ_I8 && in_dtype != RQ_I8) {
@@ -33,7 +33,7 @@ hipError_t take_rows(ProductArgs &a, int weight_type, int64_t K, int in_dtype, c
     }
     a.x_scales = x_scales;
     const int64_t ld_bytes = ldx * type_bytes(in_dtype);
-    if (aligned(x, 16) && (M == 1 || ld_bytes % 16 == 0) && row_bytes % 16 == 0) {
+    if (few || (aligned(x, 16) && (M == 1 || ld_bytes % 16 == 0) && row_bytes % 16 == 0)) {
         a.x = (const uint8_t *) x, a.pitch = ld_bytes, a.x_bytes = row_bytes;
         return counters ? launch_pack(nullptr, 0, 0, 0, nullptr, 16, a.arrived, counters, stream) : hipSuccess;
     }
@@ -161,7 +161,7 @@ int run(ProductArgs &a, const Plan &plan, int weight_type, int64_t K, int in_dty
     uint8_t *behind = workspace + rows;
     a.sums = (uint32_t *) behind;
     a.arrived = (int *) (behind + plan.sums_bytes);
-    const hipError_t e = take_rows(a, weight_type, K, in_dtype, x, ldx, x_scales, M, plan.counters, workspace, stream);
+    const hipError_t e = take_rows(a, weight_type, K, in_dtype, x, ldx, x_scales, M, plan.few, plan.counters, workspace, stream);
     return e != hipSuccess ? e : launch_product(plan, weight_type, a, stream);
 }
 

@@ -16,22 +16,25 @@ __device__ __attribute__((aligned(16))) const uint8_t kZeros[16] = { 0 };
 template <int DT>
 __device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, bool aligned, int K, int k, float (&v)[8]) {
     using T = typename Element<DT>::type;
-    if (aligned) {   // (on 16 bytes, and K a multiple of eight)
-        if constexpr (DT == RQ_F32) {
-            const float4 a = reinterpret_cast<const float4 *>(x + k)[0], b = reinterpret_cast<const float4 *>(x + k)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4    u = *reinterpret_cast<const uint4 *>(x + k);
-            const uint32_t w[4] = { u.x, u.y, u.z, u.w };
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = to_float(__builtin_bit_cast(T, (uint16_t) w[i]));
-                v[2 * i + 1] = to_float(__builtin_bit_cast(T, (uint16_t) (w[i] >> 16)));
-            }
-        }
-    } else {
+    uint32_t w[DT == RQ_F32 ? 8 : 4];
+    if (k + 8 > K) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_float(x[k + i]) : 0.0f;
+        return;
+    }
+    if (aligned) {   // (on 16 bytes)
+#pragma unroll
+        for (int i = 0; i < (DT == RQ_F32 ? 2 : 1); ++i) {
+            const uint4 u = reinterpret_cast<const uint4 *>(x + k)[i];
+            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        }
+    } else {
+        load_bytes(w, x + k);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (DT == RQ_F32) v[i] = __uint_as_float(w[i]);
+        else v[i] = to_float(__builtin_bit_cast(T, (uint16_t) (i & 1 ? w[i >> 1] >> 16 : w[i >> 1])));
     }
 }
 
@@ -68,14 +71,31 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
         v4i       A[DEPTH][NR], B[kRound ? 1 : DEPTH];
         Acc4      acc[NR];
         const uint8_t *x = lds + min(col, T - 1) * pitch + quarter * 16;   // (columns past the rows repeat the last one)
+        uint32_t       tail[4] = { 0, 0, 0, 0 };   // the row's bytes behind its last 16th, zeros behind them
         if constexpr (!kRound) {
             const int64_t row = row_read(a, first + t0 + min(col, T - 1));
-            x = a.x + (row < 0 ? 0 : row) * a.pitch + quarter * 16;
+            x = a.x + (row < 0 ? 0 : row) * a.pitch;
+            if (a.x_bytes & 15)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < (a.x_bytes & 15)) tail[j >> 2] |= (uint32_t) x[(a.x_bytes & ~15ll) + j] << (8 * (j & 3));
         }
         auto load = [&](int i, int s) __attribute__((always_inline)) {
 #pragma unroll
             for (int r = 0; r < NR; ++r) A[i][r] = *reinterpret_cast<const v4i *>(from[r] + (int64_t) s * 2048);
-            if constexpr (!kRound) B[i] = *reinterpret_cast<const v4i *>(s * 64 + quarter * 16 < a.x_bytes ? x + s * 64 : kZeros);
+            if constexpr (!kRound) {   // (a row's last bytes end anywhere, and behind them is another's memory)
+                uint32_t w[4];
+                load_bytes(w, a.x_bytes < 16 ? kZeros : x + min(s * 64 + quarter * 16, (int) a.x_bytes - 16));
+                B[i] = v4i{ (int) w[0], (int) w[1], (int) w[2], (int) w[3] };
+            }
+        };
+        // what was loaded, or the row's last bytes and zeros (looked at where it is used: a load that is looked at is waited for)
+        auto whole = [&](const v4i &v, int s) __attribute__((always_inline)) {
+            const int at = s * 64 + quarter * 16;
+            v4i       r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = at + 16 <= a.x_bytes ? v[j] : at < a.x_bytes ? (int) tail[j] : 0;
+            return r;
         };
         if constexpr (kRound) {
             using X = typename Element<DT>::type;
@@ -152,7 +172,7 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
 #pragma unroll
             for (int i = 0; i < DEPTH; ++i) {
                 if (s + i < s1) {
-                    const v4i b = kRound ? *reinterpret_cast<const v4i *>(x + (s + i) * 64) : B[kRound ? 0 : i];
+                    const v4i b = kRound ? *reinterpret_cast<const v4i *>(x + (s + i) * 64) : whole(B[kRound ? 0 : i], s + i);
 #pragma unroll
                     for (int r = 0; r < NR; ++r) acc[r] = Matrix<WT>::mfma16(A[i][r], b, acc[r]);
                     if (s + i + DEPTH < s1) load(i, s + i + DEPTH);

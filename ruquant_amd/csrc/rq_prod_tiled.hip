@@ -218,7 +218,7 @@ __device__ __forceinline__ int place_of(int index, int total) {
 // not depend on who is last. The sums go past the XCDs' caches (atomic stores and loads of the device's scope) and are waited for before the count, so
 // who sees the last count sees all sums.
 template <int WT, int RB, int TB, int WR, int WC, int S, int RA, bool GROUPED, bool SPLIT>
-__global__ __launch_bounds__(64 * WR * WC, 2) void rq_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles,
+__global__ __launch_bounds__(64 * WR * WC, RB * TB > 8 ? 1 : 2) void rq_tiled_kernel(const ProductArgs a, const int row_tiles, const int token_tiles,
                                                                                                  const int across) {
     using G = Tiled<WT, RB, TB, WR, WC, S, RA>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];

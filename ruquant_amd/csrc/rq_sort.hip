@@ -1,8 +1,10 @@
 // Sort of slots by expert: a stable counting sort, so that it is the same every time.
 //
-// Slots go in runs of kRun. A wavefront ranks 64 slots among those of the same expert by comparing the bits of their ids across its lanes, and
-// adds them to its run's count of that expert in one step. One run is one launch; more are counted by a launch in front, and every run then adds up
-// the counts of those in front of it, which are few and lie in the caches.
+// A workgroup has a run of slots, a wavefront some rows of 64 of them, whose ids its lanes keep. A wavefront ranks 64 slots among those of the same
+// expert by comparing the bits of their ids across its lanes, and adds them to its count of that expert in one step. One run is one launch; more are
+// counted by a launch in front, and every run then adds up the counts of all, which are few and lie in the caches.
+#include <type_traits>
+
 #include "rq_prod.h"
 
 namespace rq {
@@ -13,7 +15,7 @@ constexpr int kSortThreads = 1024, kWaves = kSortThreads / 64;
 
 struct SortArgs {
     const int32_t *ids;
-    int            slots, top, E, run;   // run: slots of a workgroup
+    int            slots, top, E;
     int32_t       *offsets, *slots_out, *tokens;
     int           *counts;               // [run][E + 1]
 };
@@ -33,14 +35,28 @@ __device__ __forceinline__ int expert_of(const SortArgs &a, int i) {
     return e >= 0 && e < a.E ? e : a.E;
 }
 
+// The ids of this wavefront's slots: row k of 64 begins at first + 64 k. Behind the last slot a number that no expert has.
+constexpr int kNone = 0x7FF;
+template <int PER>
+__device__ __forceinline__ int load_experts(const SortArgs &a, int (&e)[PER]) {
+    const int first = ((int) blockIdx.x * kWaves + ((int) threadIdx.x >> 6)) * 64 * PER, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) e[k] = first + 64 * k + lane < a.slots ? expert_of(a, first + 64 * k + lane) : kNone;
+    return first;
+}
+
+template <int PER>
 __global__ __launch_bounds__(kSortThreads) void rq_sort_count_kernel(const SortArgs a) {
     __shared__ int count[RQ_GROUPED_MAX_E + 1];
-    for (int e = threadIdx.x; e <= a.E; e += kSortThreads) count[e] = 0;
+    int            e[PER];
+    load_experts<PER>(a, e);
+    for (int i = threadIdx.x; i <= a.E; i += kSortThreads) count[i] = 0;
     __syncthreads();
-    const int i0 = blockIdx.x * a.run, i1 = min(i0 + a.run, a.slots);
-    for (int i = i0 + (int) threadIdx.x; i < i1; i += kSortThreads) atomicAdd(&count[expert_of(a, i)], 1);
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (e[k] != kNone) atomicAdd(&count[e[k]], 1);
     __syncthreads();
-    for (int e = threadIdx.x; e <= a.E; e += kSortThreads) a.counts[blockIdx.x * (a.E + 1) + e] = count[e];
+    for (int i = threadIdx.x; i <= a.E; i += kSortThreads) a.counts[blockIdx.x * (a.E + 1) + i] = count[i];
 }
 
 // Sum over the threads up to this one; all of the workgroup take part.
@@ -58,31 +74,43 @@ __device__ __forceinline__ int scan(int v, int *waves) {
 }
 
 // COUNTED: a.counts holds what every run has of every expert; otherwise there is one run. at[w][e]: where wavefront w's next slot of expert e goes.
-// A wavefront has a row of 64 slots after the other, its share of the run.
-template <bool COUNTED>
+template <int PER, bool COUNTED>
 __global__ __launch_bounds__(kSortThreads) void rq_sort_place_kernel(const SortArgs a) {
-    extern __shared__ int at[];   // [kWaves][E + 1]
+    extern __shared__ int at[];   // [kWaves][E + 1]; COUNTED: then [2][E + 1], all slots of an expert, and those of the runs in front
     __shared__ int waves[kWaves], behind;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, E1 = a.E + 1;
-    for (int i = t; i < kWaves * E1; i += kSortThreads) at[i] = 0;
+    int      *sums = at + kWaves * E1;
+    int       e[PER];
+    const int first = load_experts<PER>(a, e);
+    for (int i = t; i < (COUNTED ? kWaves + 2 : kWaves) * E1; i += kSortThreads) at[i] = 0;
     __syncthreads();
-    const int i0 = blockIdx.x * a.run, i1 = min(i0 + a.run, a.slots);
-    const int share = ((i1 - i0 + kWaves - 1) / kWaves + 63) & ~63;
-    const int w0 = min(i0 + wave * share, i1), w1 = min(w0 + share, i1);
-    for (int i = w0 + lane; i < w1; i += 64) atomicAdd(&at[wave * E1 + expert_of(a, i)], 1);
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (e[k] != kNone) atomicAdd(&at[wave * E1 + e[k]], 1);
+    if constexpr (COUNTED) {   // the runs in as many shares as the threads have columns for, eight loads on their way in each
+        const int stride = (E1 + 63) & ~63, shares = max(1, kSortThreads / stride), runs = gridDim.x;
+        for (int i = t; i < shares * stride; i += kSortThreads) {
+            const int share = i / stride, c = i - share * stride, r1 = runs * (share + 1) / shares;
+            if (c >= E1) continue;
+            int all = 0, front = 0;
+            for (int r = runs * share / shares; r < r1; r += 8) {
+                int n[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) n[k] = r + k < r1 ? a.counts[(r + k) * E1 + c] : 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) all += n[k], front += r + k < (int) blockIdx.x ? n[k] : 0;
+            }
+            atomicAdd(&sums[c], all);
+            atomicAdd(&sums[E1 + c], front);
+        }
+    }
     __syncthreads();
     // expert t: how many slots there are, how many of them in the runs in front, and in this run's wavefronts
-    int all = 0, front = 0;
+    int all = 0;
     if (t < a.E) {
-        if constexpr (COUNTED) {
-            for (int r = 0; r < (int) gridDim.x; ++r) {
-                const int c = a.counts[r * E1 + t];
-                all += c;
-                front += r < (int) blockIdx.x ? c : 0;
-            }
-        } else {
+        if constexpr (COUNTED) all = sums[t];
+        else
             for (int w = 0; w < kWaves; ++w) all += at[w * E1 + t];
-        }
     }
     const int end = scan(all, waves);   // (E <= 1024 = the threads)
     if (t == kSortThreads - 1) behind = end;
@@ -91,34 +119,23 @@ __global__ __launch_bounds__(kSortThreads) void rq_sort_place_kernel(const SortA
         if (t == 0) a.offsets[0] = 0;
     }
     __syncthreads();
-    if (t < a.E) {
-        int to = end - all + front;
+    for (int c = t; c < E1; c += kSortThreads) {   // (column E: the slots of no expert, behind all others)
+        int to = (c < a.E ? end - all : behind) + (COUNTED ? sums[E1 + c] : 0);
         for (int w = 0; w < kWaves; ++w) {
-            const int c = at[w * E1 + t];
-            at[w * E1 + t] = to;
-            to += c;
-        }
-    }
-    if (t == 0) {   // the slots of no expert: behind all others, as many in front of this run as its slots less those that have one
-        int to = behind;
-        if constexpr (COUNTED)
-            for (int r = 0; r < (int) blockIdx.x; ++r) to += a.counts[r * E1 + a.E];
-        for (int w = 0; w < kWaves; ++w) {
-            const int c = at[w * E1 + a.E];
-            at[w * E1 + a.E] = to;
-            to += c;
+            const int n = at[w * E1 + c];
+            at[w * E1 + c] = to;
+            to += n;
         }
     }
     __syncthreads();
-    for (int i = w0; i < w1; i += 64) {   // (this wavefront alone has its row of `at`)
-        const bool     there = i + lane < w1;
-        const int      e = there ? expert_of(a, i + lane) : 0x7FF;   // (a number that no expert has)
-        const uint64_t same = peers(e), below = same & ((1ull << lane) - 1);
-        if (there) {
-            int      *cell = &at[wave * E1 + e];
-            const int p = *cell + __builtin_popcountll(below);
-            a.slots_out[p] = i + lane;
-            a.tokens[p] = (i + lane) / a.top;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {   // (this wavefront alone has its row of `at`)
+        const uint64_t same = peers(e[k]), below = same & ((1ull << lane) - 1);
+        if (e[k] != kNone) {
+            int      *cell = &at[wave * E1 + e[k]];
+            const int p = *cell + __builtin_popcountll(below), i = first + 64 * k + lane;
+            a.slots_out[p] = i;
+            a.tokens[p] = i / a.top;
             __builtin_amdgcn_wave_barrier();
             if (below == 0) *cell = p + __builtin_popcountll(same);
             __builtin_amdgcn_wave_barrier();
@@ -127,12 +144,10 @@ __global__ __launch_bounds__(kSortThreads) void rq_sort_place_kernel(const SortA
 }
 
 constexpr int64_t kMaxSlots = 1 << 22;
-constexpr int     kOneRun = 8192;
-// Runs of at least kOneRun slots, at most 256 of them.
-int run_of(int64_t slots) {
-    const int64_t each = up_to((slots + 255) / 256, kSortThreads);
-    return (int) (each > kOneRun ? each : kOneRun);
-}
+// Rows of 64 slots that a wavefront has: short runs (2048 slots) where they are few.
+constexpr int kShort = 2, kLong = 8;
+constexpr int run_of(int per) { return kSortThreads * per; }
+int           rows_of(int64_t slots) { return slots <= 64 * run_of(kShort) ? kShort : kLong; }
 bool good(int64_t M, int top, int64_t E) {
     return M >= 0 && top >= 1 && top <= 1024 && M <= kMaxSlots / top && E >= 1 && E <= RQ_GROUPED_MAX_E;
 }
@@ -145,8 +160,11 @@ using namespace rq::prod;
 
 extern "C" size_t rq_sort_workspace_bytes(int64_t M, int top, int64_t E) {
     if (!good(M, top, E)) return 0;
-    const int64_t slots = M * top, run = run_of(slots), runs = (slots + run - 1) / run;
-    return runs <= 1 ? 0 : (size_t) up_to(runs * (E + 1) * 4, 256);
+    // (as many runs as the call's or any smaller one's, so that it grows)
+    const int64_t slots = M * top;
+    if (slots <= run_of(kShort)) return 0;
+    const int64_t few = slots < 64 * run_of(kShort) ? slots : 64 * run_of(kShort), a = (few + run_of(kShort) - 1) / run_of(kShort), b = (slots + run_of(kLong) - 1) / run_of(kLong);
+    return (size_t) up_to((a > b ? a : b) * (E + 1) * 4, 256);
 }
 
 extern "C" int rq_sort_slots(const int32_t *ids, int64_t M, int top, int64_t E, int32_t *offsets, int32_t *slots, int32_t *tokens,
@@ -156,21 +174,24 @@ extern "C" int rq_sort_slots(const int32_t *ids, int64_t M, int top, int64_t E, 
     if (!offsets || !aligned4(offsets) || (M > 0 && (!ids || !slots || !tokens || !aligned4(ids) || !aligned4(slots) || !aligned4(tokens)))) return RQ_E_ARGUMENT;
     const size_t need = rq_sort_workspace_bytes(M, top, E);
     if (need && (!workspace || (uintptr_t) workspace % 256 || workspace_bytes < need)) return RQ_E_WORKSPACE;
-    const int      n = (int) (M * top), run = run_of(n), runs = n ? (n + run - 1) / run : 1;
-    const SortArgs a = { ids, n, top, (int) E, run, offsets, slots, tokens, (int *) workspace };
-    const int      bytes = kWaves * ((int) E + 1) * (int) sizeof(int);
-    static std::atomic<uint64_t> allowed[2];
-    const void *kernels[2] = { reinterpret_cast<const void *>(rq_sort_place_kernel<false>), reinterpret_cast<const void *>(rq_sort_place_kernel<true>) };
-    const int   counted = runs > 1;
-    hipError_t  e = allow_lds(kernels[counted], kWaves * (RQ_GROUPED_MAX_E + 1) * (int) sizeof(int), allowed[counted]);
-    if (e != hipSuccess) return e;
-    if (counted) {
-        hipLaunchKernelGGL(rq_sort_count_kernel, dim3(runs), dim3(kSortThreads), 0, (hipStream_t) stream, a);
-        e = hipGetLastError();
+    const int      n = (int) (M * top), per = rows_of(n), runs = n ? (n + run_of(per) - 1) / run_of(per) : 1;
+    const SortArgs a = { ids, n, top, (int) E, offsets, slots, tokens, (int *) workspace };
+    auto           run = [&](auto rows) {
+        constexpr int PER = decltype(rows)::value;
+        static std::atomic<uint64_t> allowed[2];
+        const void *kernels[2] = { reinterpret_cast<const void *>(rq_sort_place_kernel<PER, false>), reinterpret_cast<const void *>(rq_sort_place_kernel<PER, true>) };
+        const int   counted = runs > 1, bytes = (kWaves + 2 * counted) * ((int) E + 1) * (int) sizeof(int);
+        hipError_t  e = allow_lds(kernels[counted], (kWaves + 2) * (RQ_GROUPED_MAX_E + 1) * (int) sizeof(int), allowed[counted]);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(rq_sort_place_kernel<true>, dim3(runs), dim3(kSortThreads), bytes, (hipStream_t) stream, a);
-    } else {
-        hipLaunchKernelGGL(rq_sort_place_kernel<false>, dim3(1), dim3(kSortThreads), bytes, (hipStream_t) stream, a);
-    }
-    return hipGetLastError();
+        if (counted) {
+            hipLaunchKernelGGL(rq_sort_count_kernel<PER>, dim3(runs), dim3(kSortThreads), 0, (hipStream_t) stream, a);
+            e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            hipLaunchKernelGGL((rq_sort_place_kernel<PER, true>), dim3(runs), dim3(kSortThreads), bytes, (hipStream_t) stream, a);
+        } else {
+            hipLaunchKernelGGL((rq_sort_place_kernel<PER, false>), dim3(1), dim3(kSortThreads), bytes, (hipStream_t) stream, a);
+        }
+        return hipGetLastError();
+    };
+    return per == kShort ? run(std::integral_constant<int, kShort>{}) : run(std::integral_constant<int, kLong>{});
 }
