@@ -116,37 +116,49 @@ __device__ __forceinline__ void group(const ProductArgs &a, int e, int &first, i
     first = min(max(a.offsets[e], 0), P);
     count = max(min(a.offsets[e + 1], P) - first, 0);
 }
-// Of the groups, which one has the unit `want` (a uniform number) if group e has units(its count) of them, and the place in it; all lanes
-// of a wavefront take part. Returns false (group and place left) if there are fewer. total: all units.
-template <typename F>
-__device__ __forceinline__ bool find_group(const ProductArgs &a, int want, F units, int &e_, int &first_, int &count_, int &place_, int &total_) {
+// Group e has units(its count) units, and all groups' stand in a row. Finds the group that has unit want(how many there are), and the place in it; all lanes
+// of a wavefront take part, with the same numbers. False where no group has it. TOTAL: `want` looks at its argument (else it is 0).
+template <bool TOTAL, typename U, typename W>
+__device__ __forceinline__ bool find_group(const ProductArgs &a, U units, W want, int &e_, int &first_, int &count_, int &place_) {
     const int lane = threadIdx.x & 63;
-    int       before = 0;
-    bool      found = false;
-    for (int e0 = 0; e0 < a.E; e0 += 64) {
-        int first = 0, count = 0;
+    auto      scan = [&](int e0, int &first, int &count, int &mine) __attribute__((always_inline)) {   // of 64 groups: the units up to this lane's last
+        first = count = 0;
         if (e0 + lane < a.E) group(a, e0 + lane, first, count);
-        const int mine = units(count);
-        int       sum = mine;
+        mine = units(count);
+        int sum = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int u = __shfl_up(sum, o);
             if (lane >= o) sum += u;
         }
-        const int      from = before + sum - mine;
-        const uint64_t here = __ballot(want >= from && want < from + mine);
-        if (here) {
-            const int l = __builtin_ctzll(here);
-            e_ = e0 + l;
-            first_ = __builtin_amdgcn_readlane(first, l);
-            count_ = __builtin_amdgcn_readlane(count, l);
-            place_ = want - __builtin_amdgcn_readlane(from, l);
-            found = true;
-        }
+        return sum;
+    };
+    int  first, count, mine, wanted = 0;
+    auto found = [&](int e0, int from) __attribute__((always_inline)) {
+        const uint64_t here = __ballot(wanted >= from && wanted < from + mine);
+        if (!here) return false;
+        const int l = __builtin_ctzll(here);
+        e_ = e0 + l;
+        first_ = __builtin_amdgcn_readlane(first, l);
+        count_ = __builtin_amdgcn_readlane(count, l);
+        place_ = wanted - __builtin_amdgcn_readlane(from, l);
+        return true;
+    };
+    if (a.E <= 64) {
+        const int sum = scan(0, first, count, mine);
+        wanted = want(__builtin_amdgcn_readlane(sum, 63));
+        return found(0, sum - mine);
+    }
+    int total = 0;
+    if (TOTAL)
+        for (int e0 = 0; e0 < a.E; e0 += 64) total += __builtin_amdgcn_readlane(scan(e0, first, count, mine), 63);
+    wanted = want(total);
+    for (int e0 = 0, before = 0; e0 < a.E; e0 += 64) {
+        const int sum = scan(e0, first, count, mine);
+        if (found(e0, before + sum - mine)) return true;
         before += __builtin_amdgcn_readlane(sum, 63);
     }
-    total_ = before;
-    return found;
+    return false;
 }
 
 // ---- loads and stores at any address (the card takes them, in pieces where they cross lines) ------------------

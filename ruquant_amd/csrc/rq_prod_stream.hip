@@ -51,8 +51,8 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
     int       e = 0, first = 0, count = (int) a.P;
     if constexpr (GROUPED) {
-        int place, total;
-        if (!find_group(a, (int) blockIdx.y, [](int n) { return n > 0 ? 1 : 0; }, e, first, count, place, total)) return;
+        int place;
+        if (!find_group<false>(a, [](int n) { return n > 0 ? 1 : 0; }, [](int) { return (int) blockIdx.y; }, e, first, count, place)) return;
     }
     const int      unit0 = blockIdx.x * NR, steps = a.L.steps;
     const int      s0 = steps * wave / W, s1 = steps * (wave + 1) / W;

@@ -230,11 +230,11 @@ __global__ __launch_bounds__(64 * WR * WC, RB * TB > 8 ? 1 : 2) void rq_tiled_ke
         // and read the weight together.
         constexpr int T = G::kTileTokens;
         auto units = [&](int n) { return (n + T - 1) / T * row_tiles * splits; };
-        int  gfirst, gcount, place, total;
-        find_group(a, -1, units, e, gfirst, gcount, place, total);
-        if (index >= total) return;
-        v = place_of(index, total);
-        if (!find_group(a, v, units, e, gfirst, gcount, place, total)) return;
+        int  gfirst, gcount, place;
+        v = -1;
+        auto mine = [&](int total) { return index < total ? v = place_of(index, total) : -1; };
+        if (!find_group<true>(a, units, mine, e, gfirst, gcount, place)) return;
+        if (v / splits >= row_tiles * token_tiles) return;   // (more than there can be: the offsets overlap)
         place /= splits;
         const int tiles = (gcount + T - 1) / T, tile = place % tiles;
         row_tile = place / tiles;
@@ -283,14 +283,10 @@ __global__ __launch_bounds__(64 * WR * WC, RB * TB > 8 ? 1 : 2) void rq_tiled_ke
         const int64_t row = row_read(a, first + at);
         g.b_src[i] = a.x + (row < 0 ? 0 : row) * a.pitch + (int64_t) step0 * 64 + ((g.lane & 7) ^ ((run & 1) * 4 + (g.lane >> 4))) * 16;
     }
-    if (g.wc * TB * 32 < count) g.template loop<true>();
-    else g.template loop<false>();
-
-    // 32 positions x 64 rows at a time through LDS (a region of the wavefront's own), in the output's type, so that a position's outputs
-    // leave as whole lines and LDS moves no more than they are.
+    // Which rows the outputs are, asked before the products (a position a lane; y's rows are fewer than 2^31).
     const int    lane = g.lane, wr = g.wr, wc = g.wc;
     const float *t_scales = reinterpret_cast<const float *>(w + a.L.code_bytes);
-    int          out_at[TB];   // (a position a lane; y's rows are fewer than 2^31)
+    int          out_at[TB];
     float        s_m[TB];      // of int8
     bool         in_there[TB];
 #pragma unroll
@@ -305,6 +301,11 @@ __global__ __launch_bounds__(64 * WR * WC, RB * TB > 8 ? 1 : 2) void rq_tiled_ke
                 if (row >= 0) s_m[t] = a.x_scales[row];
         }
     }
+    if (wc * TB * 32 < count) g.template loop<true>();
+    else g.template loop<false>();
+
+    // 32 positions x 64 rows at a time through LDS (a region of the wavefront's own), in the output's type, so that a position's outputs
+    // leave as whole lines and LDS moves no more than they are.
     barrier();   // (the ring is not read any more)
     if (wc * TB * 32 >= count) return;
     if constexpr (SPLIT) {
@@ -352,18 +353,24 @@ __global__ __launch_bounds__(64 * WR * WC, RB * TB > 8 ? 1 : 2) void rq_tiled_ke
         static_assert(RB % kTwo == 0, "row blocks in pairs");
         T *mine = reinterpret_cast<T *>(lds + g.wave * 32 * G::kStride * 4);
 #pragma unroll
-        for (int t = 0; t < TB; ++t) {
+        for (int r = 0; r < RB; r += kTwo) {
+            v4f tn[WT == RQ_I8 ? 4 * kTwo : 1];   // the scales of these rows
+            if constexpr (WT == RQ_I8) {
 #pragma unroll
-            for (int r = 0; r < RB; r += kTwo) {
+                for (int q = 0; q < 4 * kTwo; ++q) {
+                    const int block = min(block0 + wr * RB + r + q / 4, a.L.row_blocks - 1);
+                    tn[q] = *reinterpret_cast<const v4f *>(t_scales + block * 32 + q % 4 * 8 + (lane >> 5) * 4);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
 #pragma unroll
                 for (int q = 0; q < 4 * kTwo; ++q) {
                     const auto &c = g.acc[r + q / 4][t];
                     v4f         v;
                     if constexpr (WT == RQ_I8) {
-                        const int block = min(block0 + wr * RB + r + q / 4, a.L.row_blocks - 1);
-                        const v4f tn = *reinterpret_cast<const v4f *>(t_scales + block * 32 + q % 4 * 8 + (lane >> 5) * 4);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = (float) c[q % 4 * 4 + i] * tn[i] * s_m[t];
+                        for (int i = 0; i < 4; ++i) v[i] = (float) c[q % 4 * 4 + i] * tn[q][i] * s_m[t];
                     } else {
                         v = v4f{ c[q % 4 * 4], c[q % 4 * 4 + 1], c[q % 4 * 4 + 2], c[q % 4 * 4 + 3] };
                     }
