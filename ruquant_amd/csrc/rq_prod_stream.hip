@@ -1,9 +1,13 @@
 // Products of few rows a group (int8, or grouped by expert): weights from memory into registers.
 //
-// A call of this size is the stream of its weights. A workgroup has 32 rows of one weight (or 16) and up to 16 rows of x at a time; its wavefronts
+// A call of this size is the stream of its weights. A workgroup has 32 rows of one weight and up to 16 rows of x at a time; its wavefronts
 // split the row's bytes, each with DEPTH steps of 64 bytes on their way, and join their sums in LDS in their order. Rows of x that are still to be
-// rounded are rounded by every workgroup for itself, into LDS, while its first weights are on their way: a launch in front costs more from some hundred
-// workgroups down to few rows.
+// rounded are rounded by every workgroup for itself, into LDS, while its first weights are on their way: that saves a launch, where the rows are few.
+//
+// Bound by memory where weights are large, by the chain of a load, the products and the join where they are not: one token x 5120 x 17408 in int8 17.3 us, 89 MB
+// at 5.1 TB/s, a large copy's rate; 13 x 4099 x 5121 10.3 us; 37 tokens' 111 rows of 1376 x 4096
+// in fp16, from most of 60 experts' 676 MB, 83 us. Tried:
+// 16 wavefronts (2.4 times as long), 16 rows (more steps on their way, 10 to 60 % longer), 64 rows (as fast for groups, 10 to 25 % longer for one).
 #include "rq_prod.h"
 
 namespace rq {
@@ -220,7 +224,9 @@ hipError_t stream(const ProductArgs &a, hipStream_t s) {
     const int64_t  units = (a.L.N + 15) / 16;
     const unsigned groups = GROUPED ? (unsigned) (a.P < a.E ? a.P : a.E) : 1;
     constexpr bool kRound = DT != RQ_I8;
-    if (units * groups > 768) {
+    // Eight wavefronts a workgroup up to one workgroup a compute unit, four beyond. (us, eight -> four: one row of int8, K = 5120: N = 6592 9.9 -> 10.6, 8192 11.4 -> 11.6,
+    // 12000 18.7 -> 15.9, 17408 22.8 -> 20.3; 6, 8 and 10 groups of one row, N = 1280 10.2 -> 10.8, 15.8 -> 12.6, 16.6 -> 16.6; bf16, 8 groups 22.6 -> 19.6)
+    if (units * groups > 512) {
         hipLaunchKernelGGL((rq_stream_kernel<WT, DT, 4, 2, 4, GROUPED>), dim3((unsigned) ((units + 1) / 2), groups), dim3(256), lds_bytes(4, 2, kRound, a), s, a);
     } else {
         hipLaunchKernelGGL((rq_stream_kernel<WT, DT, 8, 2, 6, GROUPED>), dim3((unsigned) ((units + 1) / 2), groups), dim3(512), lds_bytes(8, 2, kRound, a), s, a);

@@ -2,7 +2,8 @@
 //
 // A workgroup has a run of slots, a wavefront some rows of 64 of them, whose ids its lanes keep. A wavefront ranks 64 slots among those of the same
 // expert by comparing the bits of their ids across its lanes, and adds them to its count of that expert in one step. One run is one launch; more are
-// counted by a launch in front, and every run then adds up the counts of all, which are few and lie in the caches.
+// counted by a launch in front, and every run then adds up the counts of all, which are few and lie in the caches. 131072 slots of 256 experts 2.9 + 9.3 us, 8 slots 3.0:
+// the chain of the ids' load, the counts, their sum over the wavefronts and experts, and the slots' places.
 #include <type_traits>
 
 #include "rq_prod.h"
