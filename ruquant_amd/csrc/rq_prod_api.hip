@@ -90,10 +90,12 @@ int64_t sums_bytes(int64_t P, int64_t N, int64_t E) {
     const int64_t most = up_to(N, 128) / 128 * most_token_tiles(128, P, E) * kMostSplits * 65536;
     return (most < kMostSums ? most : kMostSums) + kMostShared * 16;
 }
-constexpr int64_t kFewEach = 4;   // positions a group, on average, up to which they are few
+// Positions a group, on average, up to which they are few: the stream reads a weight again for every 16 of its group's. (us, stream -> tiles, int8, K = 5120, N = 1280: 32 of 64
+// groups 43.1 -> 49.9; K = 512, N = 1000, 60 of 8 9.4 -> 10.4; fp16, K = 1376, N = 4096, 148 of 60 98.0 -> 98.6.) And at most so many, since one group may have them all.
+constexpr int64_t kFewEach = 4, kMostFew = 512;
 // P positions, of E groups (0: one) of which the host knows no more.
 Plan plan_product(int weight_type, int64_t K, int64_t N, int64_t P, int64_t E) {
-    Plan plan = { P <= 16 || P <= kFewEach * E, 0, -1, 0, 1, 0, 0, 0 };
+    Plan plan = { P <= 16 || (P <= kFewEach * E && P <= kMostFew), 0, -1, 0, 1, 0, 0, 0 };
     if (plan.few) return plan;
     const int64_t steps = up_to(K * type_bytes(weight_type), 64) / 64, groups = E == 0 ? 1 : P < E ? P : E;
     const double  each = (double) P / (double) groups, bytes = (double) groups * (double) (N * K * type_bytes(weight_type));

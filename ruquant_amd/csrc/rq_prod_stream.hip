@@ -5,8 +5,8 @@
 // rounded are rounded by every workgroup for itself, into LDS, while its first weights are on their way: that saves a launch, where the rows are few.
 //
 // Bound by memory where weights are large, by the chain of a load, the products and the join where they are not: one token x 5120 x 17408 in int8 17.3 us, 89 MB
-// at 5.1 TB/s, a large copy's rate; 13 x 4099 x 5121 10.3 us; 37 tokens' 111 rows of 1376 x 4096
-// in fp16, from most of 60 experts' 676 MB, 83 us. Tried:
+// at 5.1 TB/s, a large copy's rate; 13 x 4099 x 5121 10.3 us; 37 tokens' 111 rows of 1376 x 4096 in fp16, from most of 60 experts' 676 MB,
+// 83 us. Tried:
 // 16 wavefronts (2.4 times as long), 16 rows (more steps on their way, 10 to 60 % longer), 64 rows (as fast for groups, 10 to 25 % longer for one).
 #include "rq_prod.h"
 

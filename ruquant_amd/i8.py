@@ -103,6 +103,11 @@ class HalfWeight(_Weight):
         self._prepare(_DTYPES[w.dtype], w, None)
 
 
+def _described(weight):
+    shape = [getattr(weight, name, "?") for name in ("E", "N", "K")]
+    return "a %s of E=%s N=%s K=%s" % (type(weight).__name__, *shape)
+
+
 def _given(x, scales, dtype, what):
     """(type of x, default type of the output) of activations that may be int8 already, checked"""
     if x.dtype != torch.int8:
@@ -119,10 +124,9 @@ def i8_mul_mat(weight, x, scales=None, dtype=None, out=None, workspace=None):
     scales [M] is taken as it is. y = (sum * the weight's scale) * the token's scale in fp32, rounded to out's type, or to dtype
     (x's by default, fp32 for int8 x). `out` shares no memory with x."""
     M, K, ldx = _rows(x, "i8_mul_mat")
+    if not isinstance(weight, I8Weight) or weight.E != 1 or K != weight.K:
+        raise RqError("i8_mul_mat: activations of %d inputs against %s, not an I8Weight [N, %d]" % (K, _described(weight), K))
     N = weight.N
-    if weight.kind != _I8 or weight.E != 1 or K != weight.K:
-        raise RqError("i8_mul_mat: activations of %d inputs against a weight (%s) of E=%d N=%d K=%d"
-                      % (K, type(weight).__name__, weight.E, N, weight.K))
     dt, dtype = _given(x, scales, dtype, "i8_mul_mat")
     ldy = N
     if out is None:
@@ -195,9 +199,9 @@ def grouped_mul_mat(weight, x, offsets, rows=None, out_rows=None, scales=None, d
     i8_mul_mat; with 16-bit weights x has the weight's type. Sums are exact or in fp32; y is rounded to out's type, or to dtype (x's by default, fp32 for
     int8 x). `out` shares no memory with the inputs."""
     M, K, ldx = _rows(x, "grouped_mul_mat")
+    if not isinstance(weight, _Weight) or K != weight.K:
+        raise RqError("grouped_mul_mat: x of %d inputs against %s, not an I8Weight or HalfWeight [E, N, %d]" % (K, _described(weight), K))
     E, N = weight.E, weight.N
-    if K != weight.K:
-        raise RqError("grouped_mul_mat: x of %d inputs against weights of E=%d N=%d K=%d" % (K, E, N, weight.K))
     if weight.kind != _I8 and x.dtype != weight.dtype:
         raise RqError("grouped_mul_mat: x has to be of the weight's type %s, got %s" % (weight.dtype, x.dtype))
     if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous():

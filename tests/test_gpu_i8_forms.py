@@ -177,11 +177,12 @@ def test_refused_tensors():
     g = torch.Generator(device=DEV).manual_seed(3)
     W, H = rq.I8Weight(_codes((2, 40, 64), g), _scales((2, 40), g)), rq.HalfWeight(torch.ones((2, 40, 64), dtype=torch.float16, device=DEV))
     x, a, s = torch.randn((6, 64), device=DEV), _codes((6, 64), g), _scales((6,), g)
+    mx = rq.MXWeight(torch.zeros((2, 40, 32), dtype=torch.uint8, device=DEV), torch.zeros((2, 40, 2), dtype=torch.uint8, device=DEV))
     offsets, rows = torch.tensor([0, 3, 6], dtype=torch.int32, device=DEV), torch.arange(6, dtype=torch.int32, device=DEV)
     call = lambda weight=W, x=x, offsets=offsets, **k: rq.grouped_mul_mat(weight, x, offsets, **k)  # noqa: E731
     call(), call(x=a, scales=s), call(H, x.half()), call(rows=rows, out_rows=rows)
     for bad in (lambda: call(x=a), lambda: call(scales=s), lambda: call(x=a, scales=s[:5]), lambda: call(x=a, scales=s.double()), lambda: call(H), lambda: call(H, x.bfloat16()),
-                lambda: call(x=x[:, :63]), lambda: call(x=x.double()), lambda: call(offsets=offsets[:2]), lambda: call(offsets=offsets.long()), lambda: call(offsets=offsets.cpu()),
+                lambda: call(weight=mx, x=x), lambda: rq.i8_mul_mat(mx, x), lambda: call(weight=x), lambda: call(x=x[:, :63]), lambda: call(x=x.double()), lambda: call(offsets=offsets[:2]), lambda: call(offsets=offsets.long()), lambda: call(offsets=offsets.cpu()),
                 lambda: call(rows=rows.long()), lambda: call(rows=rows.view(2, 3)), lambda: call(out_rows=rows[:5]), lambda: call(rows=rows.cpu()),
                 lambda: call(out=torch.empty((6, 41), device=DEV)), lambda: call(out=torch.empty((5, 40), device=DEV)), lambda: call(out=torch.empty((40, 6), device=DEV).t()),
                 lambda: call(out=torch.empty((6, 40), dtype=torch.float64, device=DEV)), lambda: call(dtype=torch.int8), lambda: rq.i8_mul_mat(W, x), lambda: rq.i8_mul_mat(H, x.half()),
@@ -191,6 +192,24 @@ def test_refused_tensors():
                 lambda: rq.i8_quantize(x[:, :0]), lambda: rq.i8_dequantize(a, s, dtype=torch.int8)):
         with pytest.raises(rq.RqError):
             bad()
+
+
+@pytest.mark.parametrize("kind", [I8, BF16])
+@pytest.mark.parametrize("E,K,N,P", [(4, 64, 40, 300), (8, 5000, 1000, 40), (2, 64, 40, 4)])
+def test_offsets_that_overlap_stay_inside(kind, E, K, N, P):
+    """every group claims all positions: more tiles than there can be. What y holds is one group's row or another's, and nothing beside it is touched"""
+    g = torch.Generator(device=DEV).manual_seed(P)
+    offsets = torch.tensor([0, P] * ((E + 2) // 2), dtype=torch.int32, device=DEV)[:E + 1]
+    room = torch.full((P + 20, N), 7.0, device=DEV)
+    ws = torch.full((rq.load_library().rq_grouped_workspace_bytes(kind, E, K, N, P, P) + 4096,), 7, dtype=torch.uint8, device=DEV)
+    n = ws.numel() - 4096
+    if kind == I8:
+        a, s = _codes((P, K), g), _scales((P,), g)
+        rq.grouped_mul_mat(rq.I8Weight(_codes((E, N, K), g), _scales((E, N), g)), a, offsets, scales=s, out=room[10:P + 10], workspace=ws[:n])
+    else:
+        rq.grouped_mul_mat(rq.HalfWeight(torch.ones((E, N, K), dtype=torch.bfloat16, device=DEV)), torch.ones((P, K), dtype=torch.bfloat16, device=DEV), offsets,
+                           out=room[10:P + 10], workspace=ws[:n])
+    assert (ws[n:] == 7).all() and (room[:10] == 7).all() and (room[P + 10:] == 7).all()
 
 
 def test_sizes_behind_32_bits():
