@@ -52,8 +52,8 @@ struct Plan {
 };
 // The tiles' forms, and what they take in microseconds: a step of 64 bytes where every compute unit has a tile of its own, a step of 256 tiles where the chip is full
 // of them (256 x 256: 2.1 POP/s, what a large int8 library product reaches here: the chip's clock falls to that, whatever the form), what stands in front of and behind the
-// steps; and, where several workgroups share a tile, their join, per part, and per tile and part of 64 KiB. Fitted to 1000 times of K = 1024 to 17408, N = 512 to
-// 17408 and 8 to 2048 rows: what they choose is 1 % slower than the fastest of seventeen forms and shares on average, 28 % at worst.
+// steps; and, where several workgroups share a tile, their join, per part, and per tile and part of 64 KiB. Fitted to 959 times of K = 1024 to 17408, N = 512 to
+// 17408 and 8 to 2048 rows: what they choose is 1 % slower than the fastest of sixteen forms and shares on average, 13 % at worst.
 struct Form {
     int    resident;   // tiles that a compute unit holds
     double alone, full, fixed, join, part, tile;
