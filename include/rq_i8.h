@@ -43,7 +43,7 @@ int rq_weight_prepare(int type, const void *w_dev, const float *scales_dev, int6
  * sum is exact; y = ((fp32 of it) t_n) s_m, each product in fp32, rounded to out_dtype. in_dtype RQ_I8: x holds codes already and
  * x_scales their scales (else null). x: row stride ldx elements, any alignment of its type; y: row stride ldy elements, no memory of x.
  * workspace: 256-byte aligned, rq_i8_workspace_bytes (for every type and alignment; it grows with M, so the most tokens' serves all), need not be
- * initialised, not shared by calls that can overlap. */
+ * initialised, not shared by calls that can overlap; where that is 256 (few rows) it is not looked at and may be null. */
 size_t rq_i8_workspace_bytes(int64_t K, int64_t N, int64_t M);
 int rq_i8_mul_mat(const void *prepared_dev, int64_t K, int64_t N, int in_dtype, const void *x_dev, int64_t ldx, const float *x_scales_dev,
                   int64_t M, int out_dtype, void *y_dev, int64_t ldy, void *workspace_dev, size_t workspace_bytes, rq_stream_t stream);

@@ -156,10 +156,15 @@ bool stream_takes_floats(ProductArgs &a, int in_dtype, const void *x, int64_t ld
     return true;
 }
 
+// Whether a call looks at no workspace, whatever the type of x and its alignment: few rows, taken as they lie or rounded where they are used.
+bool alone(int weight_type, int64_t K, int64_t N, int64_t P, int64_t E) {
+    return plan_product(weight_type, K, N, P, E).few && (weight_type != RQ_I8 || stream_rounds(P, K, N, E) > 0);
+}
+
 int run(ProductArgs &a, const Plan &plan, int weight_type, int64_t K, int in_dtype, const void *x, int64_t ldx, const float *x_scales, int64_t M,
                uint8_t *workspace, size_t workspace_bytes, hipStream_t stream) {
     const size_t rows = act_bytes(weight_type, K, M);
-    if (workspace_bytes < rows + plan.sums_bytes + 4 * (size_t) plan.counters) return RQ_E_WORKSPACE;   // (a plan that sums_bytes does not cover)
+    if (!plan.few && workspace_bytes < rows + plan.sums_bytes + 4 * (size_t) plan.counters) return RQ_E_WORKSPACE;   // (a plan that sums_bytes does not cover)
     uint8_t *behind = workspace + rows;
     a.sums = (uint32_t *) behind;
     a.arrived = (int *) (behind + plan.sums_bytes);
@@ -171,6 +176,7 @@ int run(ProductArgs &a, const Plan &plan, int weight_type, int64_t K, int in_dty
 
 extern "C" size_t rq_i8_workspace_bytes(int64_t K, int64_t N, int64_t M) {
     if (rq_weight_prepared_bytes(RQ_I8, 1, N, K) == 0 || M < 0 || M > kMaxPositions) return 0;
+    if (alone(RQ_I8, K, N, M, 0)) return 256;   // (not looked at)
     return act_bytes(RQ_I8, K, M) + pad256(sums_bytes(M, N, 0)) + 256;
 }
 
@@ -183,7 +189,7 @@ extern "C" int rq_i8_mul_mat(const void *prepared, int64_t K, int64_t N, int in_
         (in_dtype == RQ_I8) != (x_scales != nullptr) || !aligned(x_scales, 4) || (M > 1 && (ldx < K || ldy < N))) {
         return RQ_E_ARGUMENT;
     }
-    if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return RQ_E_WORKSPACE;
+    if (!alone(RQ_I8, K, N, M, 0) && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return RQ_E_WORKSPACE;
     ProductArgs a = {};
     a.L = panels(RQ_I8, N, K);
     a.w = (const uint8_t *) prepared;
@@ -199,6 +205,7 @@ extern "C" int rq_i8_mul_mat(const void *prepared, int64_t K, int64_t N, int in_
 
 extern "C" size_t rq_grouped_workspace_bytes(int weight_type, int64_t E, int64_t K, int64_t N, int64_t M, int64_t P) {
     if (rq_weight_prepared_bytes(weight_type, E, N, K) == 0 || M < 0 || M > kMaxPositions || P < 0 || P > kMaxPositions) return 0;
+    if (alone(weight_type, K, N, P, E)) return 256;
     return act_bytes(weight_type, K, M) + pad256(sums_bytes(P, N, E)) + 256;
 }
 
@@ -215,7 +222,7 @@ extern "C" int rq_grouped_mul_mat(int weight_type, const void *prepared, int64_t
         !aligned(out_rows, 4) || (M > 1 && ldx < K) || (y_rows > 1 && ldy < N)) {
         return RQ_E_ARGUMENT;
     }
-    if (!workspace || !aligned(workspace, 256) || workspace_bytes < need) return RQ_E_WORKSPACE;
+    if (!alone(weight_type, K, N, P, E) && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return RQ_E_WORKSPACE;
     ProductArgs a = {};
     a.L = panels(weight_type, N, K);
     a.w = (const uint8_t *) prepared;

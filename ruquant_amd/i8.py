@@ -140,7 +140,7 @@ def i8_mul_mat(weight, x, scales=None, dtype=None, out=None, workspace=None):
     index = x.get_device()
     if workspace is None:
         n, at = L.rq_i8_workspace_bytes(K, N, M), None
-        if n:
+        if n > 256:   # (256: nothing that the call looks at)
             workspace = x.new_empty((n,), dtype=torch.uint8)
             at = workspace.data_ptr()
     else:
@@ -161,9 +161,9 @@ def sort_slots(ids, E, workspace=None):
         raise RqError("sort_slots: ids int32 [M, top] on the GPU, contiguous, got %s %s on %s" % (ids.dtype, tuple(ids.shape), ids.device))
     M, top = ids.shape
     L = load_library()
-    offsets = ids.new_empty((E + 1,))
-    slots = ids.new_empty((M * top,))
-    tokens = ids.new_empty((M * top,))
+    if not 1 <= E <= 1024:
+        raise RqError("sort_slots: 1 to 1024 experts, got %d" % E)
+    offsets, slots, tokens = ids.new_empty((E + 1 + 2 * M * top,)).split((E + 1, M * top, M * top))   # (one allocation: a small call is the host's time)
     n = L.rq_sort_workspace_bytes(M, top, E)
     at = None
     if workspace is None:
@@ -224,7 +224,7 @@ def grouped_mul_mat(weight, x, offsets, rows=None, out_rows=None, scales=None, d
     index = x.get_device()
     if workspace is None:
         n, at = L.rq_grouped_workspace_bytes(weight.kind, E, K, N, M, P), None
-        if n:
+        if n > 256:
             workspace = x.new_empty((n,), dtype=torch.uint8)
             at = workspace.data_ptr()
     else:

@@ -173,6 +173,30 @@ def test_a_workspace_that_is_too_small_or_has_gaps_is_refused():
     assert torch.equal(rq.grouped_mul_mat(W, x, offsets, workspace=room[:n]), rq.i8_mul_mat(W, x, workspace=room))
 
 
+def test_calls_that_look_at_no_workspace():
+    """every type and alignment of x in calls whose workspace may be null"""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    L = rq.load_library()
+    w, t = _codes((3, 40, 333), g), _scales((3, 40), g)
+    dense, W, H = rq.I8Weight(w[0], t[0]), rq.I8Weight(w, t), rq.HalfWeight(w.half())
+    offsets = torch.tensor([0, 2, 2, 5], dtype=torch.int32, device=DEV)
+    assert L.rq_i8_workspace_bytes(333, 40, 2) == rq.grouped_workspace_bytes(W, 5, 5) == rq.grouped_workspace_bytes(H, 5, 5) == 256
+    none = torch.empty(0, dtype=torch.uint8, device=DEV)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        x = torch.randn((5, 339), device=DEV, generator=g).to(dtype)[:, 3:336]
+        a, s = rq.i8_quantize(x)
+        want = torch.stack([_scaled(a[p:p + 1], w[e], s[p:p + 1], t[e])[0] for p, e in enumerate((0, 0, 2, 2, 2))])
+        for rows, scales in ((x, None), (a, s)):
+            assert torch.equal(rq.i8_mul_mat(dense, rows[:2], scales=None if scales is None else scales[:2], dtype=dtype, workspace=none), want[:2].to(dtype))
+            assert torch.equal(rq.grouped_mul_mat(W, rows, offsets, scales=scales, dtype=dtype, workspace=none), want.to(dtype))
+    x = torch.randn((5, 339), device=DEV, generator=g).half()[:, 3:336]
+    want = torch.stack([x[p].double() @ w[e].double().t().contiguous() for p, e in enumerate((0, 0, 2, 2, 2))])
+    y = rq.grouped_mul_mat(H, x, offsets, dtype=torch.float32, workspace=none)
+    # (333 products of 11 by 7 bits, exact in fp32: as in the other test, 2 (K / 16 + 48) 2^-24 of their magnitudes' sum, and a rounding)
+    size = torch.stack([x[p].double().abs() @ w[e].double().abs().t().contiguous() for p, e in enumerate((0, 0, 2, 2, 2))])
+    assert ((y.double() - want).abs() <= 2 * (333 / 16 + 49) * 2.0 ** -24 * size).all()
+
+
 def test_refused_tensors():
     g = torch.Generator(device=DEV).manual_seed(3)
     W, H = rq.I8Weight(_codes((2, 40, 64), g), _scales((2, 40), g)), rq.HalfWeight(torch.ones((2, 40, 64), dtype=torch.float16, device=DEV))

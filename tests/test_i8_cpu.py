@@ -38,13 +38,14 @@ def test_sizes():
                 (I8, 1, -1, 64), (F16, 1, 64, -1), (I8, 1, 2 ** 24 + 1, 64)):
         assert size(*bad) == 0, bad
     ws = L.rq_i8_workspace_bytes
+    assert ws(5120, 64, 1) == ws(5120, 17408, 2) == 256 and ws(5120, 64, 3) > 3 * 5120   # (256: not looked at)
     assert ws(5120, 64, 2048) >= 2048 * 5124 and ws(5120, 64, -1) == 0 and ws(0, 64, 1) == 0 and ws(64, 64, 2 ** 22 + 1) == 0
     sort = L.rq_sort_workspace_bytes
     assert sort(1, 8, 64) == 0 and sort(16384, 8, 256) > 0
     for bad in ((-1, 8, 64), (1, 0, 64), (1, 8, 0), (1, 8, 1025), (1, 1025, 8), (2 ** 22, 2, 8)):
         assert sort(*bad) == 0, bad
     group = L.rq_grouped_workspace_bytes
-    assert group(I8, 64, 5120, 1280, 2048, 16384) >= 2048 * 5124
+    assert group(I8, 64, 5120, 1280, 2048, 16384) >= 2048 * 5124 and group(I8, 64, 5120, 1280, 1, 8) == group(BF16, 64, 5120, 1280, 9, 72) == 256
     for bad in ((F32, 8, 64, 64, 1, 1), (I8, 1025, 64, 64, 1, 1), (I8, 8, 64, 64, 2 ** 22 + 1, 1), (I8, 8, 64, 64, 1, 2 ** 22 + 1),
                 (I8, 8, 64, 64, -1, 1), (I8, 8, 64, 64, 1, -1)):
         assert group(*bad) == 0, bad
@@ -85,7 +86,7 @@ def test_refusals_without_a_gpu():
     assert product(dtype=4) == product(out=I8) == product(K=131072) == product(N=0) == product(M=-1) == product(M=2 ** 22 + 1) == UNSUPPORTED
     assert product(w=None) == product(w=PTR + 128) == product(x=None) == product(x=PTR + 2) == product(xs=PTR) == product(dtype=I8) == BAD
     assert product(dtype=I8, xs=PTR + 2) == product(ldx=63) == product(ldy=63) == product(y=None) == product(out=F16, y=PTR + 1) == BAD
-    assert product(ws=None) == product(ws=PTR + 8) == product(n=16) == WORKSPACE
+    assert product(M=40, ws=None) == product(M=40, ws=PTR + 8) == product(M=40, n=16) == WORKSPACE
     assert product(M=0, x=None, ws=None) == 0
     sort = lambda ids=PTR, M=2, top=4, E=8, offsets=PTR, slots=PTR, tokens=PTR, ws=None, n=0: L.rq_sort_slots(  # noqa: E731
         ids, M, top, E, offsets, slots, tokens, ws, n, None)
@@ -98,7 +99,7 @@ def test_refusals_without_a_gpu():
     assert group(E=1025) == group(P=2 ** 22 + 1) == group(M=-1) == group(out=I8) == group(Y=-1) == group(Y=2 ** 31) == UNSUPPORTED
     assert group(w=None) == group(x=None) == group(M=0) == group(offsets=None) == group(offsets=PTR + 2) == group(rows=PTR + 1) == BAD
     assert group(places=PTR + 2) == group(xs=PTR) == group(dtype=I8) == group(ldx=63) == group(ldy=63) == group(y=None) == group(w=PTR + 16) == BAD
-    assert group(ws=None) == group(n=16) == group(ws=PTR + 64) == WORKSPACE
+    assert group(P=40, ws=None) == group(P=40, n=16) == group(P=40, ws=PTR + 64) == group(kind=F16, dtype=F16, P=40, ws=None) == WORKSPACE
     assert group(P=0, x=None) == group(Y=0, y=None) == 0
 
 
