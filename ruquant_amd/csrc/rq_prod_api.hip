@@ -93,9 +93,10 @@ int64_t sums_bytes(int64_t P, int64_t N, int64_t E) {
 // Positions a group, on average, up to which they are few: the stream reads a weight again for every 16 of its group's. (us, stream -> tiles, int8, K = 5120, N = 1280: 32 of 64
 // groups 43.1 -> 49.9; K = 512, N = 1000, 60 of 8 9.4 -> 10.4; fp16, K = 1376, N = 4096, 148 of 60 98.0 -> 98.6.) And at most so many, since one group may have them all.
 constexpr int64_t kFewEach = 4, kMostFew = 512;
+bool few_rows(int64_t P, int64_t E) { return P <= 16 || (P <= kFewEach * E && P <= kMostFew); }
 // P positions, of E groups (0: one) of which the host knows no more.
 Plan plan_product(int weight_type, int64_t K, int64_t N, int64_t P, int64_t E) {
-    Plan plan = { P <= 16 || (P <= kFewEach * E && P <= kMostFew), 0, -1, 0, 1, 0, 0, 0 };
+    Plan plan = { few_rows(P, E), 0, -1, 0, 1, 0, 0, 0 };
     if (plan.few) return plan;
     const int64_t steps = up_to(K * type_bytes(weight_type), 64) / 64, groups = E == 0 ? 1 : P < E ? P : E;
     const double  each = (double) P / (double) groups, bytes = (double) groups * (double) (N * K * type_bytes(weight_type));
@@ -158,11 +159,11 @@ bool stream_takes_floats(ProductArgs &a, int in_dtype, const void *x, int64_t ld
 
 // Whether a call looks at no workspace, whatever the type of x and its alignment: few rows, taken as they lie or rounded where they are used.
 bool alone(int weight_type, int64_t K, int64_t N, int64_t P, int64_t E) {
-    return plan_product(weight_type, K, N, P, E).few && (weight_type != RQ_I8 || stream_rounds(P, K, N, E) > 0);
+    return few_rows(P, E) && (weight_type != RQ_I8 || stream_rounds(P, K, N, E) > 0);
 }
 
 int run(ProductArgs &a, const Plan &plan, int weight_type, int64_t K, int in_dtype, const void *x, int64_t ldx, const float *x_scales, int64_t M,
-               uint8_t *workspace, size_t workspace_bytes, hipStream_t stream) {
+        uint8_t *workspace, size_t workspace_bytes, hipStream_t stream) {
     const size_t rows = act_bytes(weight_type, K, M);
     if (!plan.few && workspace_bytes < rows + plan.sums_bytes + 4 * (size_t) plan.counters) return RQ_E_WORKSPACE;   // (a plan that sums_bytes does not cover)
     uint8_t *behind = workspace + rows;
