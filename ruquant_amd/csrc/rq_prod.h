@@ -110,11 +110,11 @@ __device__ __forceinline__ int64_t row_written(const ProductArgs &a, int64_t p) 
     const int64_t r = a.out_rows[p];
     return r >= 0 && r < a.y_rows ? r : -1;
 }
-// Group e's first position and how many it has.
+// Group e's first position and how many it has. (Both ends are clamped on both sides: an offset may be any number, and the difference of two is not.)
 __device__ __forceinline__ void group(const ProductArgs &a, int e, int &first, int &count) {
     const int P = (int) a.P;
     first = min(max(a.offsets[e], 0), P);
-    count = max(min(a.offsets[e + 1], P) - first, 0);
+    count = max(min(max(a.offsets[e + 1], 0), P) - first, 0);
 }
 // Group e has units(its count) units, and all groups' stand in a row. Finds the group that has unit want(how many there are), and the place in it; all lanes
 // of a wavefront take part, with the same numbers. False where no group has it. TOTAL: `want` looks at its argument (else it is 0).
