@@ -16,6 +16,9 @@ namespace {
 
 __device__ __attribute__((aligned(16))) const uint8_t kZeros[16] = { 0 };
 
+// LDS that every launch may have, and what of it a workgroup takes beside its rows.
+constexpr int kMostLds = 65536, kFixedLds = 128;
+
 // Eight elements of a row from k on, zeros behind its end.
 template <int DT>
 __device__ __forceinline__ void load_unit(const typename Element<DT>::type *x, bool aligned, int K, int k, float (&v)[8]) {
@@ -52,6 +55,7 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ uint32_t tops[2][W];
     __shared__ float    scale_of[16];
+    static_assert(sizeof(tops) + sizeof(scale_of) <= kFixedLds, "LDS beside the rows");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
     int       e = 0, first = 0, count = (int) a.P;
     if constexpr (GROUPED) {
@@ -213,8 +217,7 @@ __global__ __launch_bounds__(64 * W) void rq_stream_kernel(const ProductArgs a) 
     }
 }
 
-constexpr int kMostLds = 65536;
-int           lds_bytes(int W, int NR, bool round, const ProductArgs &a) {
+int lds_bytes(int W, int NR, bool round, const ProductArgs &a) {
     const int T = (int) (a.P < a.chunk ? a.P : a.chunk), sums = W * NR * T * 64, rows = round ? T * (a.L.steps * 64 + 16) : 0;
     return sums > rows ? sums : rows;
 }
@@ -248,7 +251,7 @@ hipError_t stream(int weight_type, int x_type, const ProductArgs &a, hipStream_t
 int stream_rounds(int64_t P, int64_t K, int64_t N, int64_t E) {
     // (us, rounded by every workgroup -> by a launch in front: K = 5120: N = 17408 1 row 21.0 -> 23.8, 2 rows 23.1 -> 24.2, 4 26.1 -> 24.6; N = 5120 1 8.0 -> 9.9,
     // 2 9.0 -> 10.1, 4 11.0 -> 10.4; N = 1024 1 6.7 -> 9.0, 4 9.6 -> 9.4; K = 17408, N = 5120 1 22.6 -> 25.7; 8 groups of 1 row, N = 1280 17.5 -> 20.6, 16 27.7 -> 26.7)
-    const int64_t most = kMostLds / (up_to(K, 64) + 16), T = most < 16 ? most : 16;
+    const int64_t most = (kMostLds - kFixedLds) / (up_to(K, 64) + 16), T = most < 16 ? most : 16;
     if (T == 0 || P > (E ? 8 : 2)) return 0;
     return P * K * ((N + 31) / 32) <= 6000000 ? (int) (T < P ? T : P) : 0;
 }

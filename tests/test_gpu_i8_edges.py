@@ -5,10 +5,11 @@ import torch
 
 import ruquant_amd as rq
 from tests import i8_plan_util as plan
-from tests.i8_plan_util import BF16, F16, I8, STREAM, TILES
+from tests.i8_plan_util import BF16, F16, F32, I8, ROUNDS, STREAM, TILES
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+FLOATS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 LOW, HIGH = -2 ** 31, 2 ** 31 - 1
 
 
@@ -62,3 +63,21 @@ def test_offsets_of_any_number(P, form, kind):
             if i < j:
                 want[i:j] = rows(p[i:j], e)
         assert torch.equal(rq.grouped_mul_mat(weight, x, _ints(offsets), out=out, **more), want), offsets
+
+
+# ---- rows rounded by every workgroup ------------------------------------------------------------------------------------
+
+def _floats(M, K, dtype, g):
+    """rows of different magnitudes"""
+    return (torch.randn((M, K), device=DEV, generator=g) * torch.exp2(torch.arange(M, device=DEV) % 7 - 3.0)[:, None]).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", sorted(FLOATS, key=str))
+@pytest.mark.parametrize("K,N,M,form,rows", [(65344, 40, 1, ROUNDS, 1), (65345, 40, 1, STREAM, 0), (65472, 40, 1, STREAM, 0), (32640, 40, 2, ROUNDS, 2),
+                                             (32641, 40, 2, ROUNDS, 1), (32704, 40, 2, ROUNDS, 1)])
+def test_longest_rounded_rows(K, N, M, form, rows, dtype):
+    assert plan.product(K, N, M, FLOATS[dtype])[:2] == [form, rows]
+    g = torch.Generator(device=DEV).manual_seed(K + M)
+    w, t, x = _codes((N, K), g), _scales((N,), g), _floats(M, K, dtype, g)
+    a, s = rq.i8_quantize(x)
+    assert torch.equal(rq.i8_mul_mat(rq.I8Weight(w, t), x), _scaled(a, w, s, t).to(dtype))
