@@ -89,6 +89,9 @@ class I8Weight(_Weight):
         self._prepare(_I8, codes, scales.contiguous())
 
     def workspace(self, M):
+        """of i8_mul_mat, for up to M rows"""
+        if self.E != 1:
+            raise RqError("I8Weight.workspace: of a weight [N, K], not of %d experts' (grouped_workspace_bytes(weight, M, P))" % self.E)
         return _device_bytes(load_library().rq_i8_workspace_bytes(self.K, self.N, M), self.device)
 
 

@@ -36,3 +36,11 @@ def test_calls_on_both_sides_of_the_longest_rounded_row():
     assert plan.product(last + 1, 32, 1, F32)[0] == STREAM
     assert L.rq_i8_workspace_bytes(last, 32, 1) == 256 and L.rq_i8_workspace_bytes(last + 1, 32, 1) > last
     assert L.rq_grouped_workspace_bytes(I8, 8, last, 32, 1, 1) == 256 and L.rq_grouped_workspace_bytes(I8, 8, last + 1, 32, 1, 1) > last
+
+
+def test_a_dense_workspace_is_of_a_dense_weight():
+    """experts' weights have no product of their own: what their workspace takes depends on the positions too"""
+    W = object.__new__(rq.I8Weight)
+    W.E, W.N, W.K, W.device = 8, 1000, 5000, "cpu"
+    with pytest.raises(rq.RqError, match="grouped_workspace_bytes"):
+        W.workspace(40)
