@@ -160,11 +160,10 @@ __global__ __launch_bounds__(256) void rq_i8_dequantize_kernel(const int8_t *cod
     }
 }
 
-// 16 bytes a thread; experts are the grid's y and z.
+// 16 bytes a thread; experts are the grid's y.
 template <bool VEC>
-__global__ __launch_bounds__(256) void rq_weight_prepare_kernel(const uint8_t *w, const float *scales, Panels L, int64_t E, uint8_t *prepared) {
-    const int64_t e = (int64_t) blockIdx.z * gridDim.y + blockIdx.y;
-    if (e >= E) return;
+__global__ __launch_bounds__(256) void rq_weight_prepare_kernel(const uint8_t *w, const float *scales, Panels L, uint8_t *prepared) {
+    const int64_t  e = blockIdx.y;
     const uint8_t *from = w + e * L.N * L.row_bytes;
     uint8_t       *to = prepared + e * L.expert_bytes;
     const int64_t  pieces = L.code_bytes / 16, words = scales ? (int64_t) L.row_blocks * 32 : 0;
@@ -329,9 +328,9 @@ extern "C" int rq_weight_prepare(int type, const void *w, const float *scales, i
     const int64_t x = (L.expert_bytes / 16 + 255) / 256;
     const dim3    grid((unsigned) (x < 4096 ? x : 4096), (unsigned) E);
     if (aligned_to(w, 16) && L.row_bytes % 16 == 0) {
-        hipLaunchKernelGGL(rq_weight_prepare_kernel<true>, grid, dim3(256), 0, (hipStream_t) stream, (const uint8_t *) w, scales, L, E, (uint8_t *) prepared);
+        hipLaunchKernelGGL(rq_weight_prepare_kernel<true>, grid, dim3(256), 0, (hipStream_t) stream, (const uint8_t *) w, scales, L, (uint8_t *) prepared);
     } else {
-        hipLaunchKernelGGL(rq_weight_prepare_kernel<false>, grid, dim3(256), 0, (hipStream_t) stream, (const uint8_t *) w, scales, L, E, (uint8_t *) prepared);
+        hipLaunchKernelGGL(rq_weight_prepare_kernel<false>, grid, dim3(256), 0, (hipStream_t) stream, (const uint8_t *) w, scales, L, (uint8_t *) prepared);
     }
     return hipGetLastError();
 }

@@ -238,8 +238,12 @@ hipError_t stream(const ProductArgs &a, hipStream_t s) {
 }
 template <bool GROUPED>
 hipError_t stream(int weight_type, int x_type, const ProductArgs &a, hipStream_t s) {
-    if (weight_type == RQ_F16) return stream<RQ_F16, RQ_I8, GROUPED>(a, s);
-    if (weight_type == RQ_BF16) return stream<RQ_BF16, RQ_I8, GROUPED>(a, s);
+    if constexpr (GROUPED) {
+        if (weight_type == RQ_F16) return stream<RQ_F16, RQ_I8, GROUPED>(a, s);
+        if (weight_type == RQ_BF16) return stream<RQ_BF16, RQ_I8, GROUPED>(a, s);
+    } else if (weight_type != RQ_I8) {
+        return hipErrorInvalidValue;
+    }
     if (x_type == RQ_F32) return stream<RQ_I8, RQ_F32, GROUPED>(a, s);
     if (x_type == RQ_F16) return stream<RQ_I8, RQ_F16, GROUPED>(a, s);
     if (x_type == RQ_BF16) return stream<RQ_I8, RQ_BF16, GROUPED>(a, s);
