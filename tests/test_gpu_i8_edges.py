@@ -78,6 +78,251 @@ def _floats(M, K, dtype, g):
 def test_longest_rounded_rows(K, N, M, form, rows, dtype):
     assert plan.product(K, N, M, FLOATS[dtype])[:2] == [form, rows]
     g = torch.Generator(device=DEV).manual_seed(K + M)
-    w, t, x = _codes((N, K), g), _scales((N,), g), _floats(M, K, dtype, g)
+    w, t, x = _codes((N, K), g), _scales((N,), g) * K ** -0.5 / 64, _floats(M, K, dtype, g)
     a, s = rq.i8_quantize(x)
     assert torch.equal(rq.i8_mul_mat(rq.I8Weight(w, t), x), _scaled(a, w, s, t).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", sorted(FLOATS, key=str))
+@pytest.mark.parametrize("E,K,N,sizes,rows", [(0, 40000, 64, [2], 1), (8, 9280, 64, [0, 0, 8], 7), (8, 9280, 1280, [0, 0, 8], 7), (8, 9344, 64, [7, 1], 6), (8, 17408, 64, [0, 8], 3),
+                                              (8, 17408, 600, [1, 0, 6, 1], 3), (64, 40000, 40, [3, 2, 0, 3], 1), (3, 30000, 40, [3, 0, 2], 2)])
+def test_rounding_in_passes(E, K, N, sizes, rows, dtype):
+    """more rows in a group than are rounded at a time: each pass fills the place that the sums of the one before had"""
+    P = sum(sizes)
+    p = plan.grouped(I8, E, K, N, P, P, FLOATS[dtype]) if E else plan.product(K, N, P, FLOATS[dtype])
+    assert p[:2] == [ROUNDS, rows] and max(sizes) > rows
+    g = torch.Generator(device=DEV).manual_seed(K + N + P)
+    w, t, x = _codes((len(sizes), N, K), g), _scales((len(sizes), N), g) * K ** -0.5 / 64, _floats(P, K, dtype, g)
+    x[P - 1, K - 1] = float("nan")
+    a, s = rq.i8_quantize(x)
+    ends = [sum(sizes[:e]) for e in range(len(sizes) + 1)]
+    want = torch.cat([_scaled(a[i:j], w[e], s[i:j], t[e]) for e, (i, j) in enumerate(zip(ends, ends[1:]))]).to(dtype)
+    if not E:
+        y = rq.i8_mul_mat(rq.I8Weight(w[0], t[0]), x)
+    else:   # (the experts behind are asked for by nobody)
+        w, t = torch.cat([w, w[:1].expand(E - len(sizes), -1, -1)]), torch.cat([t, t[:1].expand(E - len(sizes), -1)])
+        y = rq.grouped_mul_mat(rq.I8Weight(w, t), x, _ints(ends + [P] * (E - len(sizes))))
+    assert torch.isnan(y[P - 1]).all() and torch.isfinite(y[:P - 1]).all()
+    assert torch.equal(y.nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0))
+
+
+@pytest.mark.parametrize("dtype", sorted(FLOATS, key=str))
+@pytest.mark.parametrize("K,N,chunk", [(200, 70, 8), (201, 40, 8), (9344, 40, 6), (17408, 600, 3)])
+def test_rounded_rows_that_are_not_there(K, N, chunk, dtype):
+    """... give zeros, also where the row that is read in their place is NaN, and places that are not there are not written"""
+    E, M, P = 4, 5, 8
+    assert plan.grouped(I8, E, K, N, M, P, FLOATS[dtype])[:2] == [ROUNDS, chunk]
+    g = torch.Generator(device=DEV).manual_seed(K)
+    w, t, x = _codes((E, N, K), g), _scales((E, N), g) * K ** -0.5 / 64, _floats(M, K, dtype, g)
+    x[0, 3] = float("nan")
+    rows, places, offsets = [-1, 4, M, 0, HIGH, 1, LOW, 1], [9, 0, 3, 10, 8, -1, LOW, 2], [0, 1, 1, 7, 8]
+    a, s = rq.i8_quantize(x)
+    weight, out = rq.I8Weight(w, t), torch.full((10, N), 7.0, dtype=dtype, device=DEV)
+    want = out.clone()
+    for p, (r, q) in enumerate(zip(rows, places)):
+        e = next(e for e in range(E) if offsets[e] <= p < offsets[e + 1])
+        if 0 <= q < 10:
+            want[q] = _scaled(a[r:r + 1], w[e], s[r:r + 1], t[e])[0].to(dtype) if 0 <= r < M else 0
+    given = torch.full_like(out, 7.0)
+    rq.grouped_mul_mat(weight, x, _ints(offsets), rows=_ints(rows), out_rows=_ints(places), out=out)
+    rq.grouped_mul_mat(weight, a, _ints(offsets), rows=_ints(rows), out_rows=_ints(places), scales=s, out=given)
+    assert not torch.isnan(want).any() and torch.equal(out, want) and torch.equal(given, want)
+    places[3] = 1   # (row 0 itself)
+    rq.grouped_mul_mat(weight, x, _ints(offsets), rows=_ints(rows), out_rows=_ints(places), out=out)
+    assert torch.isnan(out[1]).all() and torch.equal(out[2:], want[2:]) and torch.equal(out[0], want[0])
+
+
+# ---- the streamed form ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind,dtype", [(I8, None), (I8, torch.float32), (I8, torch.bfloat16), (F16, None), (BF16, None)])
+@pytest.mark.parametrize("sizes,behind,form", [([3, 0, 2, 1], 8, STREAM), ([2, 0, 0, 1], 4, ROUNDS), ([1, 0, 2, 0] * 5, 30, STREAM), ([17, 0, 3] + 17 * [0], 20, STREAM)])
+def test_rows_of_no_group_beside_streamed_ones(sizes, behind, form, kind, dtype):
+    E, P, K, N = len(sizes), sum(sizes) + behind, 128, 72
+    used = P - behind
+    assert plan.grouped(kind, E, K, N, P, P, kind if dtype is None else FLOATS[dtype])[0] == (form if dtype is not None else STREAM)
+    g = torch.Generator(device=DEV).manual_seed(P)
+    weight, x, more, rows = _case(kind, E, K, N, P, g)
+    if dtype is not None:
+        x, codes = _floats(P, K, dtype, g), _codes((E, N, K), g)
+        scales, more, (a, s) = _scales((E, N), g), {}, rq.i8_quantize(x)
+        weight, rows = rq.I8Weight(codes, scales), lambda m, e: _scaled(a[m], codes[e], s[m], scales[e])
+        x[used:] = float("nan")
+    elif kind != I8:
+        x[used:] = float("nan")
+    out = torch.full((P, N), 7.0, device=DEV)
+    want, at = out.clone(), 0
+    for e, n in enumerate(sizes):
+        if n:
+            want[at:at + n] = rows(torch.arange(at, at + n, device=DEV), e)
+        at += n
+    offsets = _ints([sum(sizes[:e]) for e in range(E + 1)])
+    assert torch.equal(rq.grouped_mul_mat(weight, x, offsets, out=out, **more), want)
+
+
+@pytest.mark.parametrize("kind", [I8, F16, BF16])
+@pytest.mark.parametrize("E,N,sizes", [(128, 40, {77: 512}), (128, 40, {0: 17, 5: 16, 64: 33, 65: 1, 127: 445}), (128, 700, {3: 100, 126: 412})])
+def test_few_rows_of_which_one_group_has_most(E, N, sizes, kind):
+    """16 rows of a group at a time"""
+    K, P = 200, sum(sizes.values())
+    assert plan.grouped(kind, E, K, N, P, P)[0] == STREAM
+    g = torch.Generator(device=DEV).manual_seed(N)
+    weight, x, more, rows = _case(kind, E, K, N, P, g)
+    ends, want = [0], []
+    for e in range(E):
+        n = sizes.get(e, 0)
+        if n:
+            want.append(rows(torch.arange(ends[-1], ends[-1] + n, device=DEV), e))
+        ends.append(ends[-1] + n)
+    assert torch.equal(rq.grouped_mul_mat(weight, x, _ints(ends), dtype=torch.float32, **more), torch.cat(want))
+
+
+# ---- the tiles --------------------------------------------------------------------------------------------------------------
+
+# of the plan: rows and positions of a tile, whether tiles are shared, tiles a compute unit holds; then kind, E, K, N, P that reach it
+FORMS = [((64, 64, False, 2), F16, 3, 72, 70, 130), ((64, 64, True, 2), F16, 1, 1806, 16, 18), ((128, 64, False, 2), F16, 4, 33, 8804, 25),
+         ((128, 64, True, 2), F16, 64, 3602, 70, 267), ((128, 128, False, 1), F16, 1, 301, 2389, 847), ((128, 128, False, 2), F16, 64, 32, 1003, 2339),
+         ((128, 128, True, 1), F16, 1, 4487, 449, 2084), ((256, 256, False, 1), F16, 8, 32, 5616, 1009), ((64, 64, True, 2), BF16, 1, 1806, 16, 18),
+         ((128, 64, False, 2), BF16, 4, 33, 8804, 25), ((128, 64, True, 2), BF16, 64, 3602, 70, 267), ((128, 128, False, 1), BF16, 1, 301, 2389, 847),
+         ((128, 128, False, 2), BF16, 64, 32, 1003, 2339), ((128, 128, True, 1), BF16, 1, 4487, 449, 2084), ((256, 256, False, 1), BF16, 8, 32, 5616, 1009),
+         ((64, 64, False, 2), I8, 3, 72, 70, 130), ((64, 64, True, 2), I8, 1, 3499, 17, 17), ((128, 64, False, 2), I8, 40, 42, 816, 166), ((128, 64, True, 2), I8, 64, 7879, 66, 261),
+         ((128, 128, False, 1), I8, 1, 588, 7186, 263), ((128, 128, False, 2), I8, 64, 32, 1003, 2339), ((128, 128, True, 1), I8, 1, 8744, 226, 4168),
+         ((256, 256, False, 1), I8, 4, 34, 11065, 499)]
+
+
+@pytest.mark.parametrize("form,kind,E,K,N,P", FORMS)
+def test_grouped_of_every_form_to_the_bit(form, kind, E, K, N, P):
+    """rows that are gathered, one of them not there, ragged groups, outputs in an order of their own, what the workspace held"""
+    M = P // 2 + 1
+    p = plan.grouped(kind, E, K, N, M, P)
+    assert (p[1], p[2], p[6] > 1, p[7]) == form, p
+    g = torch.Generator(device=DEV).manual_seed(K + N + P)
+    weight, x, more, rows = _case(kind, E, K, N, M, g)
+    cuts = sorted(torch.randint(0, P - 1, (E - 1,), generator=torch.Generator().manual_seed(P)).tolist())
+    ends = [0] + cuts + [P - 1]   # (the last position is no group's)
+    read = torch.randint(0, M, (P,), device=DEV, generator=g)
+    places = torch.randperm(P, device=DEV, generator=g)
+    want = torch.zeros((P, N), device=DEV)
+    for e, (i, j) in enumerate(zip(ends, ends[1:])):
+        if i < j:
+            want[places[i:j]] = rows(read[i:j], e)
+    want[places[3]], want[places[P - 1]] = 0, 7
+    read[3] = M
+    ws = torch.empty((rq.grouped_workspace_bytes(weight, M, P),), dtype=torch.uint8, device=DEV)
+    out = torch.empty((P, N), device=DEV)
+    for fill in (0, 255):
+        ws.fill_(fill), out.fill_(7)
+        rq.grouped_mul_mat(weight, x, _ints(ends), rows=read.int(), out_rows=places.int(), out=out, workspace=ws, **more)
+        assert torch.equal(out, want)
+    half = torch.full((P, N), 7.0, dtype=torch.bfloat16, device=DEV)
+    rq.grouped_mul_mat(weight, x, _ints(ends), rows=read.int(), out_rows=places.int(), out=half, **more)
+    assert torch.equal(half, want.bfloat16())
+
+
+# (rows and positions of a tile, tiles a compute unit holds), N, M, the steps of 64 bytes from which on that is the plan
+STEPS = [((64, 64, 2), 33, 17, 1), ((128, 64, 2), 16500, 65, 1), ((128, 64, 2), 16500, 17, 8), ((128, 128, 2), 16500, 200, 1), ((128, 128, 1), 16500, 65, 10), ((256, 256, 1), 16500, 400, 1)]
+
+
+@pytest.mark.parametrize("form,N,M,first", STEPS)
+def test_every_number_of_steps(form, N, M, first):
+    """rows whose last step, pair of steps and turn of the rings end anywhere; the weight and x as they lie, by one more row of x than is looked at"""
+    last = 7 if (form, M) == ((128, 64, 2), 65) else 24
+    g = torch.Generator(device=DEV).manual_seed(M)
+    for steps in range(first, last + 1):
+        K = 64 * steps
+        p = plan.product(K, N, M)
+        assert (p[1], p[2], p[7]) == form and p[6] == 1, p
+        room, w, t, s = _codes((M + 1, K), g), _codes((N, K), g), _scales((N,), g), _scales((M,), g)
+        assert torch.equal(rq.i8_mul_mat(rq.I8Weight(w, t), room[:M], scales=s), _scaled(room[:M], w, s, t)), steps
+
+
+@pytest.mark.parametrize("form,N,M,steps", [((64, 64, 2), 33, 17, range(60, 86)), ((128, 64, 2), 8200, 17, range(136, 152)), ((128, 128, 1), 8200, 65, range(136, 152))])
+def test_every_number_of_steps_of_shared_tiles(form, N, M, steps):
+    """parts of equal length but the last"""
+    g = torch.Generator(device=DEV).manual_seed(M)
+    for n in steps:
+        K = 64 * n - 5
+        p = plan.product(K, N, M)
+        assert (p[1], p[2], p[7]) == form and p[6] > 1, p
+        a, w, t, s = _codes((M, K), g), _codes((N, K), g), _scales((N,), g), _scales((M,), g)
+        assert torch.equal(rq.i8_mul_mat(rq.I8Weight(w, t), a, scales=s), _scaled(a, w, s, t)), n
+
+
+# ---- both -------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [I8, F16, BF16])
+@pytest.mark.parametrize("P,form", [(9, STREAM), (300, TILES)])
+def test_one_row_read_by_all_and_one_written(P, form, kind):
+    E, K, N = 2, 65, 33
+    assert plan.grouped(kind, E, K, N, 1, P)[0] == form
+    g = torch.Generator(device=DEV).manual_seed(P)
+    weight, x, more, rows = _case(kind, E, K, N, 1, g)
+    want = torch.cat([rows(torch.zeros(n, dtype=torch.long, device=DEV), e) for e, n in enumerate((P // 3, P - P // 3))])
+    offsets, read = _ints([0, P // 3, P]), torch.zeros(P, dtype=torch.int32, device=DEV)
+    assert torch.equal(rq.grouped_mul_mat(weight, x, offsets, rows=read, dtype=torch.float32, **more), want)
+    places = torch.full((P,), -1, dtype=torch.int32, device=DEV)
+    places[P - 2], places[1] = 0, 1
+    out = torch.full((1, N), 7.0, device=DEV)
+    assert torch.equal(rq.grouped_mul_mat(weight, x, offsets, rows=read, out_rows=places, out=out, **more), want[P - 2:P - 1])
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("P,form", [(9, STREAM), (200, TILES)])
+def test_an_infinity_or_nan_in_16_bits_stays_its_rows_own(P, form, kind):
+    E, K, N = 1, 72, 40
+    assert plan.grouped(kind, E, K, N, P, P)[0] == form
+    g = torch.Generator(device=DEV).manual_seed(P)
+    weight, x, _, rows = _case(kind, E, K, N, P, g)
+    want = rows(torch.arange(P, device=DEV), 0)
+    x[2, 71], x[P - 1, 0] = float("nan"), float("inf")
+    y = rq.grouped_mul_mat(weight, x, _ints([0, P]), dtype=torch.float32)
+    assert torch.isnan(y[2]).all() and not torch.isfinite(y[P - 1]).any()
+    y[2], y[P - 1] = want[2], want[P - 1]
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("kind,least", [(F16, -24), (BF16, -133)])
+@pytest.mark.parametrize("P,form", [(9, STREAM), (200, TILES)])
+def test_the_smallest_numbers_of_16_bits_count(P, form, kind, least):
+    """numbers below the type's normal ones, in either operand, against whole numbers (powers of two: every product and sum is exact in fp32)"""
+    E, K, N = 1, 72, 40
+    assert plan.grouped(kind, E, K, N, P, P)[0] == form
+    g = torch.Generator(device=DEV).manual_seed(P)
+    dtype = torch.float16 if kind == F16 else torch.bfloat16
+    x, w = _small((P, K), g), _small((E, N, K), g)
+    want = x.double() @ w[0].double().t().contiguous()
+    tiny = lambda v: (v.double() * 2.0 ** least).to(dtype)  # noqa: E731
+    for big, a, b in ((2.0 ** 10, tiny(x), (w * 2.0 ** 10).to(dtype)), (2.0 ** 10, (x * 2.0 ** 10).to(dtype), tiny(w))):
+        y = rq.grouped_mul_mat(rq.HalfWeight(b), a, _ints([0, P]), dtype=torch.float32)
+        assert torch.equal(y.double(), want * 2.0 ** least * big)
+
+
+# ---- a layer's products, each to the bit ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,absent", [(1, False), (2, True), (5, False), (50, True), (400, False)])
+def test_products_of_a_layer_are_the_definition(M, absent, dtype):
+    """route, sort, up where the tokens lie, an activation, down to the slots' places; slots whose expert is not here give zeros in a buffer of zeros"""
+    E, K, F, top = 12, 256, 96, 3
+    g = torch.Generator(device=DEV).manual_seed(M)
+    up, down = ((_codes((E, n, k), g), _scales((E, n), g) * k ** -0.5 / 64) for n, k in ((F, K), (K, F)))
+    x = _floats(M, K, dtype, g)
+    ids, shares = rq.route(torch.randn((M, E), device=DEV, generator=g), top)
+    if absent:
+        ids = torch.where(torch.arange(M * top, device=DEV).view(M, top) % 4 == 1, -1, ids).contiguous()
+    offsets, slots, tokens = rq.sort_slots(ids, E)
+    experts, here = ids.flatten().long(), ids.flatten() >= 0
+    h = rq.grouped_mul_mat(rq.I8Weight(*up), x, offsets, rows=tokens, out=torch.zeros((M * top, F), dtype=dtype, device=DEV))
+    a, s = rq.i8_quantize(x)
+    want = torch.zeros((M * top, F), dtype=dtype, device=DEV)   # (by slot)
+    for i in here.nonzero().flatten().tolist():
+        m, e = i // top, experts[i]
+        want[i] = _scaled(a[m:m + 1], up[0][e], s[m:m + 1], up[1][e])[0].to(dtype)
+    assert torch.equal(h, want[slots.long()])
+    h = torch.relu(h)
+    y = rq.grouped_mul_mat(rq.I8Weight(*down), h, offsets, out_rows=slots, out=torch.zeros((M * top, K), device=DEV))
+    a, s = rq.i8_quantize(torch.relu(want))
+    want = torch.zeros((M * top, K), device=DEV)
+    for i in here.nonzero().flatten().tolist():
+        want[i] = _scaled(a[i:i + 1], down[0][experts[i]], s[i:i + 1], down[1][experts[i]])[0]
+    assert torch.equal(y, want)
+    assert torch.isfinite((y.view(M, top, K) * shares[:, :, None]).sum(dim=1)).all()
