@@ -326,3 +326,62 @@ def test_products_of_a_layer_are_the_definition(M, absent, dtype):
         want[i] = _scaled(a[i:i + 1], down[0][experts[i]], s[i:i + 1], down[1][experts[i]])[0]
     assert torch.equal(y, want)
     assert torch.isfinite((y.view(M, top, K) * shares[:, :, None]).sum(dim=1)).all()
+
+
+# ---- sort, and sizes that take several launches --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("E", [1, 63, 64, 65, 1023, 1024])
+@pytest.mark.parametrize("M,top", [(2048, 1), (2049, 1), (1, 1024), (131072, 1), (131073, 1), (2 ** 22, 1), (2 ** 21, 2)])
+def test_sort_on_both_sides_of_its_runs(M, top, E):
+    """one run and two, the last of the short runs and the first long ones, the most slots of a call"""
+    g = torch.Generator(device=DEV).manual_seed(E + M)
+    ids = torch.randint(-1, E + 1, (M, top), dtype=torch.int32, device=DEV, generator=g)
+    expert = torch.where(ids.flatten() < 0, E, ids.flatten())
+    order = expert.sort(stable=True)
+    ends = torch.searchsorted(order.values, torch.arange(E + 1, device=DEV, dtype=torch.int32))
+    n = rq.load_library().rq_sort_workspace_bytes(M, top, E)
+    assert (n == 0) == (M * top <= 2048)
+    ws = torch.full((max(n, 1),), 255, dtype=torch.uint8, device=DEV)
+    for workspace in (None, ws[:n]):
+        offsets, slots, tokens = rq.sort_slots(ids, E, workspace=workspace)
+        assert torch.equal(offsets, ends.int()) and torch.equal(slots, order.indices.int()) and torch.equal(tokens, slots // top)
+
+
+def test_quantiser_of_more_rows_than_a_launch_has():
+    """2^24 rows of up to 2048 inputs are one launch"""
+    M, K = 2 ** 24 + 5, 3
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn((M, K), device=DEV, generator=g)
+    codes, scales = rq.i8_quantize(x)
+    some = torch.tensor([0, 1, 2 ** 24 - 1, 2 ** 24, 2 ** 24 + 1, M - 1], device=DEV)
+    a, s = rq.i8_quantize(x[some])
+    assert torch.equal(codes[some], a) and torch.equal(scales[some], s)
+    assert torch.equal(scales, torch.maximum(x.abs().amax(dim=1) * torch.tensor(1 / 127, device=DEV), torch.tensor(2.0 ** -126, device=DEV)))
+    assert ((rq.i8_dequantize(codes, scales) - x).abs() <= scales[:, None] * 0.5001).all()
+
+
+def test_dequantiser_of_more_elements_than_a_launch_has():
+    """2^31 runs of eight elements are one launch"""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    M = 2 ** 31 + 7
+    codes = torch.full((M, 1), 3, dtype=torch.int8, device=DEV)
+    codes[2 ** 31:] = -5
+    out = rq.i8_dequantize(codes, torch.full((M,), 0.5, device=DEV), dtype=torch.float16)
+    assert bool((out[:2 ** 31] == 1.5).all()) and bool((out[2 ** 31:] == -2.5).all())
+
+
+def test_rows_brought_to_16_bytes_in_several_launches():
+    """rows at odd addresses, more of them than one launch moves, read by few positions in tiles"""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    M, K, N, P = 140001, 131071, 24, 40
+    assert plan.grouped(I8, 1, K, N, M, P)[0] == TILES
+    g = torch.Generator(device=DEV).manual_seed(3)
+    a = torch.zeros((M, K), dtype=torch.int8, device=DEV)
+    some = torch.tensor([0, 1, 65536, 130000, 131007, 131008, 131071, 131072, M - 2, M - 1], device=DEV)
+    a[some] = _codes((10, K), g)
+    w, t, s = _codes((N, K), g), _scales((N,), g), _scales((M,), g)
+    read = some.repeat(4)
+    y = rq.grouped_mul_mat(rq.I8Weight(w[None], t[None]), a, _ints([0, P]), rows=read.int(), scales=s)
+    assert torch.equal(y, _scaled(a[read], w, s[read], t))
