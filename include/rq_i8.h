@@ -60,7 +60,8 @@ int rq_sort_slots(const int32_t *ids_dev, int64_t M, int top, int64_t E, int32_t
  *   y[q(p)] = W_e x[r(p)],  r(p) = rows[p], or p where rows is null; q(p) = out_rows[p], or p where out_rows is null.
  * weight_type RQ_I8: x rounded and products scaled as by rq_i8_mul_mat, x of any float type or given as codes (in_dtype RQ_I8 with x_scales,
  * one for each of the M rows of x). RQ_F16, RQ_BF16: x of the weight's type; sums in fp32, rounded once to out_dtype.
- * x has M rows, y y_rows. Offsets are clamped to 0 .. P; a group whose end is not behind its start is empty, and groups do not overlap. An index of rows
+ * x has M rows (one at least where there are positions), y y_rows. Offsets are any numbers and are clamped to 0 .. P; a group whose end is not behind its start is empty, and groups
+ * do not overlap (a row of y that several would write holds one group's product or another's, or is left as it was). An index of rows
  * outside 0 .. M - 1 gives a row of zeros; one of out_rows outside 0 .. y_rows - 1 is not written, and no index of out_rows comes twice. Rows
  * of y that no position writes are left as they were. Sizes that the device alone knows (the groups') shape no launch. y shares no memory with the
  * inputs. Workspace as above: rq_grouped_workspace_bytes serves every type and alignment of x and grows with M and P. */

@@ -53,7 +53,9 @@ struct Plan {
 // The tiles' forms, and what they take in microseconds: a step of 64 bytes where every compute unit has a tile of its own, a step of 256 tiles where the chip is full
 // of them (256 x 256: 2.1 POP/s, what a large int8 library product reaches here: the chip's clock falls to that, whatever the form), what stands in front of and behind the
 // steps; and, where several workgroups share a tile, their join, per part, and per tile and part of 64 KiB. Fitted to 959 times of K = 1024 to 17408, N = 512 to
-// 17408 and 8 to 2048 rows: what they choose is 1 % slower than the fastest of sixteen forms and shares on average, 13 % at worst.
+// 17408 and 8 to 2048 rows of int8 in one group: what they choose is 1 % slower than the fastest of sixteen forms and shares on average, 13 % at worst. Groups and 16-bit weights go
+// by the same prices, as if all groups had as many rows: over 47 calls of 4 to 64 routed experts (int8, fp16, bf16, K and N = 256 to 5100, 22 to 1939 tokens) 2 % on average and 11 %
+// at worst behind the fastest of the five forms.
 struct Form {
     int    resident;   // tiles that a compute unit holds
     double alone, full, fixed, join, part, tile;
@@ -91,7 +93,8 @@ int64_t sums_bytes(int64_t P, int64_t N, int64_t E) {
     return (most < kMostSums ? most : kMostSums) + kMostShared * 16;
 }
 // Positions a group, on average, up to which they are few: the stream reads a weight again for every 16 of its group's. (us, stream -> tiles, int8, K = 5120, N = 1280: 32 of 64
-// groups 43.1 -> 49.9; K = 512, N = 1000, 60 of 8 9.4 -> 10.4; fp16, K = 1376, N = 4096, 148 of 60 98.0 -> 98.6.) And at most so many, since one group may have them all.
+// groups 43.1 -> 49.9; K = 512, N = 1000, 60 of 8 9.4 -> 10.4; fp16, K = 1376, N = 4096, 148 of 60 98.0 -> 98.6; K = 5120, N = 1280, 512 rows routed to 128 int8 142 -> 145, bf16 265 -> 266,
+// 256 to 64 76 -> 82 and 140 -> 145.) And at most so many, since one group may have them all: 512 rows in one of 128 184 -> 27 and 308 -> 32, 256 in one of 64 94 -> 22.
 constexpr int64_t kFewEach = 4, kMostFew = 512;
 bool few_rows(int64_t P, int64_t E) { return P <= 16 || (P <= kFewEach * E && P <= kMostFew); }
 // P positions, of E groups (0: one) of which the host knows no more.

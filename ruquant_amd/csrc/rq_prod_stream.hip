@@ -4,9 +4,10 @@
 // split the row's bytes, each with DEPTH steps of 64 bytes on their way, and join their sums in LDS in their order. Rows of x that are still to be
 // rounded are rounded by every workgroup for itself, into LDS, while its first weights are on their way: that saves a launch, where the rows are few.
 //
-// Bound by memory where weights are large, by the chain of a load, the products and the join where they are not: one token x 5120 x 17408 in int8 17.3 us, 89 MB
-// at 5.1 TB/s, a large copy's rate; 13 x 4099 x 5121 10.3 us; 37 tokens' 111 rows of 1376 x 4096 in fp16, from most of 60 experts' 676 MB,
-// 83 us. Tried:
+// Bound by memory where weights are large, by the chain of a load, the products and the join where they are not. The kernel's own time, two weights in turn: one token x 5120 x 17408
+// in int8 17.2 us, 89 MB at 5.1 TB/s, a large copy's rate (21.4 a call in a graph of calls, the next one's start among them); 13 x 4099 x 5121 10.3 us; 37 tokens' 111 rows of
+// 1376 x 4096 in fp16, from 40 to 49 of 60 experts, 452 to 554 MB, 91 us. A group's rows go 16 at a time, one pass over its weight each: 512 rows x 5120 x 1280 in int8 184 us
+// where one of 128 experts has them all, 159 where all have four. Tried:
 // 16 wavefronts (2.4 times as long), 16 rows (more steps on their way, 10 to 60 % longer), 64 rows (as fast for groups, 10 to 25 % longer for one).
 #include "rq_prod.h"
 
@@ -253,8 +254,10 @@ hipError_t stream(int weight_type, int x_type, const ProductArgs &a, hipStream_t
 }  // namespace
 
 int stream_rounds(int64_t P, int64_t K, int64_t N, int64_t E) {
-    // (us, rounded by every workgroup -> by a launch in front: K = 5120: N = 17408 1 row 21.0 -> 23.8, 2 rows 23.1 -> 24.2, 4 26.1 -> 24.6; N = 5120 1 8.0 -> 9.9,
-    // 2 9.0 -> 10.1, 4 11.0 -> 10.4; N = 1024 1 6.7 -> 9.0, 4 9.6 -> 9.4; K = 17408, N = 5120 1 22.6 -> 25.7; 8 groups of 1 row, N = 1280 17.5 -> 20.6, 16 27.7 -> 26.7)
+    // (us a call in graphs of calls, weights from memory, rounded by every workgroup -> by a launch in front: K = 5120: N = 17408 1 row 21.4 -> 24.1, 2 rows 22.6 to 25.3 -> 25.1,
+    // 4 28.3 -> 25.2; N = 5120 1 8.2 -> 10.4, 2 9.3 -> 10.6, 4 11.3 -> 10.7; N = 1024 1 6.7 -> 8.7, 2 7.7 -> 9.1, 4 9.7 -> 9.3; N = 30000 1 31.2 -> 33.6, 2 37.2 -> 32.4; N = 60000 1
+    // 62.8 -> 58.2; K = 17408, N = 5120 1 23.5 -> 24.6; groups of 1 row, K = 5120, N = 1280: 8 13.1 -> 15.8, 16 22.6 -> 23.0; K = 1280, N = 5120 16 23.0 -> 22.6; that it stops at
+    // eight rows costs some of those behind: 12 groups 16.7 -> 19.1, 16 of K = 2048, N = 512 6.8 -> 9.2)
     const int64_t most = (kMostLds - kFixedLds) / (up_to(K, 64) + 16), T = most < 16 ? most : 16;
     if (T == 0 || P > (E ? 8 : 2)) return 0;
     return P * K * ((N + 31) / 32) <= 6000000 ? (int) (T < P ? T : P) : 0;

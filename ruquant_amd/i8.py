@@ -196,7 +196,8 @@ def grouped_mul_mat(weight, x, offsets, rows=None, out_rows=None, scales=None, d
     where p itself stands for rows[p] or out_rows[p] if that is None. rows (int32 [P]) lets positions read tokens where they lie, out_rows
     (int32 [P], no row twice) write to the slots' places; without rows P is the number of x's rows. An index of rows outside x gives zeros, one
     of out_rows outside `out` is not written. Rows of `out` that no position writes are left as they were (so undefined where the call makes
-    `out`, [P, N]): among them, without out_rows, those from offsets[E] on.
+    `out`, [P, N]): among them, without out_rows, those from offsets[E] on, and with sort_slots' slots for out_rows those of experts that are not
+    here; an `out` of zeros keeps them out of later sums.
 
     With int8 weights x in fp32, fp16 or bf16 is rounded as by i8_quantize, int8 x with its scales is taken as it is, and products are scaled as by
     i8_mul_mat; with 16-bit weights x has the weight's type. Sums are exact or in fp32; y is rounded to out's type, or to dtype (x's by default, fp32 for
