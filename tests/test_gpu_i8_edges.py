@@ -385,3 +385,61 @@ def test_rows_brought_to_16_bytes_in_several_launches():
     read = some.repeat(4)
     y = rq.grouped_mul_mat(rq.I8Weight(w[None], t[None]), a, _ints([0, P]), rows=read.int(), scales=s)
     assert torch.equal(y, _scaled(a[read], w, s[read], t))
+
+
+# ---- the smallest sizes, strides of given codes, graphs ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [I8, F16, BF16])
+@pytest.mark.parametrize("K", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33])
+def test_smallest_sizes(K, kind):
+    g = torch.Generator(device=DEV).manual_seed(K)
+    for P, form in ((1, STREAM), (5, STREAM), (40, TILES)):
+        for N in (1, 2, 33):
+            assert plan.grouped(kind, 2, K, N, P, P)[0] == form
+            weight, x, more, rows = _case(kind, 2, K, N, P, g)
+            want = torch.cat([rows(torch.arange(0, P // 2, device=DEV), 0), rows(torch.arange(P // 2, P, device=DEV), 1)])
+            assert torch.equal(rq.grouped_mul_mat(weight, x, _ints([0, P // 2, P]), dtype=torch.float32, **more), want)
+
+
+@pytest.mark.parametrize("P,form", [(12, STREAM), (90, TILES)])
+@pytest.mark.parametrize("K,offset,ld", [(192, 0, 208), (192, 1, 208), (192, 16, 193), (187, 3, 197), (5, 1, 5)])
+def test_groups_of_given_codes_at_any_address(K, offset, ld, P, form):
+    E, N, M = 3, 50, P + 3
+    assert plan.grouped(I8, E, K, N, M, P)[0] == form
+    g = torch.Generator(device=DEV).manual_seed(K + ld)
+    room = _codes((M * ld + 64,), g)
+    a, w, s, t = room.as_strided((M, K), (ld, 1), offset), _codes((E, N, K), g), _scales((M,), g), _scales((E, N), g)
+    read = torch.randint(0, M, (P,), device=DEV, generator=g)
+    ends = [0, P // 4, P // 4, P]
+    want = torch.cat([_scaled(a[read[i:j]], w[e], s[read[i:j]], t[e]) for e, (i, j) in enumerate(zip(ends, ends[1:]))])
+    assert torch.equal(rq.grouped_mul_mat(rq.I8Weight(w, t), a, _ints(ends), rows=read.int(), scales=s), want)
+
+
+@pytest.mark.parametrize("kind,E,K,N,P", [(F16, 64, 3602, 70, 267), (I8, 64, 7879, 66, 261), (I8, 8, 200, 70, 8)])
+def test_captured_groups_whose_sizes_change(kind, E, K, N, P):
+    """shared tiles, and rows few: one graph, other offsets at every replay, another call on the same workspace between"""
+    p = plan.grouped(kind, E, K, N, P, P)
+    assert p[6] > 1 or p[0] == STREAM
+    g = torch.Generator(device=DEV).manual_seed(P)
+    weight, x, more, rows = _case(kind, E, K, N, P, g)
+    offsets, out = _ints([0] * (E + 1)), torch.zeros((P, N), device=DEV)
+    ws = torch.empty((rq.grouped_workspace_bytes(weight, P, P),), dtype=torch.uint8, device=DEV)
+    rq.grouped_mul_mat(weight, x, offsets, out=out, workspace=ws, **more)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rq.grouped_mul_mat(weight, x, offsets, out=out, workspace=ws, **more)
+    for turn in range(6):
+        pick = torch.Generator().manual_seed(turn)
+        cuts = [0] * (E - 1) if turn == 0 else [P] * (E - 1) if turn == 1 else sorted(torch.randint(0, P + 1, (E - 1,), generator=pick).tolist())
+        ends = [0] + cuts + [P]
+        want = torch.full((P, N), 7.0, device=DEV)
+        for e, (i, j) in enumerate(zip(ends, ends[1:])):
+            if i < j:
+                want[i:j] = rows(torch.arange(i, j, device=DEV), e)
+        offsets.copy_(_ints(ends)), out.fill_(7), ws.fill_(255 * (turn & 1))
+        graph.replay()
+        assert torch.equal(out, want), turn
+        out.fill_(7)
+        rq.grouped_mul_mat(weight, x, offsets, out=out, workspace=ws, **more)
+        assert torch.equal(out, want), turn
